@@ -122,12 +122,16 @@ def prepare(case, seed):
     return s
 
 
+def _wide(x):
+    """Rows of a few values in 64 bits (at two of them dx is what is left of a difference of 1e5 times its size)."""
+    return x.double() if x.shape[-1] <= 32 else x.float()
+
+
 def _plain_norm(x, w, b):
-    x = x.float()
     d = x - x.mean(-1, keepdim=True)
     rstd = torch.rsqrt((d * d).mean(-1, keepdim=True) + EPS_NORM)
     xhat = d * rstd
-    return xhat * w.float() + b.float(), xhat, rstd
+    return xhat * w + b, xhat, rstd
 
 
 def _plain_orth(x):
@@ -153,11 +157,11 @@ def _plain(s):
     case = s["case"]
     if case["op"] == "norm":
         x, w = s["x"], s["w"]
-        y, xhat, rstd = _plain_norm(x, w, s["b"])
+        y, xhat, rstd = _plain_norm(_wide(x), w.float(), s["b"].float())
         y = y.to(x.dtype)
         if not case["train"]:
             return y
-        dy = s["dy"].float()
+        dy = _wide(s["dy"])
         g = dy * w.float()
         dx = rstd * (g - g.mean(-1, keepdim=True) - xhat * (g * xhat).mean(-1, keepdim=True))
         return {"y": y, "dx": dx.to(x.dtype), "dw": (dy * xhat).sum(0).to(w.dtype), "db": dy.sum(0).to(w.dtype)}
