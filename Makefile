@@ -50,6 +50,9 @@ $(BUILD)/conv_wino.o: CXXFLAGS += -fno-slp-vectorize
 $(BUILD)/wgrad_wino.o: CXXFLAGS += -fno-slp-vectorize
 $(BUILD)/wgbd_wino.o: CXXFLAGS += -fno-slp-vectorize
 
+# plain float code in these is kept out of the packed f32 forms
+$(BUILD)/layernorm.o $(BUILD)/muon.o: CXXFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
+
 $(LIB): $(OBJ)
 	$(HIPCC) -shared --offload-arch=$(ARCH) -o $@ $(OBJ)
 

@@ -90,6 +90,27 @@ int pcx_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int64
                   float lr, float beta1, float beta2, float eps, float weight_decay,
                   float grad_scale, hipStream_t stream);
 
+/* ------------------------------------------------------------------ element types
+ * of the operators that take more than float32 */
+#define PCX_F32 0
+#define PCX_BF16 1
+#define PCX_F16 2
+
+/* ------------------------------------------------------------------ layer norm (last axis)
+ * x: `rows` rows of D values (1 <= D <= 32768), x_stride elements apart; y, dx: [rows][D] contiguous.
+ * w, b: [D] in x's type or in float32 (wdtype), NULL for 1 and 0.
+ *   y = (x - mean) / sqrt(var + eps) * w + b        (biased variance)
+ * Statistics, sums and products are in float32 (rows of up to 32 values: float64); each output is rounded once.
+ * The forward writes stats [rows][2] = {mean, 1 / sqrt(var + eps)} for the backward, or keeps nothing when it is
+ * NULL (rows of up to 32 values never write it: the backward forms them from x).  The backward computes any of
+ * dx, dw = sum_rows dy xhat and db = sum_rows dy (NULL: not wanted; dw, db in wdtype; workspace needed for them).
+ * Deterministic. */
+size_t pcx_layernorm_workspace_bytes(int dtype, int64_t rows, int64_t D);
+int pcx_layernorm_forward(int dtype, int wdtype, int64_t rows, int64_t D, const void* x, int64_t x_stride,
+                          const void* w, const void* b, float eps, void* y, float* stats, hipStream_t stream);
+int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64_t D, const void* x, int64_t x_stride,
+                           const void* w, float eps, const float* stats, const void* dy, int64_t dy_stride,
+                           void* dx, void* dw, void* db, void* ws, size_t ws_bytes, hipStream_t stream);
 
 /* ------------------------------------------------------------------ whole-network plans
  * A plan fixes the network configuration and the input shape [B, 1, F, T]; it owns no device

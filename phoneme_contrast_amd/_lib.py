@@ -3,6 +3,7 @@
 This is the one place Python touches the native library.  Nothing here falls back to a CPU or
 PyTorch implementation: a missing library, a CPU tensor or a failing kernel raises.
 """
+import contextlib
 import ctypes
 import os
 import threading
@@ -21,6 +22,8 @@ PCX_EHIP = -3
 PCX_EWORKSPACE = -5
 
 REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PCX_F32 / PCX_BF16 / PCX_F16
 
 _lock = threading.Lock()
 _lib = None
@@ -62,6 +65,11 @@ SIGNATURES = {
                                          c_float, c_void_p, c_void_p, c_void_p, c_size, c_void_p]),
     "pcx_adam_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_float,
                               c_float, c_float, c_float, c_float, c_float, c_void_p]),
+    "pcx_layernorm_workspace_bytes": (c_size, [c_int, c_i64, c_i64]),
+    "pcx_layernorm_forward": (c_int, [c_int, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_void_p, c_float,
+                                      c_void_p, c_void_p, c_void_p]),
+    "pcx_layernorm_backward": (c_int, [c_int, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_float, c_void_p,
+                                       c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_size, c_void_p]),
     "pcx_net_create": (c_void_p, [ctypes.POINTER(NetConfig), c_i64, c_i64, c_i64]),
     "pcx_net_destroy": (None, [c_void_p]),
     "pcx_net_workspace_bytes": (c_size, [c_void_p]),
@@ -152,6 +160,13 @@ def ptr(t):
 
 def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def on_device(t):
+    """Context in which t's device is the current one (kernels are launched on its stream)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def require_gpu(*tensors, what="phoneme_contrast_amd"):

@@ -365,6 +365,29 @@ int launch_proj_fwd(ProjArgs a, hipStream_t s);
 int launch_proj_bwd(ProjArgs a, hipStream_t s);
 int launch_transpose(const float* in, float* out, int rows, int cols, hipStream_t s);
 
+// ------------------------------------------------------------------ layer norm (layernorm.hip)
+struct LayerNormArgs {
+    int dtype, wdtype;     // PCX_F32 / PCX_BF16 / PCX_F16; wdtype: dtype or PCX_F32
+    int64_t rows;
+    int D;
+    float eps;
+    const void* x;
+    int64_t xs;            // row stride (elements)
+    const void* w;         // [D] or NULL
+    const void* b;         // [D] or NULL
+    void* y;               // [rows][D]
+    float* stat;           // [rows][2] mean, 1 / sqrt(var + eps)
+    const void* dy;
+    int64_t dys;
+    void* dx;              // [rows][D] or NULL
+    void* dw;              // [D] or NULL
+    void* db;              // [D] or NULL
+    void* ws;              // layernorm_bwd_ws bytes
+};
+size_t layernorm_bwd_ws(int64_t rows, int D, int es);
+int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s);
+int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s);
+
 // out[r] = sum_c part[r][c] (float64, fixed order)
 int launch_row_sum(const float* part, int rows, int64_t cols, float* out, hipStream_t s);
 

@@ -1,0 +1,609 @@
+// Layer norm over the last axis, forward and backward.
+//
+//   mean = sum_d x / D          var = sum_d (x - mean)^2 / D          rstd = 1 / sqrt(var + eps)
+//   xhat = (x - mean) rstd      y = xhat w + b
+//   g = dy w   c1 = sum_d g / D   c2 = sum_d g xhat / D   dx = rstd (g - c1 - xhat c2)
+//   dw = sum_rows dy xhat       db = sum_rows dy
+//
+// Both passes are bound by HBM: 2 tensors move in the forward, 3 in the backward.  A row is read once and stays in
+// registers between its two reductions (the variance is summed about the mean, not from squares: no cancellation for
+// rows far from zero), and the backward sums dw / db over the rows of its block in registers, so x and dy are read
+// once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
+//
+// A row belongs to 1 ... 64 lanes of a wave, to a block of 256 threads or to one of 1024 (the fewest that leave a
+// thread at most 32 values): sub-wave rows need no barrier, and wider ones one barrier per reduction.  Rows of up to
+// 32 values are computed in 64 bits from x itself: at D = 2 the three terms of dx cancel to eps / (var + eps) of
+// their size, which 32-bit statistics do not resolve, and such rows are short of bytes, not of arithmetic.
+#include "kernels.h"
+
+#include <type_traits>
+
+namespace pcx {
+namespace {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+constexpr int LN_MAX = 32768;    // 1024 threads x 32 values
+constexpr int LN_NARROW = 32;    // rows up to here: 64-bit arithmetic, one value per lane
+
+struct LnArgs {
+    int64_t rows;
+    int D, tpr, wf32;            // tpr: lanes of a sub-wave row; wf32: w and b are float32 (else x's type)
+    float eps;
+    const void* x;
+    int64_t xs;                  // row strides in elements
+    const void* w;               // readable rows of D values even without weights (hw, hb: 1 and 0 in their place)
+    const void* b;
+    bool hw, hb;
+    void* y;
+    float2* stat;                // [rows] {mean, rstd}; NULL: not kept
+    const void* dy;
+    int64_t dys;
+    void* dx;                    // NULL: not wanted
+    float* part;                 // [blocks][2][D] partial dw, db; NULL: not wanted
+};
+
+template <typename T, int V> struct Pack {
+    typedef T type __attribute__((ext_vector_type(V)));
+};
+template <typename T> struct Pack<T, 1> {
+    typedef T type;
+};
+
+template <int V, typename T> __device__ __forceinline__ void load_v(const T* p, float* v) {
+    if constexpr (V == 1) {
+        v[0] = (float)p[0];
+    } else {
+        constexpr int N = V * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;  // (float weights of 16-bit rows: two loads)
+#pragma unroll
+        for (int k = 0; k < V / N; ++k) {
+            const typename Pack<T, N>::type t = *reinterpret_cast<const typename Pack<T, N>::type*>(p + k * N);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[k * N + j] = (float)t[j];
+        }
+    }
+}
+template <int V, typename T> __device__ __forceinline__ void store_v(T* p, const float* v) {
+    if constexpr (V == 1) {
+        p[0] = (T)v[0];
+    } else {
+        typename Pack<T, V>::type t;
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = (T)v[j];
+        *reinterpret_cast<typename Pack<T, V>::type*>(p) = t;
+    }
+}
+// V weights; without any the pointer is some readable row of the same length, and the values are not used
+template <int V, typename W> __device__ __forceinline__ void load_w(const void* w, bool has, int d, float* v, float none) {
+    load_v<V>(static_cast<const W*>(w) + d, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = has ? v[j] : none;
+}
+
+// sums over the lanes of a row; BLOCK = 0: tpr lanes of a wave, else the whole block through `red` (one barrier; the
+// caller alternates between two `red` buffers, so a buffer is rewritten only behind the other's barrier)
+template <int BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float (*red)[16]) {
+    if constexpr (BLOCK == 0) {
+        for (int o = tpr >> 1; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) red[i][threadIdx.x >> 6] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < BLOCK / 64; ++w) s += red[i][w];
+            v[i] = s;
+        }
+    }
+}
+
+template <typename T, int V, int E, int BLOCK>
+__global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_fwd_kernel(LnArgs a) {
+    constexpr int NC = E / V;
+    __shared__ float red[2][1][16];
+    const int tpr = BLOCK ? BLOCK : a.tpr;
+    const int lane = threadIdx.x & (tpr - 1);
+    const int rpb = (BLOCK ? BLOCK : 256) / tpr;
+    const float invd = 1.f / (float)a.D;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
+        const int64_t r = r0 + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
+        const bool on = r < a.rows;  // (a whole sub-wave row; the others of its wave go on)
+        const T* x = static_cast<const T*>(a.x) + (on ? r : 0) * a.xs;
+        float v[NC][V];
+        float s[1] = {0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (lane + c * tpr) * V;
+            if (on && d < a.D) load_v<V>(x + d, v[c]);
+            else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[c][j] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[0] += v[c][j];
+        row_sum<BLOCK, 1>(s, tpr, red[0]);
+        const float mean = s[0] * invd;
+        s[0] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if ((lane + c * tpr) * V < a.D) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    v[c][j] -= mean;
+                    s[0] = fmaf(v[c][j], v[c][j], s[0]);
+                }
+            }
+        }
+        row_sum<BLOCK, 1>(s, tpr, red[1]);
+        const float rstd = 1.f / sqrtf(fmaf(s[0], invd, a.eps));
+        if (!on) continue;
+        T* y = static_cast<T*>(a.y) + r * a.D;
+        auto finish = [&](auto kind) {
+            using W = decltype(kind);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = (lane + c * tpr) * V;
+                if (d < a.D) {
+                    float w[V], b[V];
+                    load_w<V, W>(a.w, a.hw, d, w, 1.f);
+                    load_w<V, W>(a.b, a.hb, d, b, 0.f);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[j], b[j]);
+                    store_v<V>(y + d, v[c]);
+                }
+                if constexpr (V == 1)  // (single values: few weights in flight, or the registers spill)
+                    if (c % 4 == 3) asm volatile("" ::: "memory");
+            }
+        };
+        if (a.wf32) finish(float());
+        else finish(T());
+        if (a.stat && lane == 0) a.stat[r] = make_float2(mean, rstd);
+    }
+}
+
+template <typename T, int V, int E, int BLOCK>
+__global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(LnArgs a) {
+    constexpr int NC = E / V;
+    constexpr bool COLS = E <= 16;  // (32 values a thread leave no registers for two sums each: ln_long_cols_kernel)
+    __shared__ float red[2][2][16];
+    extern __shared__ __attribute__((aligned(16))) float cols[];  // sub-wave rows: [4 waves][D] of dw, then of db
+    const int tpr = BLOCK ? BLOCK : a.tpr;
+    const int lane = threadIdx.x & (tpr - 1);
+    const int rpb = (BLOCK ? BLOCK : 256) / tpr;
+    const float invd = 1.f / (float)a.D;
+    float sw[NC][V], sb[NC][V], w[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = (lane + c * tpr) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sw[c][j] = sb[c][j] = w[c][j] = 0.f;
+        if (d < a.D) {
+            if (a.wf32) load_w<V, float>(a.w, a.hw, d, w[c], 1.f);
+            else load_w<V, T>(a.w, a.hw, d, w[c], 1.f);
+        }
+    }
+    int par = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
+        const int64_t r = r0 + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
+        const bool on = r < a.rows;
+        const T* x = static_cast<const T*>(a.x) + (on ? r : 0) * a.xs;
+        const T* dy = static_cast<const T*>(a.dy) + (on ? r : 0) * a.dys;
+        const float2 st = on ? a.stat[r] : make_float2(0.f, 0.f);
+        float xh[NC][V], g[NC][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (lane + c * tpr) * V;
+            if (on && d < a.D) {
+                load_v<V>(x + d, xh[c]);
+                load_v<V>(dy + d, g[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    xh[c][j] = st.x;
+                    g[c][j] = 0.f;
+                }
+            }
+        }
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                xh[c][j] = (xh[c][j] - st.x) * st.y;
+                if constexpr (COLS) {
+                    sb[c][j] += g[c][j];
+                    sw[c][j] = fmaf(g[c][j], xh[c][j], sw[c][j]);
+                }
+                g[c][j] *= w[c][j];
+                s[0] += g[c][j];
+                s[1] = fmaf(g[c][j], xh[c][j], s[1]);
+            }
+        if (!a.dx) continue;  // (the same for the whole grid)
+        row_sum<BLOCK, 2>(s, tpr, red[par]);
+        par ^= 1;
+        const float c1 = s[0] * invd, c2 = s[1] * invd;
+        if (!on) continue;
+        T* dx = static_cast<T*>(a.dx) + r * a.D;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (lane + c * tpr) * V;
+            if (d < a.D) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[c][j] = st.y * (g[c][j] - fmaf(xh[c][j], c2, c1));
+                store_v<V>(dx + d, g[c]);
+            }
+        }
+    }
+    if (!COLS || !a.part) return;
+    float* pw = a.part + (int64_t)blockIdx.x * 2 * a.D;
+    if constexpr (BLOCK != 0) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (lane + c * tpr) * V;
+            if (d < a.D) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    pw[d + j] = sw[c][j];
+                    pw[a.D + d + j] = sb[c][j];
+                }
+            }
+        }
+    } else {
+        // the wave's rows, then the block's four waves, in lane and wave order
+        float* cw = cols + (threadIdx.x >> 6) * a.D;
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = (lane + c * tpr) * V;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float t = pass ? sb[c][j] : sw[c][j];
+                    for (int o = tpr; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+                    if ((threadIdx.x & 63) < (unsigned)tpr && d < a.D) cw[d + j] = t;
+                }
+            }
+            __syncthreads();
+            for (int d = threadIdx.x; d < a.D; d += 256)
+                pw[pass * a.D + d] = (cols[d] + cols[a.D + d]) + (cols[2 * a.D + d] + cols[3 * a.D + d]);
+            __syncthreads();
+        }
+    }
+}
+
+// Rows of up to 32 values in 64 bits, one value per lane (tpr = the power of two at or above D).
+template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow_kernel(LnArgs a) {
+    __shared__ double cols[4][LN_NARROW];
+    const int tpr = a.tpr, d = threadIdx.x & (tpr - 1), rpb = 256 / tpr;
+    const bool in = d < a.D;
+    float wf[1] = {0.f}, bf[1] = {0.f};
+    if (in) {
+        if (a.wf32) {
+            load_w<1, float>(a.w, a.hw, d, wf, 1.f);
+            load_w<1, float>(a.b, a.hb, d, bf, 0.f);
+        } else {
+            load_w<1, T>(a.w, a.hw, d, wf, 1.f);
+            load_w<1, T>(a.b, a.hb, d, bf, 0.f);
+        }
+    }
+    double sw = 0., sb = 0.;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
+        const int64_t r = r0 + (int)(threadIdx.x / (unsigned)tpr);
+        const bool on = in && r < a.rows;
+        const double x = on ? (double)(float)static_cast<const T*>(a.x)[r * a.xs + d] : 0.;
+        double s = x;
+        for (int o = tpr >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        const double u = on ? x - s / a.D : 0.;
+        s = u * u;
+        for (int o = tpr >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        const double rstd = 1. / sqrt(s / a.D + (double)a.eps), xh = u * rstd;
+        if constexpr (!BWD) {
+            if (on) static_cast<T*>(a.y)[r * a.D + d] = (T)(float)(xh * wf[0] + bf[0]);
+        } else {
+            const double dy = on ? (double)(float)static_cast<const T*>(a.dy)[r * a.dys + d] : 0.;
+            sb += dy;
+            sw += dy * xh;
+            const double g = dy * wf[0];
+            double c1 = g, c2 = g * xh;
+            for (int o = tpr >> 1; o > 0; o >>= 1) {
+                c1 += __shfl_xor(c1, o, 64);
+                c2 += __shfl_xor(c2, o, 64);
+            }
+            if (on && a.dx) static_cast<T*>(a.dx)[r * a.D + d] = (T)(float)(rstd * (g - c1 / a.D - xh * (c2 / a.D)));
+        }
+    }
+    if constexpr (BWD) {
+        if (!a.part) return;
+        float* pw = a.part + (int64_t)blockIdx.x * 2 * a.D;
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass) {
+            double t = pass ? sb : sw;
+            for (int o = tpr; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+            if ((threadIdx.x & 63) < (unsigned)tpr && in) cols[threadIdx.x >> 6][d] = t;
+            __syncthreads();
+            if (threadIdx.x < (unsigned)a.D)
+                pw[pass * a.D + threadIdx.x] = (float)((cols[0][threadIdx.x] + cols[1][threadIdx.x]) +
+                                                       (cols[2][threadIdx.x] + cols[3][threadIdx.x]));
+            __syncthreads();
+        }
+    }
+}
+
+// partial dw, db of rows of more than 16384 values: a thread owns a column, a block a slab of rows
+template <typename T> __global__ __launch_bounds__(256) void ln_long_cols_kernel(LnArgs a, int64_t slab) {
+    const int d = blockIdx.x * 256 + threadIdx.x;
+    if (d >= a.D) return;
+    const int64_t r0 = blockIdx.y * slab, r1 = r0 + slab < a.rows ? r0 + slab : a.rows;
+    float sw = 0.f, sb = 0.f;
+    for (int64_t r = r0; r < r1; ++r) {
+        const float2 st = a.stat[r];
+        const float g = (float)static_cast<const T*>(a.dy)[r * a.dys + d];
+        sb += g;
+        sw = fmaf(g, ((float)static_cast<const T*>(a.x)[r * a.xs + d] - st.x) * st.y, sw);
+    }
+    float* pw = a.part + (int64_t)blockIdx.y * 2 * a.D;
+    pw[d] = sw;
+    pw[a.D + d] = sb;
+}
+
+// dw, db from the blocks' partials: 32 columns x 32 slices of blocks per thread block, summed in slice order
+template <typename T> __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* __restrict__ part, int nblk, int D,
+                                                                            T* __restrict__ dw, T* __restrict__ db) {
+    __shared__ float red[32][33];
+    const int c = threadIdx.x & 31, sl = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c;  // of 2 D
+    float s = 0.f;
+    if (col < 2 * (int64_t)D)
+        for (int k = sl; k < nblk; k += 32) s += part[(int64_t)k * 2 * D + col];
+    red[sl][c] = s;
+    __syncthreads();
+    if (sl == 0 && col < 2 * (int64_t)D) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) s += red[k][c];
+        T* out = col < D ? dw : db;
+        if (out) out[col < D ? col : col - D] = (T)s;
+    }
+}
+
+// ---------------------------------------------------------------- host
+struct LnPick {
+    int tpr, ept, block;  // block 0: sub-wave rows
+};
+
+// the fewest threads that leave at most 32 values to each -- 16 in the backward, which holds two sums per column, and
+// 8 without 16-byte loads, where each value has an address of its own in flight
+LnPick ln_pick(int D, int V, bool bwd) {
+    LnPick p{64, V, 0};
+    if (D <= 64 * V) {
+        while (p.tpr > 1 && (p.tpr / 2) * V >= D) p.tpr /= 2;
+        return p;
+    }
+    const int cap = V == 1 ? 8 : bwd ? 16 : 32;
+    for (int e = 8; e <= cap; e *= 2)
+        if (D <= 64 * e) return {64, e, 0};
+    for (int e = 8; e <= cap; e *= 2)
+        if (D <= 256 * e) return {256, e, 256};
+    return {1024, D <= 1024 * 16 ? 16 : 32, 1024};
+}
+
+// blocks of the backward's row pass: its partial sums are 8 D bytes per block, written and read once, next to the
+// rows' own 3 tensors; two blocks per CU unless a block would get fewer than 8 passes of rows
+int ln_bwd_blocks(int64_t rows, int D, int V) {
+    const bool narrow = D <= LN_NARROW;
+    int rpb, cap;
+    if (narrow) {
+        int tpr = 1;
+        while (tpr < D) tpr *= 2;
+        rpb = 256 / tpr;
+        cap = 256;
+    } else {
+        const LnPick p = ln_pick(D, V, true);
+        rpb = p.block ? 1 : 256 / p.tpr;
+        cap = p.block == 1024 ? 256 : 512;
+    }
+    const int64_t passes = (rows + rpb - 1) / rpb;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(cap, (passes + 7) / 8));
+}
+
+template <typename T, int V, int E, int BLOCK, bool BWD> int ln_go(const LnArgs& a, int blocks, hipStream_t s) {
+    if constexpr (BWD) {
+        const size_t sm = BLOCK == 0 && a.part ? (size_t)4 * a.D * sizeof(float) : 0;
+        if constexpr (E > 16) {
+            if (a.part) {
+                const int64_t slab = (a.rows + blocks - 1) / blocks;
+                ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
+                PCX_LAUNCH_CHECK("ln_long_cols_kernel");
+            }
+            if (!a.dx) return PCX_OK;
+        }
+        ln_bwd_kernel<T, V, E, BLOCK><<<blocks, BLOCK ? BLOCK : 256, sm, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_bwd_kernel");
+    } else {
+        ln_fwd_kernel<T, V, E, BLOCK><<<blocks, BLOCK ? BLOCK : 256, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_fwd_kernel");
+    }
+    return PCX_OK;
+}
+
+template <typename T, int V, bool BWD> int ln_dispatch(LnArgs a, int blocks, hipStream_t s) {
+    const LnPick p = ln_pick(a.D, V, BWD);
+    a.tpr = p.tpr;
+    if (p.block == 0) {
+        if (p.ept == V) return ln_go<T, V, V, 0, BWD>(a, blocks, s);
+        if constexpr (V < 8)
+            if (p.ept == 8) return ln_go<T, V, 8, 0, BWD>(a, blocks, s);
+        if constexpr (V > 1)
+            if (p.ept == 16) return ln_go<T, V, 16, 0, BWD>(a, blocks, s);
+        if constexpr (V > 1 && !BWD) return ln_go<T, V, 32, 0, BWD>(a, blocks, s);
+    }
+    if (p.block == 256) {
+        if constexpr (V == 1 || BWD)
+            if (p.ept == 8) return ln_go<T, V, 8, 256, BWD>(a, blocks, s);
+        if constexpr (V > 1)
+            if (p.ept == 16) return ln_go<T, V, 16, 256, BWD>(a, blocks, s);
+        if constexpr (V > 1 && !BWD) return ln_go<T, V, 32, 256, BWD>(a, blocks, s);
+    }
+    if constexpr (V == 1 || BWD)
+        if (p.ept == 16) return ln_go<T, V, 16, 1024, BWD>(a, blocks, s);
+    return ln_go<T, V, 32, 1024, BWD>(a, blocks, s);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// 16-byte loads and stores of a row need rows, weights and strides on 16-byte boundaries
+template <typename T> int ln_run(LnArgs a, bool bwd, int blocks1, int blocksv, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (a.D <= LN_NARROW) {
+        a.tpr = 1;
+        while (a.tpr < a.D) a.tpr *= 2;
+        if (bwd) ln_narrow_kernel<T, true><<<blocks1, 256, 0, s>>>(a);
+        else ln_narrow_kernel<T, false><<<blocks1, 256, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_narrow_kernel");
+        return PCX_OK;
+    }
+    if (blocksv) return bwd ? ln_dispatch<T, V, true>(a, blocksv, s) : ln_dispatch<T, V, false>(a, blocksv, s);
+    return bwd ? ln_dispatch<T, 1, true>(a, blocks1, s) : ln_dispatch<T, 1, false>(a, blocks1, s);
+}
+
+int ln_dtype_size(int dtype) { return dtype == PCX_F32 ? 4 : dtype == PCX_BF16 || dtype == PCX_F16 ? 2 : 0; }
+
+bool ln_vectors(const LnArgs& a, int es) {
+    const int V = 16 / es;
+    return a.D > LN_NARROW && a.D % V == 0 && a.xs % V == 0 && a.dys % V == 0 && aligned16(a.x) && aligned16(a.y) &&
+           aligned16(a.dy) && aligned16(a.dx) && aligned16(a.w) && aligned16(a.b);
+}
+
+}  // namespace
+
+size_t layernorm_bwd_ws(int64_t rows, int D, int es) {
+    if (rows <= 0 || D <= 0) return 0;
+    const int n = std::max(ln_bwd_blocks(rows, D, 1), ln_bwd_blocks(rows, D, 16 / es));
+    return (size_t)n * 2 * D * sizeof(float);
+}
+
+LnArgs ln_args(const LayerNormArgs& q) {
+    LnArgs a{};
+    a.rows = q.rows;
+    a.D = q.D;
+    a.eps = q.eps;
+    a.x = q.x;
+    a.xs = q.xs;
+    a.hw = q.w != nullptr;
+    a.hb = q.b != nullptr;
+    a.wf32 = (a.hw || a.hb) && q.wdtype == PCX_F32;
+    a.w = q.w ? q.w : q.b ? q.b : q.x;
+    a.b = q.b ? q.b : a.w;
+    a.y = q.y;
+    a.stat = reinterpret_cast<float2*>(q.stat);
+    a.dy = q.dy;
+    a.dys = q.dys;
+    a.dx = q.dx;
+    return a;
+}
+
+int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s) {
+    const LnArgs a = ln_args(q);
+    const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
+    int rpb = 1;
+    if (a.D <= LN_NARROW) {
+        int tpr = 1;
+        while (tpr < a.D) tpr *= 2;
+        rpb = 256 / tpr;
+    } else {
+        const LnPick p = ln_pick(a.D, V, false);
+        rpb = p.block ? 1 : 256 / p.tpr;
+    }
+    const int blocks = (int)std::min<int64_t>(1 << 20, (a.rows + rpb - 1) / rpb);
+    const int bv = V > 1 ? blocks : 0;
+    if (q.dtype == PCX_F32) return ln_run<float>(a, false, blocks, bv, s);
+    if (q.dtype == PCX_BF16) return ln_run<bf16>(a, false, blocks, bv, s);
+    return ln_run<f16>(a, false, blocks, bv, s);
+}
+
+int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s) {
+    LnArgs a = ln_args(q);
+    a.part = q.dw || q.db ? static_cast<float*>(q.ws) : nullptr;
+    const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
+    const int blocks = ln_bwd_blocks(a.rows, a.D, V);
+    const int bv = V > 1 ? blocks : 0;
+    int rc = q.dtype == PCX_F32 ? ln_run<float>(a, true, blocks, bv, s)
+             : q.dtype == PCX_BF16 ? ln_run<bf16>(a, true, blocks, bv, s)
+                                   : ln_run<f16>(a, true, blocks, bv, s);
+    if (rc || !a.part) return rc;
+    const int cb = ceil_div(2 * (int64_t)a.D, 32);
+    if (q.wdtype == PCX_F32)
+        ln_cols_kernel<float><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<float*>(q.dw), static_cast<float*>(q.db));
+    else if (q.wdtype == PCX_BF16)
+        ln_cols_kernel<bf16><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<bf16*>(q.dw), static_cast<bf16*>(q.db));
+    else
+        ln_cols_kernel<f16><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<f16*>(q.dw), static_cast<f16*>(q.db));
+    PCX_LAUNCH_CHECK("ln_cols_kernel");
+    return PCX_OK;
+}
+
+}  // namespace pcx
+
+using namespace pcx;
+
+static int ln_check(const char* what, int dtype, int wdtype, int64_t rows, int64_t D, int64_t xs, float eps) {
+    PCX_CHECK_ARG(ln_dtype_size(dtype) != 0, "%s: unknown element type %d", what, dtype);
+    PCX_CHECK_ARG(wdtype == dtype || wdtype == PCX_F32, "%s: weight and bias must have the input's type or be float32", what);
+    PCX_CHECK_ARG(rows >= 0 && D >= 1 && D <= LN_MAX, "%s: rows of 1 to %d values supported (got %lld x %lld)", what, LN_MAX,
+                  (long long)rows, (long long)D);
+    PCX_CHECK_ARG(xs >= D || rows <= 1, "%s: row stride %lld below the row length %lld", what, (long long)xs, (long long)D);
+    PCX_CHECK_ARG(eps > 0.f && eps < 1e30f, "%s: eps must be positive (got %g)", what, (double)eps);
+    return PCX_OK;
+}
+
+extern "C" size_t pcx_layernorm_workspace_bytes(int dtype, int64_t rows, int64_t D) {
+    const int es = ln_dtype_size(dtype);
+    if (!es || rows < 0 || D < 1 || D > LN_MAX) return 0;
+    return layernorm_bwd_ws(rows, (int)D, es);
+}
+
+extern "C" int pcx_layernorm_forward(int dtype, int wdtype, int64_t rows, int64_t D, const void* x, int64_t x_stride,
+                                     const void* w, const void* b, float eps, void* y, float* stats, hipStream_t stream) {
+    int rc = ln_check("layernorm_forward", dtype, wdtype, rows, D, x_stride, eps);
+    if (rc) return rc;
+    if (rows == 0) return PCX_OK;
+    PCX_CHECK_ARG(x && y, "layernorm_forward: NULL buffer");
+    LayerNormArgs q{};
+    q.dtype = dtype; q.wdtype = wdtype; q.rows = rows; q.D = (int)D; q.eps = eps;
+    q.x = x; q.xs = x_stride; q.w = w; q.b = b; q.y = y; q.stat = stats;
+    return launch_layernorm_fwd(q, stream);
+}
+
+extern "C" int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64_t D, const void* x, int64_t x_stride,
+                                      const void* w, float eps, const float* stats, const void* dy, int64_t dy_stride,
+                                      void* dx, void* dw, void* db, void* ws, size_t ws_bytes, hipStream_t stream) {
+    int rc = ln_check("layernorm_backward", dtype, wdtype, rows, D, x_stride, eps);
+    if (rc) return rc;
+    PCX_CHECK_ARG(dy_stride >= D || rows <= 1, "layernorm_backward: gradient row stride below the row length");
+    PCX_CHECK_ARG(rows >= 1, "layernorm_backward: no rows");
+    PCX_CHECK_ARG(x && dy && stats, "layernorm_backward: NULL buffer");
+    if (!dx && !dw && !db) return PCX_OK;
+    if ((dw || db) && (!ws || ws_bytes < pcx_layernorm_workspace_bytes(dtype, rows, D))) {
+        set_error("layernorm_backward: workspace of %zu bytes, %zu needed", ws_bytes,
+                  pcx_layernorm_workspace_bytes(dtype, rows, D));
+        return PCX_EWORKSPACE;
+    }
+    LayerNormArgs q{};
+    q.dtype = dtype; q.wdtype = wdtype; q.rows = rows; q.D = (int)D; q.eps = eps;
+    q.x = x; q.xs = x_stride; q.w = w; q.stat = const_cast<float*>(stats); q.dy = dy; q.dys = dy_stride;
+    q.dx = dx; q.dw = dw; q.db = db; q.ws = ws;
+    return launch_layernorm_bwd(q, stream);
+}

@@ -1,0 +1,33 @@
+"""Argument checks of the layer norm on the CPU: nothing is launched."""
+import pytest
+import torch
+
+
+def test_cpu_tensors_are_refused():
+    from phoneme_contrast_amd.layers import LayerNorm, layer_norm
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        layer_norm(torch.randn(2, 8), 8)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        LayerNorm(8)(torch.randn(2, 8))
+
+
+def test_c_entry_points_refuse_before_any_launch():
+    from phoneme_contrast_amd import _lib
+    lib = _lib.lib()
+    buf = 4096  # any non-NULL address: refused before it is looked at
+
+    def fwd(dt=0, wdt=0, rows=4, D=8, x=buf, xs=8, eps=1e-5, y=buf):
+        return lib.pcx_layernorm_forward(dt, wdt, rows, D, x, xs, None, None, eps, y, None, None)
+
+    def bwd(dt=0, wdt=0, rows=4, D=8, xs=8, dys=8, stats=buf, dx=buf, dw=buf, ws=buf, nws=1 << 20, eps=1e-5):
+        return lib.pcx_layernorm_backward(dt, wdt, rows, D, buf, xs, None, eps, stats, buf, dys, dx, dw, None, ws, nws, None)
+    for rc in (fwd(dt=3), fwd(dt=-1), fwd(dt=0, wdt=1), fwd(dt=1, wdt=2), fwd(rows=-1), fwd(D=0), fwd(D=32769), fwd(x=None),
+               fwd(y=None), fwd(xs=7), fwd(eps=0.0), fwd(eps=-1.0), fwd(eps=float("nan")), fwd(eps=float("inf")),
+               bwd(dt=7), bwd(rows=0), bwd(xs=3), bwd(dys=7), bwd(stats=None), bwd(D=40000)):
+        assert rc == _lib.PCX_EINVAL and _lib.last_error()
+    assert bwd(ws=None) == _lib.PCX_EWORKSPACE
+    assert bwd(nws=8) == _lib.PCX_EWORKSPACE and "needed" in _lib.last_error()
+    assert fwd(rows=0) == _lib.PCX_OK          # nothing to do
+    assert bwd(dx=None, dw=None) == _lib.PCX_OK
+    assert lib.pcx_layernorm_workspace_bytes(0, 4096, 128) > 0
+    assert lib.pcx_layernorm_workspace_bytes(0, 4096, 1 << 20) == 0 and lib.pcx_layernorm_workspace_bytes(9, 4, 8) == 0
