@@ -25,6 +25,7 @@ REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # PCX_F32 / PCX_BF16 / PCX_F16
 
+_HERE_ALREADY = contextlib.nullcontext()
 _lock = threading.Lock()
 _lib = None
 
@@ -162,10 +163,16 @@ def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
+def raw_stream(t):
+    """The current stream of t's device as the integer handle (stream_of without the wrapper objects: 0.3 instead of
+    2 us, for calls that are over in a few)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def on_device(t):
     """Context in which t's device is the current one (kernels are launched on its stream)."""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE_ALREADY
     return torch.cuda.device(t.device)
 
 

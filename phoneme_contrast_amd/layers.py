@@ -5,6 +5,8 @@ differentiable (csrc/layernorm.hip: one kernel forward, two backward, float32 st
 rounded once, results that repeat bit by bit).  The networks use the same kernels for the projection head's
 `projection_norm: layer` (phoneme_contrast_amd.models).  There is no CPU path: a CPU tensor raises.
 """
+import functools
+import math
 import numbers
 
 import torch
@@ -29,10 +31,13 @@ def _rows(t, D):
     return v, rows, max(v.stride(0), D)
 
 
+def _address(t):
+    return t.data_ptr() if t is not None else None
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, D, eps):
-        lib = _lib.lib()
         xr, rows, xs = _rows(x, D)
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         wt = weight if weight is not None else bias
@@ -42,36 +47,50 @@ class _LayerNormFn(torch.autograd.Function):
         b = bias.contiguous() if bias is not None else None
         stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
         with _lib.on_device(x):
-            _lib.check(lib.pcx_layernorm_forward(dt, wdt, rows, D, _lib.ptr(xr), xs, _lib.ptr(w), _lib.ptr(b), eps,
-                                                 _lib.ptr(y), _lib.ptr(stats), _lib.stream_of(x)),
+            _lib.check(_lib.lib().pcx_layernorm_forward(dt, wdt, rows, D, xr.data_ptr(), xs, _address(w), _address(b),
+                                                        eps, y.data_ptr(), _address(stats), _lib.raw_stream(x)),
                        "pcx_layernorm_forward")
         ctx.save_for_backward(x, w, stats)
-        ctx.cfg = (D, eps, dt, wdt, None if weight is None else weight.shape, None if bias is None else bias.shape,
+        ctx.cfg = (D, eps, dt, wdt, weight is not None, None if wt is None else wt.shape,
                    None if wt is None else wt.dtype)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, stats = ctx.saved_tensors
-        D, eps, dt, wdt, wshape, bshape, wtype = ctx.cfg
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        lib = _lib.lib()
-        xr, rows, xs = _rows(x, D)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(wshape, dtype=wtype, device=x.device) if need_w else None
-        db = torch.empty(bshape, dtype=wtype, device=x.device) if need_b else None
-        if rows == 0:
-            return dx, (dw.zero_() if need_w else None), (db.zero_() if need_b else None), None, None
-        dyr, _, ds = _rows(dy, D)
-        nws = lib.pcx_layernorm_workspace_bytes(dt, rows, D)
-        ws = _lib.workspace(nws, x.device) if need_w or need_b else None
-        with _lib.on_device(x):
-            _lib.check(lib.pcx_layernorm_backward(dt, wdt, rows, D, _lib.ptr(xr), xs, _lib.ptr(w), eps,
-                                                  _lib.ptr(stats), _lib.ptr(dyr), ds, _lib.ptr(dx), _lib.ptr(dw),
-                                                  _lib.ptr(db), _lib.ptr(ws), nws if ws is not None else 0,
-                                                  _lib.stream_of(x)), "pcx_layernorm_backward")
-        return dx, dw, db, None, None
+        if torch.is_grad_enabled():  # create_graph: the gradient itself is not differentiable, and says so if asked
+            return _layernorm_backward_once(ctx, dy)
+        return _layernorm_backward(ctx, dy)
+
+
+def _layernorm_backward(ctx, dy):
+    x, w, stats = ctx.saved_tensors
+    D, eps, dt, wdt, has_w, wshape, wtype = ctx.cfg
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    xr, rows, xs = _rows(x, D)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+    dw = torch.empty(wshape, dtype=wtype, device=x.device) if need_w else None
+    db = torch.empty(wshape, dtype=wtype, device=x.device) if need_b else None
+    if rows == 0:
+        return dx, (dw.zero_() if need_w else None), (db.zero_() if need_b else None), None, None
+    dyr, _, ds = _rows(dy, D)
+    ws, nws = None, 0
+    if need_w or need_b:
+        nws = _workspace_bytes(dt, rows, D)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    with _lib.on_device(x):
+        _lib.check(_lib.lib().pcx_layernorm_backward(dt, wdt, rows, D, xr.data_ptr(), xs, _address(w), eps,
+                                                     stats.data_ptr(), dyr.data_ptr(), ds, _address(dx), _address(dw),
+                                                     _address(db), _address(ws), nws, _lib.raw_stream(x)),
+                   "pcx_layernorm_backward")
+    return dx, dw, db, None, None
+
+
+_layernorm_backward_once = torch.autograd.function.once_differentiable(_layernorm_backward)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(dt, rows, D):
+    return _lib.lib().pcx_layernorm_workspace_bytes(dt, rows, D)
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
@@ -84,17 +103,15 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     _lib.require_gpu(x, weight, bias, what="layer_norm")
     if x.dtype not in _lib.DTYPES:
         raise ValueError(f"layer_norm: float32, bfloat16 or float16 expected, got {x.dtype}")
-    if not shape or tuple(x.shape[-len(shape):]) != shape or len(shape) > x.dim():
+    if not shape or x.shape[-len(shape):] != shape:
         raise ValueError(f"layer_norm: input of shape {tuple(x.shape)} does not end in {shape}")
-    D = 1
-    for n in shape:
-        D *= n
+    D = math.prod(shape)
     if not 1 <= D <= MAX_DIM:
         raise ValueError(f"layer_norm: rows of 1 to {MAX_DIM} values supported, got {shape}")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"layer_norm: {name} of shape {tuple(t.shape)}, {shape} expected")
         if t.dtype not in (x.dtype, torch.float32):
             raise ValueError(f"layer_norm: {name} must be {x.dtype} or float32, got {t.dtype}")
