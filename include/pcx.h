@@ -112,6 +112,42 @@ int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64_t D, const
                            const void* w, float eps, const float* stats, const void* dy, int64_t dy_stride,
                            void* dx, void* dw, void* db, void* ws, size_t ws_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------------ orthogonalised updates
+ * Newton-Schulz iteration: X = u / (|u|_F + eps), transposed where it has more rows than columns; then, for each of
+ * `steps` triples (a, b, c) of coef (host memory), A = X X^T and X <- a X + (b A + c A A) X.  Products of operands
+ * held to 22 bits or more, summed in float32; sums of squares in float64.  Coefficients that take some singular value
+ * in [0, 1] beyond 8 are refused.  The short side is at most 16384, the long one 2^20, a matrix 2^31 values.
+ * Deterministic.
+ *
+ * pcx_orthogonalize: `batch` matrices [rows][cols] of one type, any strides (in elements) -> out [batch][rows][cols].
+ * pcx_muon_step: for every matrix of the list (float32, contiguous, none twice)
+ *   momentum <- mu momentum + (1 - mu) grad_scale grad
+ *   u = nesterov ? (1 - mu) grad_scale grad + mu momentum : momentum
+ *   param <- (1 - lr weight_decay) param - lr scale orthogonalized(u)
+ * pcx_adam_segments: pcx_adam_step on segments [offset, offset + n) of p, g and m and [v_offset, v_offset + n) of v
+ * (any alignment, none overlapping). */
+typedef struct pcx_muon_matrix {
+    float* param;
+    const float* grad;
+    float* momentum;
+    int64_t rows, cols;
+    float scale;
+} pcx_muon_matrix;
+typedef struct pcx_segment {
+    int64_t offset, v_offset, n;
+} pcx_segment;
+size_t pcx_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+int pcx_orthogonalize(int dtype, int64_t batch, int64_t rows, int64_t cols, const void* x, int64_t batch_stride,
+                      int64_t row_stride, int64_t col_stride, void* out, int steps, const float* coef, float eps,
+                      void* ws, size_t ws_bytes, hipStream_t stream);
+size_t pcx_muon_workspace_bytes(const pcx_muon_matrix* mats, int n);
+int pcx_muon_step(const pcx_muon_matrix* mats, int n, float lr, float momentum, int nesterov, float weight_decay,
+                  float grad_scale, int steps, const float* coef, float eps, void* ws, size_t ws_bytes,
+                  hipStream_t stream);
+int pcx_adam_segments(float* p, const float* g, float* m, float* v, const pcx_segment* segs, int n, int64_t step,
+                      float lr, float beta1, float beta2, float eps, float weight_decay, float grad_scale,
+                      hipStream_t stream);
+
 /* ------------------------------------------------------------------ whole-network plans
  * A plan fixes the network configuration and the input shape [B, 1, F, T]; it owns no device
  * memory.  Parameters are passed as an array of device pointers in the reference's

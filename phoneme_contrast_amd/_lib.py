@@ -45,6 +45,17 @@ class NetConfig(ctypes.Structure):
                 ("conv_bf16", ctypes.c_int)]
 
 
+class MuonMatrix(ctypes.Structure):
+    """pcx_muon_matrix (include/pcx.h)."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("momentum", c_void_p), ("rows", c_i64), ("cols", c_i64),
+                ("scale", c_float)]
+
+
+class Segment(ctypes.Structure):
+    """pcx_segment (include/pcx.h)."""
+    _fields_ = [("offset", c_i64), ("v_offset", c_i64), ("n", c_i64)]
+
+
 _pp = ctypes.POINTER(ctypes.c_void_p)
 _pi = ctypes.POINTER(ctypes.c_int)
 _ps = ctypes.POINTER(ctypes.c_size_t)
@@ -71,6 +82,14 @@ SIGNATURES = {
                                       c_void_p, c_void_p, c_void_p]),
     "pcx_layernorm_backward": (c_int, [c_int, c_int, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_float, c_void_p,
                                        c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_size, c_void_p]),
+    "pcx_orthogonalize_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "pcx_orthogonalize": (c_int, [c_int, c_i64, c_i64, c_i64, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int,
+                                  ctypes.POINTER(c_float), c_float, c_void_p, c_size, c_void_p]),
+    "pcx_muon_workspace_bytes": (c_size, [ctypes.POINTER(MuonMatrix), c_int]),
+    "pcx_muon_step": (c_int, [ctypes.POINTER(MuonMatrix), c_int, c_float, c_float, c_int, c_float, c_float, c_int,
+                              ctypes.POINTER(c_float), c_float, c_void_p, c_size, c_void_p]),
+    "pcx_adam_segments": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(Segment), c_int, c_i64, c_float,
+                                  c_float, c_float, c_float, c_float, c_float, c_void_p]),
     "pcx_net_create": (c_void_p, [ctypes.POINTER(NetConfig), c_i64, c_i64, c_i64]),
     "pcx_net_destroy": (None, [c_void_p]),
     "pcx_net_workspace_bytes": (c_size, [c_void_p]),
