@@ -12,7 +12,9 @@
 // hi hi + hi lo + lo hi, exact in each term and summed in float32 (the dropped lo lo is below 2^-24 of the product):
 // three float16 MFMAs for one of float32, 16 / 3 of its rate at float32's accuracy.  S is a power of two that keeps
 // hi below 2^15 for the largest singular value the coefficients can reach (the caller's interval bound), so nothing
-// overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  a X is added to the
+// overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  A matrix whose norm is
+// far below eps starts far below 1: its S is larger by the power of two that all steps together cannot grow back
+// (ns_scale; A needs none, it only corrects a X there).  a X is added to the
 // sum in float32, not folded into B: folded, the large term makes every partial sum of the product round at its size
 // (2 to 3 times the float32 error).
 //
@@ -52,7 +54,7 @@ struct NsMat {
 struct NsTable {
     NsMat e[NS_LIST];
     int first[NS_LIST + 1];      // blocks of the launch up to each entry
-    int count;
+    int count, mats;
 };
 
 struct NsArgs {
@@ -62,7 +64,9 @@ struct NsArgs {
     int is_step, nesterov;
     float mu, gs, decay;         // momentum, gradient scale, 1 - lr wd
     float eps;
-    float sx, sa;                // S of X and of A, B
+    float sx, sa;                // S of X (of a matrix that starts near 1) and of A, B
+    double growth;               // most that all steps together enlarge a small singular value
+    float* unit;                 // [matrices] 1 / S of X
     float a, b, c;               // this step's coefficients
     int src;                     // which X buffer the step reads
 };
@@ -141,10 +145,17 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable t, NsArgs q) {
     if (threadIdx.x == 0) q.part[(int64_t)(e.norm + bat) * NS_PART + blk] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// exponent of the power of two above sx: 0 unless |X|_F times the growth of all steps stays below 1
+__device__ __forceinline__ int ns_scale(double fro, double growth) {
+    const double far = 1. / (fro * growth);
+    if (!(far >= 2.)) return 0;  // (NaN too)
+    return far > 1e27 ? 90 : ilogb(far);
+}
+
 // ---------------------------------------------------------------- X = u S / (|u| + eps) as planes, both ways round
 __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
     __shared__ float tile[64][65];
-    __shared__ float scale_s;
+    __shared__ double scale_s;
     const int ei = find_entry(t, blockIdx.x);
     const NsMat& e = t.e[ei];
     const int tm = e.mp / 64, tn = e.np / 64, per = tm * tn;
@@ -155,10 +166,15 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
         double s = q.part[(int64_t)(e.norm + bat) * NS_PART + threadIdx.x];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-        if (threadIdx.x == 0) scale_s = (float)(q.sx / (sqrt(s) + (double)q.eps));
+        if (threadIdx.x == 0) {
+            const double norm = sqrt(s), inv = 1. / (norm + (double)q.eps);
+            const int k = ns_scale(norm * inv, q.growth);
+            scale_s = ldexp(q.sx * inv, k);
+            if (tl == 0) q.unit[e.norm + bat] = ldexpf(1.f / q.sx, -k);
+        }
     }
     __syncthreads();
-    const float scale = scale_s;
+    const double scale = scale_s;
     const bool tall = e.rows > e.cols;
     // read with the source's columns across the threads
     for (int k = threadIdx.x; k < 64 * 64; k += 256) {
@@ -173,7 +189,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
                 v = load_any(e.x, bat * e.xb + r * e.xr + c * e.xc, q.dtype);
             }
         }
-        tile[tall ? sc : sr][tall ? sr : sc] = v * scale;
+        tile[tall ? sc : sr][tall ? sr : sc] = (float)(v * scale);
     }
     __syncthreads();
     for (int k = threadIdx.x; k < 64 * 16; k += 256) {
@@ -283,7 +299,7 @@ template <int PHASE> __global__ __launch_bounds__(256) void ns_sym_kernel(NsTabl
         const int r = i0 + (wave & 1) * 32 + acc_row(4 * g, lane >> 5);
         f16x4 h, l;
         if (PHASE == 0) {
-            const float k = q.sa / (q.sx * q.sx);
+            const float unit = q.unit[e.norm + bat], k = q.sa * unit * unit;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 f16 a, b;
@@ -352,7 +368,7 @@ template <bool LAST> __global__ __launch_bounds__(256) void ns_apply_kernel(NsTa
             store_planes(p.x(1 - q.src, 0), p.x(1 - q.src, 1), e.np, r, c, h, l);
             store_planes_t(p.xt(1 - q.src, 0), p.xt(1 - q.src, 1), e.mp, r, c, h, l);
         } else {
-            const float u = 1.f / q.sx;
+            const float u = q.unit[e.norm + bat];
             if (c >= e.rows) continue;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -386,32 +402,36 @@ void set_shape(NsMat& e, int64_t rows, int64_t cols) {
 
 // largest singular value any step can leave, starting in [0, 1], and the largest of |b s^2 + c s^4| on the way: by
 // dense sampling of the interval each step maps into (the polynomials are smooth: 1 % covers the gaps)
-void ns_bounds(const float* coef, int steps, double* smax, double* bmax) {
+void ns_bounds(const float* coef, int steps, double* smax, double* bmax, double* growth) {
     double hi = 1.0;
     *smax = 1.0;
     *bmax = 0.0;
+    *growth = 1.0;
     for (int k = 0; k < steps; ++k) {
         const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
-        double next = 0.0;
+        double next = 0.0, grow = 1.0;
         for (int i = 0; i <= 4096; ++i) {
             const double s = hi * i / 4096, l = s * s, bb = b * l + c * l * l;
             next = std::max(next, fabs(s * (a + bb)));
+            grow = std::max(grow, 1.01 * fabs(a + bb));
             *bmax = std::max(*bmax, std::max(fabs(bb), l));
         }
         hi = next * 1.01;
+        *growth *= grow;
         *smax = std::max(*smax, hi);
         if (!(hi < 1e6)) break;
     }
 }
 
-// One launch table's workspace: the partial sums of every matrix, then the planes, 256-byte aligned.
+// One launch table's workspace: the partial sums and the unit of every matrix, then the planes, 256-byte aligned.
 int64_t ns_place(NsTable& t) {
     int64_t mats = 0;
     for (int i = 0; i < t.count; ++i) {
         t.e[i].norm = (int)mats;
         mats += t.e[i].batch;
     }
-    int64_t off = mats * NS_PART * (int64_t)sizeof(double);
+    t.mats = (int)mats;
+    int64_t off = mats * (NS_PART * (int64_t)sizeof(double) + (int64_t)sizeof(float));
     for (int i = 0; i < t.count; ++i) {
         off = (off + 255) / 256 * 256;
         t.e[i].ws = off;
@@ -422,7 +442,7 @@ int64_t ns_place(NsTable& t) {
 
 int ns_scales(NsArgs& q, const float* coef, int steps) {
     double smax, bmax;
-    ns_bounds(coef, steps, &smax, &bmax);
+    ns_bounds(coef, steps, &smax, &bmax, &q.growth);
     PCX_CHECK_ARG(smax <= 8.0 && bmax <= 64.0,
                   "orthogonalize: the coefficients take singular values in [0, 1] to %g (8 at most)", smax);
     q.sx = (float)exp2(floor(log2(32768.0 / smax)));
@@ -431,6 +451,7 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
 }
 
 int ns_run(NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
+    q.unit = reinterpret_cast<float*>(q.part + (int64_t)t.mats * NS_PART);
     auto blocks = [&](auto per) {
         int64_t n = 0;
         for (int i = 0; i < t.count; ++i) {

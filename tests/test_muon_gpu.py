@@ -1,0 +1,367 @@
+"""Newton-Schulz orthogonalisation, the optimiser step on it and FusedMuon against float64 (csrc/muon.hip, optim.py).
+
+Error bound.  One step maps X to p(X) = a X + (b A + c A A) X with every product summed in float32 from operands held to
+2^-24, the lo lo terms (2^-24) dropped: a K-term sum is off by at most g = (4 + 2 sqrt(K)) 2^-24 of the product of its
+operands' Frobenius and spectral norms (roundings of random sign).  With s the largest singular value before the step
+and f = |X|_F, the step adds at most g f (|a| + 3 |b| s^2 + 5 |c| s^4), and later steps multiply an error by at most
+max |p'| over the singular values on the way: the sum over the steps of the one times the other bounds the result's
+Frobenius error (`bound`), from the float64 singular values of the case itself.  The sharper claim of the documentation,
+float32's own accuracy, is tested against the float32 iteration on the CPU."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+COEF = (3.4445, -4.7750, 2.0315)
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def triples(coef, steps):
+    return [coef] * steps if not isinstance(coef[0], (tuple, list)) else list(coef)
+
+
+def iterate(x, coef=COEF, steps=5, eps=1e-7):
+    """The definition, in x's type, on the shorter side."""
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT.contiguous() if tall else x
+    norm = x.double().square().sum((-1, -2), keepdim=True).sqrt()
+    x = (x.double() / (norm + eps)).to(x.dtype)
+    for a, b, c in triples(coef, steps):
+        g = x @ x.mT.contiguous()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x.mT.contiguous() if tall else x
+
+
+def bound(x, coef=COEF, steps=5, eps=1e-7):
+    """Largest Frobenius error of the iteration for one float64 matrix."""
+    if x.shape[0] > x.shape[1]:
+        x = x.mT
+    g = (4 + 2 * math.sqrt(max(x.shape))) * 2.0 ** -24
+    s = torch.linalg.svdvals(x / (torch.linalg.vector_norm(x) + eps))
+    err = 2.0 ** -23 * s.norm().item()  # the scaled input: two roundings
+    for a, b, c in triples(coef, steps):
+        slope = (a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max().item()
+        top, f = s.max().item(), s.norm().item()
+        err = err * max(slope, 1e-3) + g * f * (abs(a) + 3 * abs(b) * top ** 2 + 5 * abs(c) * top ** 4)
+        s = (a * s + b * s ** 3 + c * s ** 5).abs()
+    return err
+
+
+def gradient(rows, cols, seed, n=96, noise=0.1):
+    """A minibatch gradient: n samples' outer products of falling weight, and noise."""
+    gen = torch.Generator().manual_seed(seed)
+    w = torch.arange(1, n + 1).float().pow(-0.5)[:, None]
+    g = (torch.randn(n, rows, generator=gen) * w).T @ torch.randn(n, cols, generator=gen)
+    return 1e-2 * (g + noise * torch.randn(rows, cols, generator=gen))
+
+
+def close(got, x, coef=COEF, steps=5, eps=1e-7):
+    """got (any type) against the float64 iteration of x (float64, one matrix)."""
+    ref = iterate(x, coef, steps, eps)
+    off = torch.linalg.vector_norm(got.detach().cpu().double() - ref).item()
+    h = torch.finfo(got.dtype).eps / 2 if got.dtype != torch.float32 else 2.0 ** -24
+    limit = bound(x, coef, steps, eps) * (1 + h) + h * torch.linalg.vector_norm(ref).item()
+    assert off <= limit, (off, limit)
+    return off
+
+
+SHAPES = [(1, 1), (1, 2), (2, 1), (1, 300), (300, 1), (2, 3), (3, 5), (9, 32), (31, 33), (63, 64), (64, 64), (65, 64), (64, 129),
+          (65, 65), (128, 128), (100, 577), (577, 100), (128, 1152), (200, 1001), (333, 129), (512, 512), (257, 2305)]
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_shapes_and_types(rows, cols, t):
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = gradient(rows, cols, rows * 7 + cols).to(TYPES[t])
+    out = orthogonalize(x.cuda())
+    assert out.dtype == x.dtype and out.shape == x.shape and out.is_contiguous()
+    close(out, x.double())
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 576), (128, 128), (200, 333), (512, 1024), (640, 640)])
+def test_as_exact_as_float32_arithmetic(rows, cols):
+    """Twice the float32 iteration's own error: its operands and sums round at 2^-24 as these do, and the dropped
+    lo lo terms and the rescaled input add no more than as much again."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    for seed in range(3):
+        x = gradient(rows, cols, seed)
+        ref = iterate(x.double())
+        err32 = torch.linalg.vector_norm(iterate(x).double() - ref)
+        err = torch.linalg.vector_norm(orthogonalize(x.cuda()).cpu().double() - ref)
+        assert err <= 2 * err32, (err.item(), err32.item())
+
+
+def test_result_is_nearly_orthogonal():
+    """Five steps take singular values in [0.01, 1] of the normalised matrix into [0.68, 1.21] (the polynomial's own
+    range, by its definition); a well-conditioned matrix of 64 rows starts above 0.05."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = torch.randn(64, 400, generator=torch.Generator().manual_seed(1))
+    s = torch.linalg.svdvals(orthogonalize(x.cuda()).cpu().double())
+    assert 0.68 < s.min() and s.max() < 1.21
+
+
+@pytest.mark.parametrize("steps,coef", [(1, COEF), (2, COEF), (3, COEF), (8, COEF), (6, (1.875, -1.25, 0.375)),
+                                        (4, ((4.0, -6.0, 2.5), (3.0, -3.5, 1.4), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0)))])
+def test_steps_and_coefficients(steps, coef):
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = gradient(90, 150, 5)
+    close(orthogonalize(x.cuda(), ns_steps=steps, ns_coefficients=coef), x.double(), coef, steps)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-7, 1e4, 1e18, 1e30])
+def test_any_size_of_input(scale):
+    """Sums of squares have no range to leave (float64); below eps the matrix is only scaled up, to |x| / eps."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = gradient(70, 130, 6) * scale
+    close(orthogonalize(x.cuda()), x.double())
+
+
+def test_strides_views_and_batches():
+    from phoneme_contrast_amd.optim import orthogonalize
+    big = torch.stack([gradient(80, 220, s) for s in range(6)]).view(2, 3, 80, 220)
+    dev = big.cuda()
+    views = {"transposed": lambda t: t.mT, "sliced": lambda t: t[..., 3:70, 5:205], "every second": lambda t: t[..., ::2, ::3],
+             "swapped batch": lambda t: t.transpose(0, 1), "expanded": lambda t: t[:1].expand(4, 3, 80, 220),
+             "one": lambda t: t[1, 2], "rows of one": lambda t: t[..., :1, :], "uneven batch": lambda t: t[:, :2]}
+    for name, view in views.items():
+        x, out = view(big), orthogonalize(view(dev))
+        assert out.shape == x.shape and out.is_contiguous()
+        for i, (m, o) in enumerate(zip(x.reshape(-1, *x.shape[-2:]), out.reshape(-1, *x.shape[-2:]))):
+            close(o, m.double())
+    assert torch.equal(orthogonalize(dev)[1, 1], orthogonalize(dev[1, 1]))  # a batch changes nothing
+
+
+def test_empty_zero_and_non_finite_matrices():
+    from phoneme_contrast_amd.optim import orthogonalize
+    for shape in ((0, 5, 6), (3, 0, 6), (3, 5, 0), (0, 0)):
+        assert orthogonalize(torch.empty(shape, device="cuda")).shape == shape
+    x = torch.stack([gradient(70, 100, s) for s in range(5)])
+    clean = orthogonalize(x.cuda())
+    x[1], x[2, 3, 4], x[3, 69, 99] = 0, float("nan"), float("inf")
+    out = orthogonalize(x.cuda())
+    assert torch.equal(out[0], clean[0]) and torch.equal(out[4], clean[4])
+    assert not out[1].any() and torch.isnan(out[2]).all() and torch.isnan(out[3]).all()
+
+
+def test_no_gradient_and_repeats_on_any_stream():
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = gradient(300, 500, 8).cuda().requires_grad_(True)
+    a = orthogonalize(x)
+    assert not a.requires_grad
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = orthogonalize(x)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(a, b) and torch.equal(a, orthogonalize(x))
+
+
+def test_two_captured_graphs():
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = gradient(130, 260, 9).cuda()
+    y = gradient(260, 130, 10).cuda()
+    orthogonalize(x), orthogonalize(y)
+    torch.cuda.synchronize()
+    graphs = []
+    for t in (x, y):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0][0].pool() if graphs else None):
+            out = orthogonalize(t)
+        graphs.append((g, t, out))
+    for i in range(4):
+        g, t, out = graphs[i % 2]
+        t.copy_(gradient(*t.shape, 20 + i))
+        want = orthogonalize(t)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_refusals():
+    from phoneme_contrast_amd.optim import FusedMuon, muon_step, orthogonalize
+    x = torch.randn(8, 9, device="cuda")
+    for bad in (lambda: orthogonalize(x[0]), lambda: orthogonalize(x.double()), lambda: orthogonalize(x.int()),
+                lambda: orthogonalize(x, ns_steps=0), lambda: orthogonalize(x, ns_steps=65), lambda: orthogonalize(x, eps=0.0),
+                lambda: orthogonalize(x, eps=float("nan")), lambda: orthogonalize(x, ns_coefficients=(1.0, 2.0)),
+                lambda: orthogonalize(x, ns_coefficients=((1.0, 2.0, 3.0),) * 4),
+                lambda: orthogonalize(x, ns_coefficients=(10.0, 0.0, 0.0)),
+                lambda: orthogonalize(x, ns_coefficients=(float("nan"), 0.0, 0.0)),
+                lambda: orthogonalize(torch.empty(1, 1, device="cuda").expand(20000, 20000))):
+        with pytest.raises(ValueError):
+            bad()
+    p, g, m = (torch.randn(8, 9, device="cuda") for _ in range(3))
+
+    def step(ps=(p,), gs=(g,), ms=(m,), **kw):
+        muon_step(ps, gs, ms, **{"lr": 0.1, **kw})
+    before = p.clone()
+    for bad in (lambda: step(gs=()), lambda: step(ps=(p, p), gs=(g, g), ms=(m, m.clone())), lambda: step(ms=(p,)),
+                lambda: step(ps=(p, p.clone()), gs=(g, g), ms=(m, m)), lambda: step(gs=(g[:, :8],)), lambda: step(gs=(g.half(),)),
+                lambda: step(ps=(p.T.contiguous().T,)), lambda: step(ps=(p[0],), gs=(g[0],), ms=(m[0],)), lambda: step(lr=-1.0),
+                lambda: step(momentum=1.0), lambda: step(weight_decay=-0.1), lambda: step(eps=0.0), lambda: step(adjust="no"),
+                lambda: FusedMuon([torch.nn.Parameter(p)], momentum=1.5), lambda: FusedMuon([torch.nn.Parameter(p)], lr=-1.0),
+                lambda: FusedMuon([torch.nn.Parameter(p)], adjust="x"), lambda: FusedMuon([torch.nn.Parameter(p)], ns_steps=0)):
+        with pytest.raises(ValueError):
+            bad()
+    assert torch.equal(p, before)
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        step(gs=(g.cpu(),))
+    step(ps=(), gs=(), ms=())
+
+
+def reference_step(p, g, m, lr, momentum, nesterov, wd, adjust, gs=1.0, **kw):
+    """float64 -> new parameter, new momentum, and the bound on the parameter's error."""
+    p, g, m = (t.cpu().double() for t in (p, g, m))
+    m = momentum * m + (1 - momentum) * gs * g
+    u = ((1 - momentum) * gs * g + momentum * m if nesterov else m).reshape(p.shape[0], -1)
+    rows, cols = u.shape
+    k = {"rms": 0.2 * math.sqrt(max(rows, cols)), "spectral": math.sqrt(max(1, rows / cols)), None: 1.0}[adjust]
+    o = iterate(u, **kw)
+    # u itself carries three float32 roundings; the iteration multiplies them as it does the input's
+    tol = 3 * bound(u, **kw) * lr * k + 3 * 2.0 ** -24 * (p.norm().item() + lr * k * o.norm().item())
+    return (1 - lr * wd) * p - lr * k * o.view_as(p), m, tol
+
+
+@pytest.mark.parametrize("nesterov,adjust,wd,gs", [(True, "rms", 0.1, 1.0), (False, "spectral", 0.0, 0.125), (True, None, 1e-2, 4.0)])
+def test_step_of_a_list(nesterov, adjust, wd, gs):
+    """More matrices than one launch takes, of every kind of shape."""
+    from phoneme_contrast_amd.optim import muon_step
+    shapes = [(32, 1, 3, 3), (64, 32, 3, 3), (128, 128), (96, 200), (200, 96), (5, 2), (2, 70), (1, 40), (40, 1), (130, 64, 1, 1)]
+    shapes = shapes * 3 + [(256, 600)]
+    gen = torch.Generator().manual_seed(2)
+    p = [torch.randn(s, generator=gen) for s in shapes]
+    g = [gradient(s[0], math.prod(s[1:]), i).view(s) for i, s in enumerate(shapes)]
+    m = [gradient(s[0], math.prod(s[1:]), 100 + i).view(s) for i, s in enumerate(shapes)]
+    dp, dg, dm = ([t.cuda() for t in ts] for ts in (p, g, m))
+    for _ in range(2):
+        ref = [reference_step(a, b, c, 0.02, 0.9, nesterov, wd, adjust, gs) for a, b, c in zip(dp, dg, dm)]
+        muon_step(dp, dg, dm, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=wd, adjust=adjust, grad_scale=gs)
+        for a, c, (ra, rc, tol) in zip(dp, dm, ref):
+            assert (a.cpu().double() - ra).norm().item() <= tol
+            assert ((c.cpu().double() - rc).abs() <= 3 * 2.0 ** -24 * (rc.abs() + c.cpu().abs().max())).all()
+    for a, b in zip(dg, g):
+        assert torch.equal(a.cpu(), b)
+
+
+def small_model(seed=0):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Conv2d(3, 20, 3), torch.nn.BatchNorm2d(20), torch.nn.Conv2d(20, 1, 1),
+                               torch.nn.Flatten(), torch.nn.Linear(36, 50), torch.nn.Linear(50, 7, bias=False)).cuda()
+
+
+def set_grads(model, seed):
+    gen = torch.Generator().manual_seed(seed)
+    for p in model.parameters():
+        p.grad = torch.randn(p.shape, generator=gen).cuda() * 0.1
+
+
+def adam_reference(p, g, m, v, step, lr, wd, betas=(0.9, 0.999), eps=1e-8):
+    g = g + wd * p
+    m = betas[0] * m + (1 - betas[0]) * g
+    v = betas[1] * v + (1 - betas[1]) * g * g
+    den = v.sqrt() / math.sqrt(1 - betas[1] ** step) + eps
+    return p - lr / (1 - betas[0] ** step) * m / den, m, v
+
+
+@pytest.mark.parametrize("flat", [False, True])
+def test_optimizer_matches_the_formulas(flat):
+    from phoneme_contrast_amd.optim import FusedMuon
+    model = small_model()
+    opt = FusedMuon(model.parameters(), lr=0.01, weight_decay=0.05)
+    names = [n for n, _ in model.named_parameters()]
+    mats = {"0.weight", "4.weight", "5.weight"}  # the 1 x 20 convolution, norms and biases take Adam
+    state = {n: (torch.zeros_like(p).cpu().double(), torch.zeros_like(p).cpu().double()) for n, p in model.named_parameters()}
+    for step in range(1, 4):
+        set_grads(model, step)
+        before = {n: p.detach().cpu().double() for n, p in model.named_parameters()}
+        grads = {n: p.grad.cpu().double() for n, p in model.named_parameters()}
+        if flat:  # the summed gradients of two ranks, averaged in the step
+            fg = torch.cat([2 * p.grad.reshape(-1) for p in model.parameters()])
+            opt.step(flat_grads=[fg], grad_scale=0.5)
+        else:
+            opt.step()
+        for n, p in model.named_parameters():
+            got = p.detach().cpu().double()
+            m, v = state[n]
+            if n in mats:
+                ref, m2, tol = reference_step(before[n].float(), grads[n].float(), m.float(), 0.01, 0.95, True, 0.05, "rms")
+                assert (got - ref).norm().item() <= tol, n
+                state[n] = (m2, v)
+            else:
+                ref, m2, v2 = adam_reference(before[n], grads[n], m, v, step, 0.01, 0.05)
+                # eight float32 operations on an update of size lr and on p
+                assert ((got - ref).abs() <= 16 * 2.0 ** -24 * (ref.abs() + 0.01 * 4)).all(), n
+                state[n] = (m2, v2)
+    sd = opt.state_dict()
+    for i, n in enumerate(names):
+        s = sd["state"][i]
+        assert set(s) == ({"step", "momentum_buffer"} if n in mats else {"step", "exp_avg", "exp_avg_sq"}) and int(s["step"]) == 3
+        own = s["momentum_buffer" if n in mats else "exp_avg"].cpu().double()
+        assert ((own - state[n][0]).abs() <= 16 * 2.0 ** -24 * (state[n][0].abs() + 0.2)).all()
+
+
+def test_optimizer_state_moves_on(tmp_path):
+    """Save, load and go on; parameters bound anew behind the optimizer's back; a group of Adam only; a schedule."""
+    from phoneme_contrast_amd.optim import FusedAdam, FusedMuon
+    a, b = small_model(1), small_model(1)
+    oa, ob = FusedMuon(a.parameters(), lr=0.02), FusedMuon(b.parameters(), lr=0.02)
+    for k in range(2):
+        set_grads(a, k), set_grads(b, k)
+        oa.step(), ob.step()
+    torch.save({"o": ob.state_dict(), "m": b.state_dict()}, tmp_path / "c.pt")
+    c = small_model(2)
+    saved = torch.load(tmp_path / "c.pt", weights_only=True, map_location="cuda")
+    c.load_state_dict(saved["m"])
+    oc = FusedMuon(c.parameters(), lr=0.5)
+    oc.load_state_dict(saved["o"])
+    a.cpu(), a.cuda()  # re-bound: new storages
+    sched = torch.optim.lr_scheduler.StepLR(oa, 1, 0.5)
+    for k in range(2, 4):
+        for mdl, o in ((a, oa), (c, oc)):
+            o.param_groups[0]["lr"] = 0.02
+            set_grads(mdl, k)
+            o.step()
+    for p, q in zip(a.parameters(), c.parameters()):
+        assert torch.equal(p, q)
+    oa.param_groups[0]["lr"] = sched.base_lrs[0]
+    sched.step()
+    assert oa.param_groups[0]["lr"] == 0.01
+    fa = FusedAdam(small_model(3).parameters())
+    with pytest.raises(ValueError, match="another optimizer"):
+        oc.load_state_dict(fa.state_dict())
+    d, e = small_model(4), small_model(4)
+    od, oe = FusedMuon([{"params": d.parameters(), "muon": False}], lr=0.01, weight_decay=0.1), FusedAdam(e.parameters(), 0.01, weight_decay=0.1)
+    for k in range(2):
+        set_grads(d, k), set_grads(e, k)
+        od.step(), oe.step()
+    for p, q in zip(d.parameters(), e.parameters()):
+        assert ((p - q).abs() <= 4 * 2.0 ** -24 * (q.abs() + 0.02)).all()  # (two kernels: contractions may differ)
+    assert oc.step() is None  # (no further gradients set: the last ones again)
+    with pytest.raises(ValueError, match="flat gradient"):
+        oc.step(flat_grads=[torch.zeros(3, device="cuda")])
+
+
+def test_step_in_a_captured_graph():
+    from phoneme_contrast_amd.optim import muon_step
+    shapes = [(32, 9), (64, 288), (128, 128)]
+    p = [gradient(*s, 1).cuda() for s in shapes]
+    m = [gradient(*s, 2).cuda() for s in shapes]
+    g = [gradient(*s, 3).cuda() for s in shapes]
+    p2, m2 = [t.clone() for t in p], [t.clone() for t in m]
+    warm = [t.clone() for t in p], [t.clone() for t in m]
+    muon_step(warm[0], g, warm[1], lr=0.01)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step(p, g, m, lr=0.01)
+    for k in range(3):
+        for i, s in enumerate(shapes):
+            g[i].copy_(gradient(*s, 10 + k))
+        graph.replay()
+        muon_step(p2, g, m2, lr=0.01)
+        torch.cuda.synchronize()
+        for a, b in zip(p + m, p2 + m2):
+            assert torch.equal(a, b)
