@@ -18,10 +18,13 @@
 // sum in float32, not folded into B: folded, the large term makes every partial sum of the product round at its size
 // (2 to 3 times the float32 error).
 //
-// Layout.  X is kept as hi / lo planes [mp][np] and transposed [np][mp], A and B as [mp][mp], all padded with zeros to
-// the tile, so that every product is one of rows with rows (K contiguous on both sides) and no tile checks bounds.
+// Layout.  X is kept as hi / lo planes and transposed, A and B once, all padded with zeros to 64, so that every product is
+// one of rows with rows.  A plane is stored in panels of 32 values of K, [K / 32][rows][32]: what a tile needs of a panel
+// is one run of memory.  (Row by row, the rows of a tile lie a power of two apart more often than not and queue at one
+// L2 channel: 512 x 4608 took 35 us for the product that takes XXX us now.)
 // A and B are symmetric: only tiles on and above the diagonal are computed, and written twice.
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -36,8 +39,10 @@ typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int NS_LIST = 24;      // entries per launch (their table is a kernel argument)
-constexpr int NS_TILE = 64;      // rows and columns of a tile; X, A, B are padded to it
-constexpr int NS_K = 32;         // K values staged at a time
+constexpr int NS_PAD = 64;       // X, A, B are padded to it; tiles that reach over the padding read their last rows again
+constexpr int NS_K = 32;         // K values of a stage
+constexpr int NS_BUF = 3;        // stages in LDS: one computed on, two on their way
+constexpr int NS_PART = 512;     // most partial sums of squares per matrix
 
 struct NsMat {
     const void* x;               // orthogonalize: the matrices; step: gradients
@@ -45,33 +50,45 @@ struct NsMat {
     float* mom;                  // step: momentum
     int64_t xb, xr, xc;          // strides of x in elements: matrix, row, column
     int rows, cols, batch;
-    int m, n, mp, np;            // short and long side, and padded
+    int mp, np;                  // short and long side, padded
     float step;                  // step: lr k
     int64_t ws;                  // byte offset of the entry's planes in the workspace
-    int norm;                    // first of its partial sums of squares
+    int mat, parts;              // first of its matrices in the launch, partial sums of each
 };
 
 struct NsTable {
     NsMat e[NS_LIST];
-    int first[NS_LIST + 1];      // blocks of the launch up to each entry
     int count, mats;
+};
+
+// Work units of a product launch, per entry: its tiles in order, the first `whole` over all of K, the others in `split`
+// parts each (joined by whichever unit of a tile ends last, in part order).
+struct NsUnits {
+    int first[NS_LIST + 1];      // units of the launch up to each entry
+    int tiles[NS_LIST];          // tiles of one matrix of the entry
+    int whole[NS_LIST];          // of the entry's tiles times batch
+    int split[NS_LIST];
+    int tail[NS_LIST];           // first counter of the entry's split tiles
+    int joint[NS_LIST];          // first of their parts' sums
+    int count;
 };
 
 struct NsArgs {
     char* ws;
-    double* part;                // [.] partial sums of squares, NS_PART per matrix
+    double* part;                // [matrices][NS_PART] partial sums of squares
+    float* unit;                 // [matrices] 1 / S of X
+    unsigned* done;              // [split tiles] parts that have been written
+    float* joint;                // [split tiles][parts][tile] their sums
+    int ndone;
     int dtype;                   // orthogonalize: type of x and out
     int is_step, nesterov;
     float mu, gs, decay;         // momentum, gradient scale, 1 - lr wd
     float eps;
     float sx, sa;                // S of X (of a matrix that starts near 1) and of A, B
     double growth;               // most that all steps together enlarge a small singular value
-    float* unit;                 // [matrices] 1 / S of X
     float a, b, c;               // this step's coefficients
     int src;                     // which X buffer the step reads
 };
-
-constexpr int NS_PART = 64;      // partial sums per matrix
 
 // planes of one matrix, in float16 numbers from its workspace: X hi, lo, X^T hi, lo (two buffers), A hi, lo, B hi, lo
 struct Planes {
@@ -82,6 +99,10 @@ struct Planes {
     __device__ f16* a(int lo) const { return base + 8 * mn + lo * mm; }
     __device__ f16* b(int lo) const { return base + 8 * mn + (2 + lo) * mm; }
 };
+// value (row, k) of a plane of `rows` rows
+__device__ __forceinline__ int64_t at_panel(int row, int k, int rows) {
+    return ((int64_t)(k >> 5) * rows + row) * 32 + (k & 31);
+}
 __host__ __device__ inline int64_t plane_bytes(int mp, int np) {
     return 2 * (8 * (int64_t)mp * np + 4 * (int64_t)mp * mp);
 }
@@ -93,10 +114,17 @@ __device__ __forceinline__ Planes planes_of(const NsArgs& q, const NsMat& e, int
     return p;
 }
 
-__device__ __forceinline__ int find_entry(const NsTable& t, int blk) {
+__device__ __forceinline__ int find_entry(const int* first, int count, int blk) {
     int i = 0;
-    while (i + 1 < t.count && blk >= t.first[i + 1]) ++i;
+    while (i + 1 < count && blk >= first[i + 1]) ++i;
     return i;
+}
+
+// blocks go to the 8 XCDs in turn: block b of n works as unit xcd_order(b, n), which gives each XCD (its own L2) adjacent
+// units
+__device__ __forceinline__ int xcd_order(int b, int n) {
+    const int q = n >> 3, r = n & 7, x = b & 7;
+    return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);
 }
 
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
@@ -115,34 +143,54 @@ __device__ __forceinline__ float nesterov_u(const NsArgs& q, float g, float m) {
 }
 
 // ---------------------------------------------------------------- u, and the sums of its squares (in float64: no range)
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsTable t, NsArgs q) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsTable t, NsUnits un, NsArgs q) {
     __shared__ double red[4];
-    const int ei = find_entry(t, blockIdx.x);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < q.ndone; i += 256) q.done[i] = 0;
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
-    const int bat = (blockIdx.x - t.first[ei]) / NS_PART, blk = (blockIdx.x - t.first[ei]) % NS_PART;
-    const int64_t n = (int64_t)e.rows * e.cols;
-    const int64_t per = (n + NS_PART - 1) / NS_PART, i0 = blk * per, i1 = i0 + per < n ? i0 + per : n;
+    const int bat = (blockIdx.x - un.first[ei]) / e.parts, blk = (blockIdx.x - un.first[ei]) % e.parts;
     double s = 0.;
-    if (q.is_step) {
-        const float* g = static_cast<const float*>(e.x);
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-            const float gv = g[i], mv = fmaf(1.f - q.mu, gv * q.gs, q.mu * e.mom[i]);
-            e.mom[i] = mv;
-            const float u = nesterov_u(q, gv, mv);
-            s += (double)u * u;
+    const int64_t n = (int64_t)e.rows * e.cols;
+    if (q.is_step || (e.xc == 1 && e.xr == e.cols)) {  // adjacent values
+        const int64_t per = (n + e.parts - 1) / e.parts, i0 = blk * per, i1 = i0 + per < n ? i0 + per : n;
+        if (q.is_step) {
+            const float* g = static_cast<const float*>(e.x);
+#pragma unroll 8
+            for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
+                const float gv = g[i], mv = fmaf(1.f - q.mu, gv * q.gs, q.mu * e.mom[i]);
+                e.mom[i] = mv;
+                const float u = nesterov_u(q, gv, mv);
+                s += (double)u * u;
+            }
+        } else {
+            const auto run = [&](auto kind) {
+                const auto* x = static_cast<const decltype(kind)*>(e.x) + bat * e.xb;
+#pragma unroll 8
+                for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
+                    const double u = (float)x[i];
+                    s += u * u;
+                }
+            };
+            if (q.dtype == PCX_F32) run(float());
+            else if (q.dtype == PCX_BF16) run(bf16());
+            else run(f16());
         }
-    } else {
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-            const int64_t r = i / e.cols, c = i - r * e.cols;
-            const float u = load_any(e.x, bat * e.xb + r * e.xr + c * e.xc, q.dtype);
-            s += (double)u * u;
-        }
+    } else {  // along the axis of the smaller stride
+        const bool turn = llabs(e.xr) < llabs(e.xc);
+        const int no = turn ? e.cols : e.rows, ni = turn ? e.rows : e.cols;
+        const int64_t so = turn ? e.xc : e.xr, si = turn ? e.xr : e.xc;
+        for (int r = blk; r < no; r += e.parts)
+            for (int c = threadIdx.x; c < ni; c += 256) {
+                const double u = load_any(e.x, bat * e.xb + r * so + c * si, q.dtype);
+                s += u * u;
+            }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) q.part[(int64_t)(e.norm + bat) * NS_PART + blk] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) q.part[(int64_t)(e.mat + bat) * NS_PART + blk] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // exponent of the power of two above sx: 0 unless |X|_F times the growth of all steps stays below 1
@@ -153,47 +201,69 @@ __device__ __forceinline__ int ns_scale(double fro, double growth) {
 }
 
 // ---------------------------------------------------------------- X = u S / (|u| + eps) as planes, both ways round
-__global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
+__global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsUnits un, NsArgs q) {
     __shared__ float tile[64][65];
+    __shared__ double red[4];
     __shared__ double scale_s;
-    const int ei = find_entry(t, blockIdx.x);
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
-    const int tm = e.mp / 64, tn = e.np / 64, per = tm * tn;
-    const int rel = blockIdx.x - t.first[ei], bat = rel / per, tl = rel % per;
+    const int tn = e.np / 64, per = (e.mp / 64) * tn;
+    const int rel = blockIdx.x - un.first[ei], bat = rel / per, tl = rel % per;
     const int i0 = (tl / tn) * 64, j0 = (tl % tn) * 64;  // of X (m x n)
     const Planes P = planes_of(q, e, bat);
-    if (threadIdx.x < 64) {
-        double s = q.part[(int64_t)(e.norm + bat) * NS_PART + threadIdx.x];
+    const bool tall = e.rows > e.cols;
+    // 16 values a thread, the source's columns across the threads, on their way while the norm is formed
+    const int sc = threadIdx.x & 63, c = (tall ? i0 : j0) + sc;
+    float v[16];
+    const auto fetch = [&](auto kind) {
+        const auto* x = static_cast<const decltype(kind)*>(e.x) + bat * e.xb + c * e.xc;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int r = (tall ? j0 : i0) + (threadIdx.x >> 6) + 4 * k;
+            v[k] = r < e.rows && c < e.cols ? (float)x[r * e.xr] : 0.f;
+        }
+    };
+    if (q.is_step) {
+        fetch(float());
+        float m[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int r = (tall ? j0 : i0) + (threadIdx.x >> 6) + 4 * k;
+            m[k] = r < e.rows && c < e.cols ? e.mom[(int64_t)r * e.cols + c] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = nesterov_u(q, v[k], m[k]);
+    } else if (q.dtype == PCX_F32) {
+        fetch(float());
+    } else if (q.dtype == PCX_BF16) {
+        fetch(bf16());
+    } else {
+        fetch(f16());
+    }
+    {
+        double s = 0.;
+        for (int i = threadIdx.x; i < e.parts; i += 256) s += q.part[(int64_t)(e.mat + bat) * NS_PART + i];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+        __syncthreads();
         if (threadIdx.x == 0) {
-            const double norm = sqrt(s), inv = 1. / (norm + (double)q.eps);
+            const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3])), inv = 1. / (norm + (double)q.eps);
             const int k = ns_scale(norm * inv, q.growth);
             scale_s = ldexp(q.sx * inv, k);
-            if (tl == 0) q.unit[e.norm + bat] = ldexpf(1.f / q.sx, -k);
+            if (tl == 0) q.unit[e.mat + bat] = ldexpf(1.f / q.sx, -k);
         }
     }
     __syncthreads();
     const double scale = scale_s;
-    const bool tall = e.rows > e.cols;
-    // read with the source's columns across the threads
-    for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-        const int sr = k >> 6, sc = k & 63;
-        const int r = (tall ? j0 : i0) + sr, c = (tall ? i0 : j0) + sc;
-        float v = 0.f;
-        if (r < e.rows && c < e.cols) {
-            if (q.is_step) {
-                const int64_t i = (int64_t)r * e.cols + c;
-                v = nesterov_u(q, static_cast<const float*>(e.x)[i], e.mom[i]);
-            } else {
-                v = load_any(e.x, bat * e.xb + r * e.xr + c * e.xc, q.dtype);
-            }
-        }
-        tile[tall ? sc : sr][tall ? sr : sc] = (float)(v * scale);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int sr = (threadIdx.x >> 6) + 4 * k;
+        tile[tall ? sc : sr][tall ? sr : sc] = (float)(v[k] * scale);
     }
     __syncthreads();
     for (int k = threadIdx.x; k < 64 * 16; k += 256) {
-        const int r = k >> 4, c = (k & 15) * 4;
+        const int r = (k >> 3) & 63, c = (k & 7) * 4 + (k >> 9) * 32;
         f16x4 h, l, ht, lt;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -205,7 +275,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
             ht[j] = a;
             lt[j] = b;
         }
-        const int64_t o = (int64_t)(i0 + r) * e.np + j0 + c, ot = (int64_t)(j0 + r) * e.mp + i0 + c;
+        const int64_t o = at_panel(i0 + r, j0 + c, e.mp), ot = at_panel(j0 + r, i0 + c, e.np);
         *reinterpret_cast<f16x4*>(P.x(0, 0) + o) = h;
         *reinterpret_cast<f16x4*>(P.x(0, 1) + o) = l;
         *reinterpret_cast<f16x4*>(P.xt(0, 0) + ot) = ht;
@@ -214,178 +284,355 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsArgs q) {
 }
 
 // ---------------------------------------------------------------- the products
-// 64 x 64 tile of C[r][c] = sum_k P[r][k] Q[c][k], four waves of 32 x 32 each; P, Q: hi / lo planes with row length ld.
-// On return lane l of wave w holds rows r = 32 (w & 1) + acc_row(i, l >> 5), column c = 32 (w >> 1) + (l & 31) of the
-// tile, so four consecutive i are four consecutive rows of one column.
-struct Operand {
-    const f16* hi;
-    const f16* lo;
-    int64_t ld;
-};
+// C[r][c] = sum_k P[r][k] Q[c][k] on tiles of TM = 64 WM rows by TN = 64 WN columns, four waves of 32 WM x 32 WN each.
+// The operands' four plane tiles (32 K values of TM + TN rows, hi and lo) are copied to LDS by global_load_lds, 16 bytes
+// per lane, NS_BUF stages deep; run q of row r sits in slot q ^ ((r >> 2) & 3), which spreads the operand reads over all
+// banks.  One barrier per stage, half a stage ahead of its first read: while the first half's MFMAs run, the second
+// half's operands are read; then the next stage has landed, its first half is read under the second half's MFMAs.
+typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ const char* uniform(const void* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+    return (const char*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+// (inline asm: behind the builtin, every later LDS read would wait for all copies in flight)
+__device__ __forceinline__ void copy16(const char* base, unsigned off, unsigned lds) {
+    const unsigned m0 = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(m0) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
-__device__ __forceinline__ void tile_product(const Operand& P, const Operand& Q, int K, f16* sm, f32x16& acc) {
-    constexpr int RS = NS_K + 8;  // padded row (16-byte aligned)
-    f16* sp[2] = {sm, sm + 64 * RS};
-    f16* sq[2] = {sm + 2 * 64 * RS, sm + 3 * 64 * RS};
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = tid >> 2, kc = (tid & 3) * 8;
-    const int wr = (wave & 1) * 32 + (lane & 31), wc = (wave >> 1) * 32 + (lane & 31), kh = (lane >> 5) * 8;
-    for (int k0 = 0; k0 < K; k0 += NS_K) {
-        const f16x8 p0 = *reinterpret_cast<const f16x8*>(P.hi + row * P.ld + k0 + kc);
-        const f16x8 p1 = *reinterpret_cast<const f16x8*>(P.lo + row * P.ld + k0 + kc);
-        const f16x8 q0 = *reinterpret_cast<const f16x8*>(Q.hi + row * Q.ld + k0 + kc);
-        const f16x8 q1 = *reinterpret_cast<const f16x8*>(Q.lo + row * Q.ld + k0 + kc);
-        __syncthreads();
-        *reinterpret_cast<f16x8*>(sp[0] + row * RS + kc) = p0;
-        *reinterpret_cast<f16x8*>(sp[1] + row * RS + kc) = p1;
-        *reinterpret_cast<f16x8*>(sq[0] + row * RS + kc) = q0;
-        *reinterpret_cast<f16x8*>(sq[1] + row * RS + kc) = q1;
-        __syncthreads();
+// Values exchanged between blocks of one launch.  Each XCD has an L2 of its own: these go past it, store and load by
+// store and load, where a fence would write back and drop the whole L2 (measured: a 6 x 333 x 1000 batch in 4 parts per
+// tile took 2850 us with fences around the exchange).
+__device__ __forceinline__ void put_shared(uint64_t* p, float a, float b) {
+    const uint64_t v = (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_shared(const uint64_t* p) {
+    const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
+struct Rows {  // the rows of an operand's tile: its planes, first row, rows of the planes
+    const f16* hi;
+    const f16* lo;
+    int first, rows;
+};
+
+template <int WM, int WN> struct Frags {
+    f16x8 ph[WM], pl[WM], qh[WN], ql[WN];
+};
+
+template <int WM, int WN> struct Product {
+    static constexpr int TM = 64 * WM, TN = 64 * WN;
+    static constexpr int PB = TM * 64, QB = TN * 64;        // bytes of a plane's tile
+    static constexpr int STAGE = 2 * (PB + QB);
+    static constexpr int LDS = NS_BUF * STAGE;
+    static constexpr int COPIES = 2 * (WM + WN);            // of a wave and stage
+
+    __device__ static void load(const char* st, int half, Frags<WM, WN>& f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, run = 2 * half + (lane >> 5);
+        const int r0 = (wave & 1) * 32 * WM + l32, c0 = (wave >> 1) * 32 * WN + l32;
+        const int slot = 16 * (run ^ ((l32 >> 2) & 3));     // (rows differ by multiples of 16 between the fragments)
 #pragma unroll
-        for (int k = 0; k < NS_K; k += 16) {
-            const f16x8 ph = *reinterpret_cast<const f16x8*>(sp[0] + wr * RS + k + kh);
-            const f16x8 pl = *reinterpret_cast<const f16x8*>(sp[1] + wr * RS + k + kh);
-            const f16x8 qh = *reinterpret_cast<const f16x8*>(sq[0] + wc * RS + k + kh);
-            const f16x8 ql = *reinterpret_cast<const f16x8*>(sq[1] + wc * RS + k + kh);
-            acc = mfma16(ph, ql, acc);
-            acc = mfma16(pl, qh, acc);
-            acc = mfma16(ph, qh, acc);
+        for (int i = 0; i < WM; ++i) {
+            f.ph[i] = *reinterpret_cast<const f16x8*>(st + (r0 + 32 * i) * 64 + slot);
+            f.pl[i] = *reinterpret_cast<const f16x8*>(st + PB + (r0 + 32 * i) * 64 + slot);
+        }
+#pragma unroll
+        for (int i = 0; i < WN; ++i) {
+            f.qh[i] = *reinterpret_cast<const f16x8*>(st + 2 * PB + (c0 + 32 * i) * 64 + slot);
+            f.ql[i] = *reinterpret_cast<const f16x8*>(st + 2 * PB + QB + (c0 + 32 * i) * 64 + slot);
         }
     }
-}
+    __device__ static void multiply(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN]) {
+        // the small terms first; neighbouring instructions write different accumulators
+#pragma unroll
+        for (int i = 0; i < WM; ++i)
+#pragma unroll
+            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.ph[i], f.ql[j], acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < WM; ++i)
+#pragma unroll
+            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.pl[i], f.qh[j], acc[i][j]);
+#pragma unroll
+        for (int i = 0; i < WM; ++i)
+#pragma unroll
+            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.ph[i], f.qh[j], acc[i][j]);
+    }
 
-// C[c][r .. r+3] and, transposed, C[r .. r+3][c] of four values
-__device__ __forceinline__ void store_planes(f16* hi, f16* lo, int64_t ld, int r, int c, const f16x4& h, const f16x4& l) {
-    *reinterpret_cast<f16x4*>(hi + c * ld + r) = h;
-    *reinterpret_cast<f16x4*>(lo + c * ld + r) = l;
-}
-__device__ __forceinline__ void store_planes_t(f16* hi, f16* lo, int64_t ld, int r, int c, const f16x4& h, const f16x4& l) {
+    // stages [s0, s1) of K
+    __device__ static void run(const Rows& P, const Rows& Q, int s0, int s1, char* sm, f32x16 (&acc)[WM][WN]) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)sm;
+        unsigned offp[WM], offq[WN];  // (rows behind the planes' last: that one again, for sums that nobody stores)
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {  // this wave's 16-row groups wave, wave + 4, ...
+            const int r = (wave + 4 * i) * 16 + (lane >> 2);
+            offp[i] = (unsigned)(min(r, P.rows - P.first - 1) * 64 + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
+        }
+#pragma unroll
+        for (int i = 0; i < WN; ++i) {
+            const int r = (wave + 4 * i) * 16 + (lane >> 2);
+            offq[i] = (unsigned)(min(r, Q.rows - Q.first - 1) * 64 + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
+        }
+        const char* base[4] = {uniform(P.hi + P.first * 32), uniform(P.lo + P.first * 32), uniform(Q.hi + Q.first * 32),
+                               uniform(Q.lo + Q.first * 32)};
+        const auto issue = [&](int s, int buf) {
+            const unsigned at = lds0 + (unsigned)(buf * STAGE + wave * 1024);
+            const int64_t kp = (int64_t)s * P.rows * 64, kq = (int64_t)s * Q.rows * 64;
+#pragma unroll
+            for (int i = 0; i < WM; ++i) {
+                copy16(base[0] + kp, offp[i], at + i * 4096);
+                copy16(base[1] + kp, offp[i], at + PB + i * 4096);
+            }
+#pragma unroll
+            for (int i = 0; i < WN; ++i) {
+                copy16(base[2] + kq, offq[i], at + 2 * PB + i * 4096);
+                copy16(base[3] + kq, offq[i], at + 2 * PB + QB + i * 4096);
+            }
+        };
+        const int n = s1 - s0;
+        issue(s0, 0);
+        if (n > 1) issue(s0 + 1, 1);
+        if (n > 2) issue(s0 + 2, 2);
+        if (n > 2) wait_copies<2 * COPIES>();
+        else if (n > 1) wait_copies<COPIES>();
+        else wait_copies<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        Frags<WM, WN> f0, f1;
+        load(sm, 0, f0);
+        int buf = 0;
+        for (int s = 0; s < n; ++s) {
+            load(sm + buf * STAGE, 1, f1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f0, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < n) {
+                // every wave is done with this stage's buffer, and the next stage has landed
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (s + 2 < n) wait_copies<COPIES>();
+                else wait_copies<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (s + NS_BUF < n) issue(s0 + s + NS_BUF, buf);
+                buf = buf + 1 == NS_BUF ? 0 : buf + 1;
+                load(sm + buf * STAGE, 0, f0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            multiply(f1, acc);
+        }
+    }
+};
+
+__device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        hi[(r + j) * ld + c] = h[j];
-        lo[(r + j) * ld + c] = l[j];
+        f16 a, b;
+        split(v[j], a, b);
+        h[j] = a;
+        l[j] = b;
     }
 }
+enum NsPhase { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 
-// PHASE 0: A = X X^T.  1: B = b A + c A A.  Tiles (ti <= tj), the mirrored one written too.
-template <int PHASE> __global__ __launch_bounds__(256) void ns_sym_kernel(NsTable t, NsArgs q) {
-    __shared__ __attribute__((aligned(16))) f16 sm[4 * 64 * (NS_K + 8)];
-    const int ei = find_entry(t, blockIdx.x);
+// NS_GRAM: A = X X^T.  NS_POLY: B = b A + c A A.  Both symmetric: of each pair of 64-blocks across the diagonal one is
+// computed and written twice.  NS_APPLY: X <- a X + B X, both ways round.  NS_LAST: that to the caller's matrices.
+template <int PHASE, int WM, int WN> __global__ __launch_bounds__(256) void ns_product_kernel(NsTable t, NsUnits un, NsArgs q) {
+    using G = Product<WM, WN>;
+    constexpr bool SYM = PHASE <= NS_POLY;
+    extern __shared__ __attribute__((aligned(16))) char sm[];
+    __shared__ int last;
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
-    const int tm = e.mp / 64, per = tm * (tm + 1) / 2;
-    const int rel = blockIdx.x - t.first[ei], bat = rel / per;
-    int tj = 0, tl = rel % per;
-    while (tl > tj) tl -= ++tj;  // column tj holds tiles 0 .. tj
-    const int i0 = tl * 64, j0 = tj * 64;
+    const int rel = blockIdx.x - un.first[ei], whole = un.whole[ei], split = un.split[ei];
+    const int cut = un.tiles[ei] * e.batch - whole;
+    // split tiles in part order, and adjacent ones to one XCD: its units then share their K range
+    const int over = rel < whole ? -1 : xcd_order(rel - whole, cut * split);
+    const int tile = over < 0 ? rel : whole + over % cut, part = over < 0 ? 0 : over / cut;
+    const int bat = tile / un.tiles[ei];
+    int tl = tile % un.tiles[ei];
     const Planes p = planes_of(q, e, bat);
-    f32x16 acc{};
-    if (PHASE == 0) {
-        const Operand P{p.x(q.src, 0) + (int64_t)i0 * e.np, p.x(q.src, 1) + (int64_t)i0 * e.np, e.np};
-        const Operand Q{p.x(q.src, 0) + (int64_t)j0 * e.np, p.x(q.src, 1) + (int64_t)j0 * e.np, e.np};
-        tile_product(P, Q, e.np, sm, acc);
+    // rows r0 .., columns c0 .. of the product, and its operands.  The accumulators hold four adjacent rows per lane, so
+    // the side that lies along memory in the output gives the rows.
+    const bool tall = PHASE == NS_LAST && e.rows > e.cols;
+    int r0, c0;
+    Rows P, Q;
+    if (SYM) {
+        const int nc = (e.mp + G::TN - 1) / G::TN;
+        int ti = 0;
+        for (;; ++ti) {
+            const int w = min((WM / WN) * (ti + 1), nc);
+            if (tl < w) break;
+            tl -= w;
+        }
+        r0 = ti * G::TM;
+        c0 = tl * G::TN;
+        const f16* hi = PHASE == NS_GRAM ? p.x(q.src, 0) : p.a(0);
+        const f16* lo = PHASE == NS_GRAM ? p.x(q.src, 1) : p.a(1);
+        P = Rows{hi, lo, r0, e.mp};
+        Q = Rows{hi, lo, c0, e.mp};
     } else {
-        const Operand P{p.a(0) + (int64_t)i0 * e.mp, p.a(1) + (int64_t)i0 * e.mp, e.mp};
-        const Operand Q{p.a(0) + (int64_t)j0 * e.mp, p.a(1) + (int64_t)j0 * e.mp, e.mp};
-        tile_product(P, Q, e.mp, sm, acc);
+        const int tc = ((tall ? e.np : e.mp) + G::TN - 1) / G::TN;
+        r0 = (tl / tc) * G::TM;
+        c0 = (tl % tc) * G::TN;
+        const Rows B{p.b(0), p.b(1), tall ? r0 : c0, e.mp};
+        const Rows X{p.xt(q.src, 0), p.xt(q.src, 1), tall ? c0 : r0, e.np};
+        P = tall ? B : X;
+        Q = tall ? X : B;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = j0 + (wave >> 1) * 32 + (lane & 31);
+    const int stages = (int)((PHASE == NS_GRAM ? e.np : e.mp) / NS_K);
+    f32x16 acc[WM][WN];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int r = i0 + (wave & 1) * 32 + acc_row(4 * g, lane >> 5);
-        f16x4 h, l;
-        if (PHASE == 0) {
-            const float unit = q.unit[e.norm + bat], k = q.sa * unit * unit;
+    for (int i = 0; i < WM; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f16 a, b;
-                split(acc[4 * g + j] * k, a, b);
-                h[j] = a;
-                l[j] = b;
+        for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
+    if (over < 0) {
+        G::run(P, Q, 0, stages, sm, acc);
+    } else {
+        G::run(P, Q, (int)((int64_t)stages * part / split), (int)((int64_t)stages * (part + 1) / split), sm, acc);
+        if (split > 1) {
+            // the tile's parts meet in memory; the unit that ends last adds them in part order
+            constexpr int SZ = G::TM * G::TN;
+            uint64_t* mine = reinterpret_cast<uint64_t*>(q.joint + (int64_t)(un.joint[ei] + over) * SZ) + threadIdx.x;
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int j = 0; j < WN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 8; ++g)
+                        put_shared(mine + ((i * WN + j) * 8 + g) * 256, acc[i][j][2 * g], acc[i][j][2 * g + 1]);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (they have reached what every XCD reads)
+            __syncthreads();
+            unsigned* done = q.done + un.tail[ei] + over % cut;
+            if (threadIdx.x == 0)
+                last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)split - 1u;
+            __syncthreads();
+            if (!last) return;
+            if (threadIdx.x == 0) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+#pragma unroll
+            for (int i = 0; i < WM; ++i)
+#pragma unroll
+                for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
+            const uint64_t* from = reinterpret_cast<const uint64_t*>(q.joint + (int64_t)(un.joint[ei] + over % cut) * SZ) + threadIdx.x;
+            constexpr int FLY = 8 / (WM * WN) > 0 ? 8 / (WM * WN) : 1;  // parts in flight
+            for (int k = 0; k < split; k += FLY) {
+#pragma unroll
+                for (int i = 0; i < WM; ++i)
+#pragma unroll
+                    for (int j = 0; j < WN; ++j) {
+                        float2 v[FLY][8];
+#pragma unroll
+                        for (int f = 0; f < FLY; ++f)
+#pragma unroll
+                            for (int g = 0; g < 8; ++g)
+                                v[f][g] = get_shared(from + (int64_t)min(k + f, split - 1) * cut * (SZ / 2) + ((i * WN + j) * 8 + g) * 256);
+#pragma unroll
+                        for (int f = 0; f < FLY; ++f)
+                            if (k + f < split) {
+#pragma unroll
+                                for (int g = 0; g < 8; ++g) {
+                                    acc[i][j][2 * g] += v[f][g].x;
+                                    acc[i][j][2 * g + 1] += v[f][g].y;
+                                }
+                            }
+                    }
             }
-            store_planes(p.a(0), p.a(1), e.mp, r, c, h, l);
-            if (i0 != j0) store_planes_t(p.a(0), p.a(1), e.mp, r, c, h, l);
-        } else {
-            const f16x4 ah = *reinterpret_cast<const f16x4*>(p.a(0) + (int64_t)c * e.mp + r);
-            const f16x4 al = *reinterpret_cast<const f16x4*>(p.a(1) + (int64_t)c * e.mp + r);
-            const float k = q.c / q.sa;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f16 a, b;
-                split(fmaf(q.b, (float)ah[j] + (float)al[j], acc[4 * g + j] * k), a, b);
-                h[j] = a;
-                l[j] = b;
-            }
-            store_planes(p.b(0), p.b(1), e.mp, r, c, h, l);
-            if (i0 != j0) store_planes_t(p.b(0), p.b(1), e.mp, r, c, h, l);
         }
     }
-}
-
-// X <- a X + B X, as planes both ways round; LAST: to the caller's matrices instead
-template <bool LAST> __global__ __launch_bounds__(256) void ns_apply_kernel(NsTable t, NsArgs q) {
-    __shared__ __attribute__((aligned(16))) f16 sm[4 * 64 * (NS_K + 8)];
-    const int ei = find_entry(t, blockIdx.x);
-    const NsMat& e = t.e[ei];
-    const int tm = e.mp / 64, tn = e.np / 64, per = tm * tn;
-    const int rel = blockIdx.x - t.first[ei], bat = rel / per, tl = rel % per;
-    const int i0 = (tl / tn) * 64, j0 = (tl % tn) * 64;
-    const Planes p = planes_of(q, e, bat);
-    const Operand B{p.b(0) + (int64_t)i0 * e.mp, p.b(1) + (int64_t)i0 * e.mp, e.mp};
-    const Operand X{p.xt(q.src, 0) + (int64_t)j0 * e.mp, p.xt(q.src, 1) + (int64_t)j0 * e.mp, e.mp};
-    // the accumulator's rows (four adjacent per lane) run along the output's rows in memory
-    const bool tall = LAST && e.rows > e.cols;
-    f32x16 acc{};
-    if (tall) tile_product(B, X, e.mp, sm, acc);
-    else tile_product(X, B, e.mp, sm, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c = (tall ? j0 : i0) + (wave >> 1) * 32 + (lane & 31);
-    const float k = 1.f / q.sa;
-    const f16* xh = tall ? p.xt(q.src, 0) : p.x(q.src, 0);
-    const f16* xl = tall ? p.xt(q.src, 1) : p.x(q.src, 1);
-    const int64_t ld = tall ? e.mp : e.np;
+    // The tile goes through LDS, [column][row], so that both passes over it touch whole lines of memory: along the rows
+    // first, where the old values are added, then across.
+    constexpr int LS = G::TM + 1;
+    float* tv = reinterpret_cast<float*>(sm);
+    const float unit = q.unit[e.mat + bat];
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? q.c / q.sa : 1.f / q.sa;
+        __syncthreads();
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int r = (tall ? i0 : j0) + (wave & 1) * 32 + acc_row(4 * g, lane >> 5);
-        const f16x4 oh = *reinterpret_cast<const f16x4*>(xh + c * ld + r);
-        const f16x4 ol = *reinterpret_cast<const f16x4*>(xl + c * ld + r);
-        float v[4];
+        for (int i = 0; i < WM; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = fmaf(q.a, (float)oh[j] + (float)ol[j], acc[4 * g + j] * k);
-        if (!LAST) {
+            for (int j = 0; j < WN; ++j) {
+                float* at = tv + ((wave >> 1) * 32 * WN + 32 * j + (lane & 31)) * LS + (wave & 1) * 32 * WM + 32 * i;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) at[acc_row(x, lane >> 5)] = acc[i][j][x] * k;
+            }
+        __syncthreads();
+    }
+    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
+    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
+    const int orow = tall ? e.np : e.mp;  // rows of the old values' and the output's planes: the product's columns
+    const int nr = min(G::TM, (SYM || tall ? e.mp : e.np) - r0), nc = min(G::TN, (SYM ? e.mp : tall ? e.np : e.mp) - c0);
+    f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
+    f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
+#pragma unroll 4
+    for (int x = threadIdx.x; x < G::TM * G::TN / 4; x += 256) {
+        const int c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
+        if (r >= nr || c >= nc) continue;
+        if (SYM && (r0 + r) / 64 < (c0 + c) / 64) continue;  // (the mirrored block writes it)
+        float* at = tv + c * LS + r;
+        float v[4] = {at[0], at[1], at[2], at[3]};
+        const int64_t o = at_panel(c0 + c, r0 + r, orow);
+        if (PHASE != NS_GRAM) {
+            const f16x4 oh = *reinterpret_cast<const f16x4*>(oldh + o);
+            const f16x4 ol = *reinterpret_cast<const f16x4*>(oldl + o);
+            const float f = PHASE == NS_POLY ? q.b : q.a;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] = fmaf(f, (float)oh[y] + (float)ol[y], v[y]);
+        }
+        if (PHASE != NS_LAST) {
             f16x4 h, l;
+            split4(v, h, l);
+            *reinterpret_cast<f16x4*>(outh + o) = h;
+            *reinterpret_cast<f16x4*>(outl + o) = l;
+        }
+        if (PHASE >= NS_POLY) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f16 a, b;
-                split(v[j], a, b);
-                h[j] = a;
-                l[j] = b;
-            }
-            store_planes(p.x(1 - q.src, 0), p.x(1 - q.src, 1), e.np, r, c, h, l);
-            store_planes_t(p.xt(1 - q.src, 0), p.xt(1 - q.src, 1), e.mp, r, c, h, l);
-        } else {
-            const float u = q.unit[e.norm + bat];
-            if (c >= e.rows) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (r + j >= e.cols) continue;
-                const int64_t o = (int64_t)c * e.cols + r + j;
-                if (q.is_step) {
-                    float* w = static_cast<float*>(e.out);
-                    w[o] = fmaf(q.decay, w[o], -e.step * (v[j] * u));
-                } else {
-                    const int64_t ob = (int64_t)bat * e.rows * e.cols + o;
-                    if (q.dtype == PCX_F32) static_cast<float*>(e.out)[ob] = v[j] * u;
-                    else if (q.dtype == PCX_BF16) static_cast<bf16*>(e.out)[ob] = (bf16)(v[j] * u);
-                    else static_cast<f16*>(e.out)[ob] = (f16)(v[j] * u);
-                }
-            }
+            for (int y = 0; y < 4; ++y) at[y] = v[y];
         }
     }
+    __syncthreads();
+    if (PHASE != NS_LAST) {
+        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - q.src, 0) : outh;
+        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - q.src, 1) : outl;
+#pragma unroll 4
+        for (int x = threadIdx.x; x < G::TM * G::TN / 4; x += 256) {
+            const int r = x / 8 % G::TM, c = x % 8 * 4 + x / (8 * G::TM) * 32;
+            if (r >= nr || c >= nc) continue;
+            if (SYM && (r0 + r) / 64 <= (c0 + c) / 64) continue;
+            const float* at = tv + c * LS + r;
+            const float v[4] = {at[0], at[LS], at[2 * LS], at[3 * LS]};
+            f16x4 h, l;
+            split4(v, h, l);
+            const int64_t o = at_panel(r0 + r, c0 + c, PHASE == NS_APPLY ? e.np : e.mp);
+            *reinterpret_cast<f16x4*>(acrh + o) = h;
+            *reinterpret_cast<f16x4*>(acrl + o) = l;
+        }
+        return;
+    }
+    const auto finish = [&](auto kind, auto put) {
+        using T = decltype(kind);
+        T* out = static_cast<T*>(e.out) + (int64_t)bat * e.rows * e.cols;
+#pragma unroll 8
+        for (int x = threadIdx.x; x < G::TM * G::TN; x += 256) {
+            const int c = x / G::TM, r = x % G::TM;
+            if (r0 + r >= e.cols || c0 + c >= e.rows) continue;
+            T* o = out + (int64_t)(c0 + c) * e.cols + r0 + r;
+            *o = put(*o, tv[c * LS + r] * unit);
+        }
+    };
+    if (q.is_step) finish(float(), [&](float w, float v) { return fmaf(q.decay, w, -e.step * v); });
+    else if (q.dtype == PCX_F32) finish(float(), [](float, float v) { return v; });
+    else if (q.dtype == PCX_BF16) finish(bf16(), [](bf16, float v) { return (bf16)v; });
+    else finish(f16(), [](f16, float v) { return (f16)v; });
 }
 
 // ---------------------------------------------------------------- host
@@ -394,10 +641,9 @@ int round_up(int v, int k) { return (v + k - 1) / k * k; }
 void set_shape(NsMat& e, int64_t rows, int64_t cols) {
     e.rows = (int)rows;
     e.cols = (int)cols;
-    e.m = (int)std::min(rows, cols);
-    e.n = (int)std::max(rows, cols);
-    e.mp = round_up(e.m, NS_TILE);
-    e.np = round_up(e.n, NS_TILE);
+    e.mp = round_up((int)std::min(rows, cols), NS_PAD);
+    e.np = round_up((int)std::max(rows, cols), NS_PAD);
+    e.parts = (int)std::min<int64_t>(NS_PART, (rows * cols + 2047) / 2048);
 }
 
 // largest singular value any step can leave, starting in [0, 1], and the largest of |b s^2 + c s^4| on the way: by
@@ -423,21 +669,137 @@ void ns_bounds(const float* coef, int steps, double* smax, double* bmax, double*
     }
 }
 
-// One launch table's workspace: the partial sums and the unit of every matrix, then the planes, 256-byte aligned.
-int64_t ns_place(NsTable& t) {
-    int64_t mats = 0;
+template <int WM, int WN> struct Config {
+    static constexpr int wm = WM, wn = WN;
+};
+int ns_config(const NsTable& t, int phase) {
+    static const int force = getenv("NS_CFG") ? atoi(getenv("NS_CFG")) : -1;
+    if (force >= 0) return force;
+    return 0;
+}
+constexpr int NS_TM[3] = {64, 128, 256}, NS_TN[3] = {64, 128, 128}, NS_PER_CU[3] = {3, 1, 1};
+
+struct NsPlan {
+    NsUnits un;
+    int cfg;
+    unsigned blocks;
+    int64_t counters, joint;  // split tiles, floats of their parts
+};
+
+// Units of a product launch: as many as the card holds at a time (`slots`), of about the same number of stages.
+NsPlan ns_plan(const NsTable& t, int phase) {
+    NsPlan p{};
+    p.cfg = ns_config(t, phase);
+    const int TM = NS_TM[p.cfg], TN = NS_TN[p.cfg];
+    static const int least = getenv("NS_LEAST") ? atoi(getenv("NS_LEAST")) : 4, most = getenv("NS_MOST") ? atoi(getenv("NS_MOST")) : 1000;
+    const int64_t slots = (int64_t)num_cus() * NS_PER_CU[p.cfg];
+    int64_t work = 0, units = 0, parts = 0;
+    int stages[NS_LIST];
     for (int i = 0; i < t.count; ++i) {
-        t.e[i].norm = (int)mats;
+        const NsMat& e = t.e[i];
+        int64_t n = 0;
+        if (phase <= NS_POLY) {
+            const int nc = (e.mp + TN - 1) / TN;
+            for (int ti = 0; ti * TM < e.mp; ++ti) n += std::min(TM / TN * (ti + 1), nc);
+        } else {
+            const bool tall = phase == NS_LAST && e.rows > e.cols;
+            n = (int64_t)(((tall ? e.mp : e.np) + TM - 1) / TM) * (((tall ? e.np : e.mp) + TN - 1) / TN);
+        }
+        p.un.tiles[i] = (int)n;
+        stages[i] = (phase == NS_GRAM ? e.np : e.mp) / NS_K;
+        work += n * e.batch * stages[i];
+    }
+    const int64_t level = std::max<int64_t>(least, (work + slots - 1) / slots);
+    p.un.count = t.count;
+    for (int i = 0; i < t.count; ++i) {
+        const int64_t n = (int64_t)p.un.tiles[i] * t.e[i].batch;
+        int64_t whole, split;
+        if (t.count == 1 && n >= slots) {  // full rounds of whole tiles, the rest in parts
+            whole = n / slots * slots;
+            split = n > whole ? std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / least)) : 1;
+        } else {
+            whole = 0;
+            split = std::max<int64_t>(1, std::min<int64_t>((stages[i] + level - 1) / level, stages[i] / least));
+        }
+        split = std::min<int64_t>(split, most);
+        if (split == 1) whole = n;
+        p.un.whole[i] = (int)whole;
+        p.un.split[i] = (int)split;
+        p.un.tail[i] = (int)p.counters;
+        p.un.joint[i] = (int)parts;
+        p.un.first[i] = (int)units;
+        p.counters += n - whole;
+        parts += (n - whole) * split;
+        units += whole + (n - whole) * split;
+    }
+    p.un.first[t.count] = (int)units;
+    p.blocks = (unsigned)units;
+    p.joint = parts * TM * TN;
+    return p;
+}
+
+// Units of the passes over values: `per` blocks to a matrix of an entry.
+template <typename F> unsigned ns_blocks(const NsTable& t, NsUnits& un, F per) {
+    int64_t n = 0;
+    un.count = t.count;
+    for (int i = 0; i < t.count; ++i) {
+        un.first[i] = (int)n;
+        n += per(t.e[i]) * t.e[i].batch;
+    }
+    un.first[t.count] = (int)n;
+    return (unsigned)n;
+}
+
+// One launch table's workspace: partial sums and unit of every matrix, counters and partial products of split tiles,
+// then the planes.  Fills in the places; returns its size.
+int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
+    int64_t mats = 0, counters = 0, joint = 0;
+    for (int i = 0; i < t.count; ++i) {
+        t.e[i].mat = (int)mats;
         mats += t.e[i].batch;
     }
     t.mats = (int)mats;
-    int64_t off = mats * (NS_PART * (int64_t)sizeof(double) + (int64_t)sizeof(float));
+    for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
+        const NsPlan p = ns_plan(t, ph);
+        counters = std::max(counters, p.counters);
+        joint = std::max(joint, p.joint);
+    }
+    int64_t off = 0;
+    const auto take = [&](int64_t bytes) {
+        const int64_t at = off;
+        off = (off + bytes + 255) / 256 * 256;
+        return reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(ws) + (uintptr_t)at);
+    };
+    q.ws = static_cast<char*>(ws);
+    q.ndone = (int)counters;
+    char* a = take(mats * NS_PART * (int64_t)sizeof(double));
+    char* b = take(mats * (int64_t)sizeof(float));
+    char* c = take(counters * (int64_t)sizeof(unsigned));
+    char* d = take(joint * (int64_t)sizeof(float));
+    q.part = reinterpret_cast<double*>(a);
+    q.unit = reinterpret_cast<float*>(b);
+    q.done = reinterpret_cast<unsigned*>(c);
+    q.joint = reinterpret_cast<float*>(d);
     for (int i = 0; i < t.count; ++i) {
-        off = (off + 255) / 256 * 256;
         t.e[i].ws = off;
-        off += t.e[i].batch * plane_bytes(t.e[i].mp, t.e[i].np);
+        take(t.e[i].batch * plane_bytes(t.e[i].mp, t.e[i].np));
     }
     return off;
+}
+
+template <int PHASE, int WM, int WN> int ns_product_as(const NsTable& t, const NsPlan& p, const NsArgs& q, hipStream_t s) {
+    constexpr int sm = Product<WM, WN>::LDS;
+    if (sm > 64 * 1024)
+        (void)hipFuncSetAttribute((const void*)ns_product_kernel<PHASE, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+    ns_product_kernel<PHASE, WM, WN><<<p.blocks, 256, sm, s>>>(t, p.un, q);
+    PCX_LAUNCH_CHECK("ns_product_kernel");
+    return PCX_OK;
+}
+template <int PHASE> int ns_product(const NsTable& t, const NsArgs& q, hipStream_t s) {
+    const NsPlan p = ns_plan(t, PHASE);
+    if (p.cfg == 0) return ns_product_as<PHASE, 1, 1>(t, p, q, s);
+    if (p.cfg == 1) return ns_product_as<PHASE, 2, 2>(t, p, q, s);
+    return ns_product_as<PHASE, 4, 2>(t, p, q, s);
 }
 
 int ns_scales(NsArgs& q, const float* coef, int steps) {
@@ -450,39 +812,23 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
     return PCX_OK;
 }
 
-int ns_run(NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
-    q.unit = reinterpret_cast<float*>(q.part + (int64_t)t.mats * NS_PART);
-    auto blocks = [&](auto per) {
-        int64_t n = 0;
-        for (int i = 0; i < t.count; ++i) {
-            t.first[i] = (int)n;
-            n += per(t.e[i]) * t.e[i].batch;
-        }
-        t.first[t.count] = (int)n;
-        return (unsigned)n;
-    };
-    const auto full = [](const NsMat& e) { return (int64_t)(e.mp / 64) * (e.np / 64); };
-    const auto half = [](const NsMat& e) { return (int64_t)(e.mp / 64) * (e.mp / 64 + 1) / 2; };
-    unsigned n = blocks([](const NsMat&) { return (int64_t)NS_PART; });
-    ns_norm_kernel<<<n, 256, 0, s>>>(t, q);
+int ns_run(const NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
+    NsUnits un{};
+    unsigned n = ns_blocks(t, un, [](const NsMat& e) { return (int64_t)e.parts; });
+    ns_norm_kernel<<<n, 256, 0, s>>>(t, un, q);
     PCX_LAUNCH_CHECK("ns_norm_kernel");
-    n = blocks(full);
-    ns_split_kernel<<<n, 256, 0, s>>>(t, q);
+    n = ns_blocks(t, un, [](const NsMat& e) { return (int64_t)(e.mp / 64) * (e.np / 64); });
+    ns_split_kernel<<<n, 256, 0, s>>>(t, un, q);
     PCX_LAUNCH_CHECK("ns_split_kernel");
     for (int k = 0; k < steps; ++k) {
         q.a = coef[3 * k];
         q.b = coef[3 * k + 1];
         q.c = coef[3 * k + 2];
         q.src = k & 1;
-        n = blocks(half);
-        ns_sym_kernel<0><<<n, 256, 0, s>>>(t, q);
-        PCX_LAUNCH_CHECK("ns_sym_kernel");
-        ns_sym_kernel<1><<<n, 256, 0, s>>>(t, q);
-        PCX_LAUNCH_CHECK("ns_sym_kernel");
-        n = blocks(full);
-        if (k + 1 < steps) ns_apply_kernel<false><<<n, 256, 0, s>>>(t, q);
-        else ns_apply_kernel<true><<<n, 256, 0, s>>>(t, q);
-        PCX_LAUNCH_CHECK("ns_apply_kernel");
+        int rc = ns_product<NS_GRAM>(t, q, s);
+        if (!rc) rc = ns_product<NS_POLY>(t, q, s);
+        if (!rc) rc = k + 1 < steps ? ns_product<NS_APPLY>(t, q, s) : ns_product<NS_LAST>(t, q, s);
+        if (rc) return rc;
     }
     return PCX_OK;
 }
@@ -514,7 +860,7 @@ bool ns_shape_ok(int64_t batch, int64_t rows, int64_t cols) {
     // tile and block counts stay in 32 bits
     if (batch < 0 || rows < 1 || cols < 1 || std::max(rows, cols) > 1 << 20 || std::min(rows, cols) > 1 << 14) return false;
     const int64_t tiles = ((rows + 63) / 64) * ((cols + 63) / 64) + NS_PART;
-    return rows * cols <= (int64_t)1 << 31 && batch < (int64_t)1 << 24 && batch * tiles < (int64_t)1 << 30;
+    return rows * cols <= (int64_t)1 << 31 && batch < (int64_t)1 << 24 && batch * tiles < (int64_t)1 << 26;
 }
 
 int ns_check(const char* what, int steps, const float* coef, float eps) {
@@ -542,6 +888,8 @@ int muon_part(const pcx_muon_matrix* mats, int n, int at, NsTable& t) {
         set_shape(e, a.rows, a.cols);
         e.batch = 1;
         e.x = a.grad;
+        e.xr = a.cols;
+        e.xc = 1;
         e.out = a.param;
         e.mom = a.momentum;
     }
@@ -556,8 +904,9 @@ using namespace pcx;
 extern "C" size_t pcx_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
     if (!ns_shape_ok(batch, rows, cols) || batch == 0) return 0;
     NsTable t{};
+    NsArgs q{};
     ns_single(t, batch, rows, cols);
-    return (size_t)ns_place(t);
+    return (size_t)ns_place(t, q, nullptr);
 }
 
 extern "C" int pcx_orthogonalize(int dtype, int64_t batch, int64_t rows, int64_t cols, const void* x, int64_t batch_stride,
@@ -574,7 +923,7 @@ extern "C" int pcx_orthogonalize(int dtype, int64_t batch, int64_t rows, int64_t
     PCX_CHECK_ARG(x && out, "orthogonalize: NULL buffer");
     NsTable t{};
     ns_single(t, batch, rows, cols);
-    const int64_t need = ns_place(t);
+    const int64_t need = ns_place(t, q, ws);
     if (!ws || (int64_t)ws_bytes < need) {
         set_error("orthogonalize: workspace of %zu bytes, %lld needed", ws_bytes, (long long)need);
         return PCX_EWORKSPACE;
@@ -585,8 +934,6 @@ extern "C" int pcx_orthogonalize(int dtype, int64_t batch, int64_t rows, int64_t
     e.xr = row_stride;
     e.xc = col_stride;
     e.out = out;
-    q.ws = static_cast<char*>(ws);
-    q.part = static_cast<double*>(ws);
     q.dtype = dtype;
     q.eps = eps;
     return ns_run(t, q, coef, steps, stream);
@@ -597,8 +944,9 @@ extern "C" size_t pcx_muon_workspace_bytes(const pcx_muon_matrix* mats, int n) {
     int64_t most = 0;
     for (int at = 0; at < n; at += NS_LIST) {
         NsTable t{};
+        NsArgs q{};
         if (muon_part(mats, n, at, t) != PCX_OK) return 0;
-        most = std::max(most, ns_place(t));
+        most = std::max(most, ns_place(t, q, nullptr));
     }
     return (size_t)most;
 }
@@ -619,14 +967,12 @@ extern "C" int pcx_muon_step(const pcx_muon_matrix* mats, int n, float lr, float
         if (rc) return rc;
         for (int i = 0; i < t.count; ++i)
             PCX_CHECK_ARG(t.e[i].x && t.e[i].out && t.e[i].mom, "muon_step: NULL buffer of matrix %d", at + i);
-        const int64_t need = ns_place(t);
+        const int64_t need = ns_place(t, q, ws);
         if (!ws || (int64_t)ws_bytes < need) {
             set_error("muon_step: workspace of %zu bytes, %lld needed", ws_bytes, (long long)need);
             return PCX_EWORKSPACE;
         }
     }
-    q.ws = static_cast<char*>(ws);
-    q.part = static_cast<double*>(ws);
     q.is_step = 1;
     q.nesterov = nesterov != 0;
     q.mu = momentum;
@@ -637,7 +983,7 @@ extern "C" int pcx_muon_step(const pcx_muon_matrix* mats, int n, float lr, float
         NsTable t{};
         rc = muon_part(mats, n, at, t);
         if (rc) return rc;
-        ns_place(t);
+        ns_place(t, q, ws);
         for (int i = 0; i < t.count; ++i) t.e[i].step = lr * mats[at + i].scale;
         rc = ns_run(t, q, coef, steps, stream);
         if (rc) return rc;
