@@ -27,6 +27,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -330,42 +331,57 @@ template <int WM, int WN> struct Frags {
     f16x8 ph[WM], pl[WM], qh[WN], ql[WN];
 };
 
-template <int WM, int WN> struct Product {
+template <int WM, int WN, int NB> struct Product {
     static constexpr int TM = 64 * WM, TN = 64 * WN;
     static constexpr int PB = TM * 64, QB = TN * 64;        // bytes of a plane's tile
     static constexpr int STAGE = 2 * (PB + QB);
-    static constexpr int LDS = NS_BUF * STAGE;
+    static constexpr int LDS = NB * STAGE > (TM + 1) * TN * 4 ? NB * STAGE : (TM + 1) * TN * 4;  // (the epilogue's tile)
     static constexpr int COPIES = 2 * (WM + WN);            // of a wave and stage
 
-    __device__ static void load(const char* st, int half, Frags<WM, WN>& f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l32 = lane & 31, run = 2 * half + (lane >> 5);
-        const int r0 = (wave & 1) * 32 * WM + l32, c0 = (wave >> 1) * 32 * WN + l32;
-        const int slot = 16 * (run ^ ((l32 >> 2) & 3));     // (rows differ by multiples of 16 between the fragments)
-#pragma unroll
-        for (int i = 0; i < WM; ++i) {
-            f.ph[i] = *reinterpret_cast<const f16x8*>(st + (r0 + 32 * i) * 64 + slot);
-            f.pl[i] = *reinterpret_cast<const f16x8*>(st + PB + (r0 + 32 * i) * 64 + slot);
-        }
-#pragma unroll
-        for (int i = 0; i < WN; ++i) {
-            f.qh[i] = *reinterpret_cast<const f16x8*>(st + 2 * PB + (c0 + 32 * i) * 64 + slot);
-            f.ql[i] = *reinterpret_cast<const f16x8*>(st + 2 * PB + QB + (c0 + 32 * i) * 64 + slot);
+    static constexpr int READS = 2 * (WM + WN), MFMAS = 3 * WM * WN;
+
+    // operand t of a stage's half, this lane's 8 values
+    __device__ static const char* operand_at(const char* st, int half) {
+        const int lane = threadIdx.x & 63, l32 = lane & 31, run = 2 * half + (lane >> 5);
+        return st + l32 * 64 + 16 * (run ^ ((l32 >> 2) & 3));  // (rows differ by multiples of 32 between the operands)
+    }
+    template <int T> __device__ static void read(const char* at, Frags<WM, WN>& f) {
+        const int wave = threadIdx.x >> 6;
+        const char* p = at + (wave & 1) * 2048 * WM;
+        const char* c = at + 2 * PB + (wave >> 1) * 2048 * WN;
+        if constexpr (T < WM) f.ph[T] = *reinterpret_cast<const f16x8*>(p + 2048 * T);
+        else if constexpr (T < WM + WN) f.ql[T - WM] = *reinterpret_cast<const f16x8*>(c + QB + 2048 * (T - WM));
+        else if constexpr (T < 2 * WM + WN) f.pl[T - WM - WN] = *reinterpret_cast<const f16x8*>(p + PB + 2048 * (T - WM - WN));
+        else f.qh[T - 2 * WM - WN] = *reinterpret_cast<const f16x8*>(c + 2048 * (T - 2 * WM - WN));
+    }
+    // MFMA t of a half: the small terms first, neighbours in different accumulators
+    template <int T> __device__ static void mfma(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN]) {
+        constexpr int term = T / (WM * WN), i = T / WN % WM, j = T % WN;
+        acc[i][j] = mfma16(term == 1 ? f.pl[i] : f.ph[i], term == 0 ? f.ql[j] : f.qh[j], acc[i][j]);
+    }
+    // One half's MFMAs with the next half's operand reads (and a stage's copies, `fetch`) spread between them: all the
+    // reads in one run fill the LDS queue, and a wave's MFMAs wait behind its own reads.
+    template <int T = 0, typename F>
+    __device__ __forceinline__ static void half_step(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN], const char* next, Frags<WM, WN>& g, F fetch) {
+        if constexpr (T < READS) {
+            read<T>(next, g);
+            fetch(std::integral_constant<int, T>());
+            mfmas<T * MFMAS / READS, (T + 1) * MFMAS / READS>(f, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            half_step<T + 1>(f, acc, next, g, fetch);
         }
     }
-    __device__ static void multiply(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN]) {
-        // the small terms first; neighbouring instructions write different accumulators
-#pragma unroll
-        for (int i = 0; i < WM; ++i)
-#pragma unroll
-            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.ph[i], f.ql[j], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < WM; ++i)
-#pragma unroll
-            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.pl[i], f.qh[j], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < WM; ++i)
-#pragma unroll
-            for (int j = 0; j < WN; ++j) acc[i][j] = mfma16(f.ph[i], f.qh[j], acc[i][j]);
+    template <int A, int B> __device__ static void mfmas(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN]) {
+        if constexpr (A < B) {
+            mfma<A>(f, acc);
+            mfmas<A + 1, B>(f, acc);
+        }
+    }
+    template <int T = 0> __device__ static void read_all(const char* at, Frags<WM, WN>& f) {
+        if constexpr (T < READS) {
+            read<T>(at, f);
+            read_all<T + 1>(at, f);
+        }
     }
 
     // stages [s0, s1) of K
@@ -385,50 +401,51 @@ template <int WM, int WN> struct Product {
         }
         const char* base[4] = {uniform(P.hi + P.first * 32), uniform(P.lo + P.first * 32), uniform(Q.hi + Q.first * 32),
                                uniform(Q.lo + Q.first * 32)};
-        const auto issue = [&](int s, int buf) {
+        // copy T of this wave for a stage
+        const auto copy = [&](auto t, int s, int buf) {
+            constexpr int T = decltype(t)::value, pl = T / (WM + WN), x = T % (WM + WN);
             const unsigned at = lds0 + (unsigned)(buf * STAGE + wave * 1024);
-            const int64_t kp = (int64_t)s * P.rows * 64, kq = (int64_t)s * Q.rows * 64;
-#pragma unroll
-            for (int i = 0; i < WM; ++i) {
-                copy16(base[0] + kp, offp[i], at + i * 4096);
-                copy16(base[1] + kp, offp[i], at + PB + i * 4096);
-            }
-#pragma unroll
-            for (int i = 0; i < WN; ++i) {
-                copy16(base[2] + kq, offq[i], at + 2 * PB + i * 4096);
-                copy16(base[3] + kq, offq[i], at + 2 * PB + QB + i * 4096);
-            }
+            if constexpr (x < WM) copy16(base[pl] + (int64_t)s * P.rows * 64, offp[x], at + pl * PB + x * 4096);
+            else copy16(base[2 + pl] + (int64_t)s * Q.rows * 64, offq[x - WM], at + 2 * PB + pl * QB + (x - WM) * 4096);
         };
         const int n = s1 - s0;
-        issue(s0, 0);
-        if (n > 1) issue(s0 + 1, 1);
-        if (n > 2) issue(s0 + 2, 2);
-        if (n > 2) wait_copies<2 * COPIES>();
+        copies(copy, s0, 0);
+        if (n > 1) copies(copy, s0 + 1, 1);
+        if (NB > 2 && n > 2) copies(copy, s0 + 2, 2);
+        if (NB > 2 && n > 2) wait_copies<2 * COPIES>();
         else if (n > 1) wait_copies<COPIES>();
         else wait_copies<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         Frags<WM, WN> f0, f1;
-        load(sm, 0, f0);
-        int buf = 0;
-        for (int s = 0; s < n; ++s) {
-            load(sm + buf * STAGE, 1, f1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(f0, acc);
-            __builtin_amdgcn_sched_barrier(0);
-            if (s + 1 < n) {
-                // every wave is done with this stage's buffer, and the next stage has landed
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (s + 2 < n) wait_copies<COPIES>();
-                else wait_copies<0>();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                if (s + NS_BUF < n) issue(s0 + s + NS_BUF, buf);
-                buf = buf + 1 == NS_BUF ? 0 : buf + 1;
-                load(sm + buf * STAGE, 0, f0);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            multiply(f1, acc);
+        read_all(operand_at(sm, 0), f0);
+        int buf = 0, s = 0;
+        // (two loops and no branch inside: a join would move all accumulators)
+        for (; s + NB < n; ++s) {
+            half_step(f0, acc, operand_at(sm + buf * STAGE, 1), f1, [](auto) {});
+            turn<(NB - 2) * COPIES>();
+            const int freed = buf;
+            buf = buf + 1 == NB ? 0 : buf + 1;
+            half_step(f1, acc, operand_at(sm + buf * STAGE, 0), f0, [&](auto t) { copy(t, s0 + s + NB, freed); });
+        }
+        for (; s < n; ++s) {  // (the operands read behind the last stage are not used)
+            half_step(f0, acc, operand_at(sm + buf * STAGE, 1), f1, [](auto) {});
+            turn<0>();
+            buf = buf + 1 == NB ? 0 : buf + 1;
+            half_step(f1, acc, operand_at(sm + buf * STAGE, 0), f0, [](auto) {});
+        }
+    }
+    // every wave is done with the stage's buffer, and the next stage has landed
+    template <int N> __device__ __forceinline__ static void turn() {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_copies<N>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+    template <int T = 0, typename F> __device__ static void copies(F copy, int s, int buf) {
+        if constexpr (T < COPIES) {
+            copy(std::integral_constant<int, T>(), s, buf);
+            copies<T + 1>(copy, s, buf);
         }
     }
 };
@@ -446,20 +463,21 @@ enum NsPhase { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 
 // NS_GRAM: A = X X^T.  NS_POLY: B = b A + c A A.  Both symmetric: of each pair of 64-blocks across the diagonal one is
 // computed and written twice.  NS_APPLY: X <- a X + B X, both ways round.  NS_LAST: that to the caller's matrices.
-template <int PHASE, int WM, int WN> __global__ __launch_bounds__(256) void ns_product_kernel(NsTable t, NsUnits un, NsArgs q) {
-    using G = Product<WM, WN>;
+template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) void ns_product_kernel(NsTable t, NsUnits un, NsArgs q) {
+    using G = Product<WM, WN, NB>;
     constexpr bool SYM = PHASE <= NS_POLY;
     extern __shared__ __attribute__((aligned(16))) char sm[];
     __shared__ int last;
     const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
-    const int rel = blockIdx.x - un.first[ei], whole = un.whole[ei], split = un.split[ei];
-    const int cut = un.tiles[ei] * e.batch - whole;
+    const unsigned rel = blockIdx.x - un.first[ei], whole = un.whole[ei], split = un.split[ei], tiles = un.tiles[ei];
+    const unsigned cut = tiles * e.batch - whole;
     // split tiles in part order, and adjacent ones to one XCD: its units then share their K range
     const int over = rel < whole ? -1 : xcd_order(rel - whole, cut * split);
-    const int tile = over < 0 ? rel : whole + over % cut, part = over < 0 ? 0 : over / cut;
-    const int bat = tile / un.tiles[ei];
-    int tl = tile % un.tiles[ei];
+    const int part = over < 0 ? 0 : (unsigned)over / cut;
+    const unsigned tile = over < 0 ? rel : whole + over - part * cut;
+    const int bat = e.batch == 1 ? 0 : tile / tiles;
+    int tl = tile - bat * tiles;
     const Planes p = planes_of(q, e, bat);
     // rows r0 .., columns c0 .. of the product, and its operands.  The accumulators hold four adjacent rows per lane, so
     // the side that lies along memory in the output gives the rows.
@@ -482,24 +500,43 @@ template <int PHASE, int WM, int WN> __global__ __launch_bounds__(256) void ns_p
         Q = Rows{hi, lo, c0, e.mp};
     } else {
         const int tc = ((tall ? e.np : e.mp) + G::TN - 1) / G::TN;
-        r0 = (tl / tc) * G::TM;
-        c0 = (tl % tc) * G::TN;
+        const int tr = (unsigned)tl / (unsigned)tc;
+        r0 = tr * G::TM;
+        c0 = (tl - tr * tc) * G::TN;
         const Rows B{p.b(0), p.b(1), tall ? r0 : c0, e.mp};
         const Rows X{p.xt(q.src, 0), p.xt(q.src, 1), tall ? c0 : r0, e.np};
         P = tall ? B : X;
         Q = tall ? X : B;
     }
     const int stages = (int)((PHASE == NS_GRAM ? e.np : e.mp) / NS_K);
+    // the old values of small tiles are on their way during the product (these are latency, not throughput)
+    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
+    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
+    const int orow = tall ? e.np : e.mp;  // rows of the old values' and the output's planes: the product's columns
+    const int nr = min(G::TM, (SYM || tall ? e.mp : e.np) - r0), nc = min(G::TN, (SYM ? e.mp : tall ? e.np : e.mp) - c0);
+    constexpr bool EARLY = WM * WN == 1 && PHASE != NS_GRAM;
+    f16x4 eh[EARLY ? 4 : 1], el[EARLY ? 4 : 1];
+    if (EARLY) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const int x = threadIdx.x + 256 * y, c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
+            const int64_t o = at_panel(c0 + c, r0 + r, orow);  // (64 x 64: nothing reaches over the padding)
+            eh[y] = *reinterpret_cast<const f16x4*>(oldh + o);
+            el[y] = *reinterpret_cast<const f16x4*>(oldl + o);
+        }
+    }
+    const float unit = q.unit[e.mat + bat];
     f32x16 acc[WM][WN];
 #pragma unroll
     for (int i = 0; i < WM; ++i)
 #pragma unroll
         for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
-    if (over < 0) {
-        G::run(P, Q, 0, stages, sm, acc);
-    } else {
-        G::run(P, Q, (int)((int64_t)stages * part / split), (int)((int64_t)stages * (part + 1) / split), sm, acc);
-        if (split > 1) {
+    // (a matrix of 2^20 columns has 2^15 stages, and at most 16 parts)
+    const int s0 = over < 0 ? 0 : (int)((unsigned)(stages * part) / (unsigned)split);
+    const int s1 = over < 0 ? stages : (int)((unsigned)(stages * (part + 1)) / (unsigned)split);
+    G::run(P, Q, s0, s1, sm, acc);
+    if (over >= 0) {
+        {
             // the tile's parts meet in memory; the unit that ends last adds them in part order
             constexpr int SZ = G::TM * G::TN;
             uint64_t* mine = reinterpret_cast<uint64_t*>(q.joint + (int64_t)(un.joint[ei] + over) * SZ) + threadIdx.x;
@@ -552,7 +589,6 @@ template <int PHASE, int WM, int WN> __global__ __launch_bounds__(256) void ns_p
     // first, where the old values are added, then across.
     constexpr int LS = G::TM + 1;
     float* tv = reinterpret_cast<float*>(sm);
-    const float unit = q.unit[e.mat + bat];
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? q.c / q.sa : 1.f / q.sa;
@@ -567,23 +603,19 @@ template <int PHASE, int WM, int WN> __global__ __launch_bounds__(256) void ns_p
             }
         __syncthreads();
     }
-    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
-    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
-    const int orow = tall ? e.np : e.mp;  // rows of the old values' and the output's planes: the product's columns
-    const int nr = min(G::TM, (SYM || tall ? e.mp : e.np) - r0), nc = min(G::TN, (SYM ? e.mp : tall ? e.np : e.mp) - c0);
     f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
     f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
 #pragma unroll 4
-    for (int x = threadIdx.x; x < G::TM * G::TN / 4; x += 256) {
-        const int c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
+    for (int x0 = 0; x0 < G::TM * G::TN / 4; x0 += 256) {
+        const int x = x0 + threadIdx.x, c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
         if (r >= nr || c >= nc) continue;
         if (SYM && (r0 + r) / 64 < (c0 + c) / 64) continue;  // (the mirrored block writes it)
         float* at = tv + c * LS + r;
         float v[4] = {at[0], at[1], at[2], at[3]};
         const int64_t o = at_panel(c0 + c, r0 + r, orow);
         if (PHASE != NS_GRAM) {
-            const f16x4 oh = *reinterpret_cast<const f16x4*>(oldh + o);
-            const f16x4 ol = *reinterpret_cast<const f16x4*>(oldl + o);
+            const f16x4 oh = EARLY ? eh[EARLY ? x0 / 256 : 0] : *reinterpret_cast<const f16x4*>(oldh + o);
+            const f16x4 ol = EARLY ? el[EARLY ? x0 / 256 : 0] : *reinterpret_cast<const f16x4*>(oldl + o);
             const float f = PHASE == NS_POLY ? q.b : q.a;
 #pragma unroll
             for (int y = 0; y < 4; ++y) v[y] = fmaf(f, (float)oh[y] + (float)ol[y], v[y]);
@@ -677,7 +709,7 @@ int ns_config(const NsTable& t, int phase) {
     if (force >= 0) return force;
     return 0;
 }
-constexpr int NS_TM[3] = {64, 128, 256}, NS_TN[3] = {64, 128, 128}, NS_PER_CU[3] = {3, 1, 1};
+constexpr int NS_TM[5] = {64, 128, 256, 128, 64}, NS_TN[5] = {64, 128, 128, 128, 64}, NS_PER_CU[5] = {3, 1, 1, 2, 4};
 
 struct NsPlan {
     NsUnits un;
@@ -691,9 +723,9 @@ NsPlan ns_plan(const NsTable& t, int phase) {
     NsPlan p{};
     p.cfg = ns_config(t, phase);
     const int TM = NS_TM[p.cfg], TN = NS_TN[p.cfg];
-    static const int least = getenv("NS_LEAST") ? atoi(getenv("NS_LEAST")) : 4, most = getenv("NS_MOST") ? atoi(getenv("NS_MOST")) : 1000;
+    static const int most = getenv("NS_MOST") ? atoi(getenv("NS_MOST")) : 16;
     const int64_t slots = (int64_t)num_cus() * NS_PER_CU[p.cfg];
-    int64_t work = 0, units = 0, parts = 0;
+    int64_t units = 0, parts = 0;
     int stages[NS_LIST];
     for (int i = 0; i < t.count; ++i) {
         const NsMat& e = t.e[i];
@@ -707,19 +739,18 @@ NsPlan ns_plan(const NsTable& t, int phase) {
         }
         p.un.tiles[i] = (int)n;
         stages[i] = (phase == NS_GRAM ? e.np : e.mp) / NS_K;
-        work += n * e.batch * stages[i];
     }
-    const int64_t level = std::max<int64_t>(least, (work + slots - 1) / slots);
     p.un.count = t.count;
+    int64_t all = 0;
+    for (int i = 0; i < t.count; ++i) all += (int64_t)p.un.tiles[i] * t.e[i].batch;
     for (int i = 0; i < t.count; ++i) {
         const int64_t n = (int64_t)p.un.tiles[i] * t.e[i].batch;
-        int64_t whole, split;
+        int64_t whole = 0, split = 1;
         if (t.count == 1 && n >= slots) {  // full rounds of whole tiles, the rest in parts
             whole = n / slots * slots;
-            split = n > whole ? std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / least)) : 1;
-        } else {
-            whole = 0;
-            split = std::max<int64_t>(1, std::min<int64_t>((stages[i] + level - 1) / level, stages[i] / least));
+            if (n > whole) split = std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / 16));
+        } else if (stages[i] >= 48) {
+            split = std::min<int64_t>((int64_t)(sqrt(0.6 * stages[i]) + 0.5), std::max<int64_t>(1, slots / all));
         }
         split = std::min<int64_t>(split, most);
         if (split == 1) whole = n;
@@ -787,19 +818,21 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
     return off;
 }
 
-template <int PHASE, int WM, int WN> int ns_product_as(const NsTable& t, const NsPlan& p, const NsArgs& q, hipStream_t s) {
-    constexpr int sm = Product<WM, WN>::LDS;
+template <int PHASE, int WM, int WN, int NB> int ns_product_as(const NsTable& t, const NsPlan& p, const NsArgs& q, hipStream_t s) {
+    constexpr int sm = Product<WM, WN, NB>::LDS;
     if (sm > 64 * 1024)
-        (void)hipFuncSetAttribute((const void*)ns_product_kernel<PHASE, WM, WN>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-    ns_product_kernel<PHASE, WM, WN><<<p.blocks, 256, sm, s>>>(t, p.un, q);
+        (void)hipFuncSetAttribute((const void*)ns_product_kernel<PHASE, WM, WN, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+    ns_product_kernel<PHASE, WM, WN, NB><<<p.blocks, 256, sm, s>>>(t, p.un, q);
     PCX_LAUNCH_CHECK("ns_product_kernel");
     return PCX_OK;
 }
 template <int PHASE> int ns_product(const NsTable& t, const NsArgs& q, hipStream_t s) {
     const NsPlan p = ns_plan(t, PHASE);
-    if (p.cfg == 0) return ns_product_as<PHASE, 1, 1>(t, p, q, s);
-    if (p.cfg == 1) return ns_product_as<PHASE, 2, 2>(t, p, q, s);
-    return ns_product_as<PHASE, 4, 2>(t, p, q, s);
+    if (p.cfg == 0) return ns_product_as<PHASE, 1, 1, 3>(t, p, q, s);
+    if (p.cfg == 1) return ns_product_as<PHASE, 2, 2, 3>(t, p, q, s);
+    if (p.cfg == 3) return ns_product_as<PHASE, 2, 2, 2>(t, p, q, s);
+    if (p.cfg == 4) return ns_product_as<PHASE, 1, 1, 2>(t, p, q, s);
+    return ns_product_as<PHASE, 4, 2, 3>(t, p, q, s);
 }
 
 int ns_scales(NsArgs& q, const float* coef, int steps) {
