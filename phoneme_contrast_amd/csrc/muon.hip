@@ -43,6 +43,7 @@ constexpr int NS_LIST = 24;      // entries per launch (their table is a kernel 
 constexpr int NS_PAD = 64;       // X, A, B are padded to it; tiles that reach over the padding read their last rows again
 constexpr int NS_K = 32;         // K values of a stage
 constexpr int NS_BUF = 3;        // stages in LDS: one computed on, two on their way
+constexpr int NS_STEPS = 64;     // most steps
 constexpr int NS_PART = 512;     // most partial sums of squares per matrix
 
 struct NsMat {
@@ -72,6 +73,11 @@ struct NsUnits {
     int tail[NS_LIST];           // first counter of the entry's split tiles
     int joint[NS_LIST];          // first of their parts' sums
     int count;
+};
+
+struct NsCoef {
+    int steps;
+    float c[3 * NS_STEPS];
 };
 
 struct NsArgs {
@@ -133,9 +139,19 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
     if (dtype == PCX_BF16) return (float)static_cast<const bf16*>(p)[i];
     return (float)static_cast<const f16*>(p)[i];
 }
-__device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
-    hi = (f16)v;
-    lo = (f16)(v - (float)hi);
+// v = hi + lo to 2^-24 of v: hi by pairs in one conversion, lo = f16(v - hi) in one mixed-precision instruction each
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void split2(float a, float b, f16x2& hi, f16x2& lo) {
+    hi = __builtin_convertvector((f32x2{a, b}), f16x2);
+    lo = f16x2{(f16)fmaf((float)hi[0], -1.f, a), (f16)fmaf((float)hi[1], -1.f, b)};
+}
+__device__ __forceinline__ void split4(const float* v, f16x4& hi, f16x4& lo) {
+    f16x2 h0, l0, h1, l1;
+    split2(v[0], v[1], h0, l0);
+    split2(v[2], v[3], h1, l1);
+    hi = f16x4{h0[0], h0[1], h1[0], h1[1]};
+    lo = f16x4{l0[0], l0[1], l1[0], l1[1]};
 }
 
 // the momentum update of one element -> u (the same operations in both passes that need u)
@@ -196,8 +212,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable t, NsUnits un, NsA
 
 // exponent of the power of two above sx: 0 unless |X|_F times the growth of all steps stays below 1
 __device__ __forceinline__ int ns_scale(double fro, double growth) {
+    if (!(fro * growth <= 0.5)) return 0;  // (NaN too)
     const double far = 1. / (fro * growth);
-    if (!(far >= 2.)) return 0;  // (NaN too)
     return far > 1e27 ? 90 : ilogb(far);
 }
 
@@ -266,16 +282,10 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsUnits un, Ns
     for (int k = threadIdx.x; k < 64 * 16; k += 256) {
         const int r = (k >> 3) & 63, c = (k & 7) * 4 + (k >> 9) * 32;
         f16x4 h, l, ht, lt;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            f16 a, b;
-            split(tile[r][c + j], a, b);
-            h[j] = a;
-            l[j] = b;
-            split(tile[c + j][r], a, b);
-            ht[j] = a;
-            lt[j] = b;
-        }
+        const float va[4] = {tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]};
+        const float vt[4] = {tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]};
+        split4(va, h, l);
+        split4(vt, ht, lt);
         const int64_t o = at_panel(i0 + r, j0 + c, e.mp), ot = at_panel(j0 + r, i0 + c, e.np);
         *reinterpret_cast<f16x4*>(P.x(0, 0) + o) = h;
         *reinterpret_cast<f16x4*>(P.x(0, 1) + o) = l;
@@ -450,15 +460,6 @@ template <int WM, int WN, int NB> struct Product {
     }
 };
 
-__device__ __forceinline__ void split4(const float* v, f16x4& h, f16x4& l) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        f16 a, b;
-        split(v[j], a, b);
-        h[j] = a;
-        l[j] = b;
-    }
-}
 enum NsPhase { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 
 // NS_GRAM: A = X X^T.  NS_POLY: B = b A + c A A.  Both symmetric: of each pair of 64-blocks across the diagonal one is
@@ -658,13 +659,261 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
             const int c = x / G::TM, r = x % G::TM;
             if (r0 + r >= e.cols || c0 + c >= e.rows) continue;
             T* o = out + (int64_t)(c0 + c) * e.cols + r0 + r;
-            *o = put(*o, tv[c * LS + r] * unit);
+            *o = put(o, tv[c * LS + r] * unit);
         }
     };
-    if (q.is_step) finish(float(), [&](float w, float v) { return fmaf(q.decay, w, -e.step * v); });
-    else if (q.dtype == PCX_F32) finish(float(), [](float, float v) { return v; });
-    else if (q.dtype == PCX_BF16) finish(bf16(), [](bf16, float v) { return (bf16)v; });
-    else finish(f16(), [](f16, float v) { return (f16)v; });
+    if (q.is_step) finish(float(), [&](const float* w, float v) { return fmaf(q.decay, *w, -e.step * v); });
+    else if (q.dtype == PCX_F32) finish(float(), [](const float*, float v) { return v; });
+    else if (q.dtype == PCX_BF16) finish(bf16(), [](const bf16*, float v) { return (bf16)v; });
+    else finish(f16(), [](const f16*, float v) { return (f16)v; });
+}
+
+// ---------------------------------------------------------------- small matrices: all steps in one block
+// X of up to 32 tiles of 32 x 32 stays in the registers of eight waves (in float32, T tiles a wave); its planes, X for the
+// gram product and then X^T, and the planes of A and then B pass through LDS.  A launch per product costs 5 us and more
+// however small it is, and there are 3 per step: 128 x 128 took 96 us that way, YYY us here.
+constexpr int NSB_WAVES = 8, NSB_LDS = 159 * 1024;
+
+// float16 number (row, k) of an LDS plane of `rows` rows: panels of 32 K values, runs of 8 swizzled over the slots
+__device__ __forceinline__ int at_lds(int row, int k, int rows) {
+    return ((k >> 5) * rows + row) * 32 + 8 * (((k >> 3) & 3) ^ ((row >> 2) & 3)) + (k & 7);
+}
+
+struct LdsRows {  // planes in LDS: hi, lo `d` numbers further, rows of a panel
+    const f16* hi;
+    int d, rows;
+};
+// two 32 x 32 tiles of sum_k P[p0 + r][k] Q[q + c][k], k < 16 n, for q = q0 and q1: the P operands are read once (the
+// kernel is bound by its LDS reads).  The small terms have sums of their own: an MFMA does not wait for its neighbour.
+__device__ __forceinline__ void block_product(const LdsRows& P, int p0, const LdsRows& Q, int q0, int q1, int n, int l32, int h,
+                                              f32x16 (&c)[2]) {
+    f32x16 s[2] = {};
+    c[0] = c[1] = f32x16{};
+    const int slot[2] = {8 * (h ^ ((l32 >> 2) & 3)), 8 * ((2 + h) ^ ((l32 >> 2) & 3))};
+    const f16* pp = P.hi + (p0 + l32) * 32;
+    const f16* qq = Q.hi + (q0 + l32) * 32;
+    const int dq = (q1 - q0) * 32;
+    for (int k = 0; k < n; k += 2, pp += P.rows * 32, qq += Q.rows * 32) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const f16x8 ph = *reinterpret_cast<const f16x8*>(pp + slot[y]), pl = *reinterpret_cast<const f16x8*>(pp + slot[y] + P.d);
+            f16x8 qh[2], ql[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                qh[i] = *reinterpret_cast<const f16x8*>(qq + slot[y] + i * dq);
+                ql[i] = *reinterpret_cast<const f16x8*>(qq + slot[y] + i * dq + Q.d);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[i] = mfma16(ph, ql[i], s[i]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) c[i] = mfma16(ph, qh[i], c[i]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s[i] = mfma16(pl, qh[i], s[i]);
+        }
+    }
+    c[0] += s[0];
+    c[1] += s[1];
+}
+// a tile's value (r, c) as plane element (row c, k r): four adjacent k at a time
+__device__ __forceinline__ void put_along(f16* pl, int d, int rows, int r0, int c, int h, const f32x16& v) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const float x[4] = {v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+        f16x4 hi, lo;
+        split4(x, hi, lo);
+        f16* at = pl + at_lds(c, r0 + acc_row(4 * g, h), rows);
+        *reinterpret_cast<f16x4*>(at) = hi;
+        *reinterpret_cast<f16x4*>(at + d) = lo;
+    }
+}
+
+// and as (row r, k c): adjacent lanes swap rows first, so that each writes two adjacent k
+__device__ __forceinline__ void put_across(f16* pl, int d, int rows, int r0, int c0, int l32, int h, const f32x16& v) {
+    const bool odd = l32 & 1;
+    // rows 16 apart are swizzled alike, and the lane's row of a pair (odd: the second) in the same slot
+    f16* at[2] = {pl + at_lds(r0 + 4 * h, c0 + (l32 & ~1), rows) + 32 * odd,
+                  pl + at_lds(r0 + 4 * h + 8, c0 + (l32 & ~1), rows) + 32 * odd - 8 * 32};
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+        // of rows k, k + 1 the even lane keeps the first and gets its neighbour's, the odd one the second
+        float first = v[k], second = v[k + 1];
+        asm("" : "+v"(first), "+v"(second));  // (or the choice becomes an index into v)
+        const float give = odd ? first : second, keep = odd ? second : first;
+        const float got = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(give), 0xb1, 0xf, 0xf, true));
+        f16x2 hi, lo;
+        split2(odd ? got : keep, odd ? keep : got, hi, lo);
+        f16* to = at[(k >> 2) & 1] + acc_row(k, 0) * 32;
+        *reinterpret_cast<f16x2*>(to) = hi;
+        *reinterpret_cast<f16x2*>(to + d) = lo;
+    }
+}
+
+template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kernel(NsTable t, NsUnits un, NsArgs q, NsCoef coef) {
+    extern __shared__ __attribute__((aligned(16))) char sm[];
+    __shared__ double red[NSB_WAVES + 2];
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
+    const NsMat& e = t.e[ei];
+    const int bat = blockIdx.x - un.first[ei];
+    const bool tall = e.rows > e.cols;
+    const int m = tall ? e.cols : e.rows, n = tall ? e.rows : e.cols;
+    const int mb = (m + 31) / 32, nb = (n + 31) / 32, mp = 32 * mb, np = 32 * nb;
+    f16* X = reinterpret_cast<f16*>(sm);
+    f16* A = X + 2 * mp * np;
+    const int dx = mp * np, da = mp * mp;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+    // u comes in through LDS, whole rows at a time: [rows][cols | 1]
+    float* raw = reinterpret_cast<float*>(sm);
+    const int pitch = e.cols | 1, total = e.rows * e.cols;
+    double s = 0.;
+    constexpr int THREADS = 64 * NSB_WAVES, FLY = 16;
+    const bool linear = e.xc == 1 && e.xr == e.cols;
+    const float by_cols = 1.f / (float)e.cols;  // (i + 1/2 is 2^-11 of a column away from the next row: i < 2^15)
+    const auto fetch = [&](auto kind) {
+        const auto* src = static_cast<const decltype(kind)*>(e.x) + bat * e.xb;
+        for (int i0 = threadIdx.x; i0 < total; i0 += FLY * THREADS) {
+            float u[FLY], mo[FLY];
+            int at[FLY];
+#pragma unroll
+            for (int y = 0; y < FLY; ++y) {
+                const int i = min(i0 + y * THREADS, total - 1), r = (int)((i + 0.5f) * by_cols), c = i - r * e.cols;
+                at[y] = r * pitch + c;
+                u[y] = (float)src[linear ? i : r * e.xr + c * e.xc];
+                if (q.is_step) mo[y] = e.mom[i];
+            }
+#pragma unroll
+            for (int y = 0; y < FLY; ++y) {
+                if (i0 + y * THREADS >= total) break;
+                if (q.is_step) {
+                    const float mv = fmaf(1.f - q.mu, u[y] * q.gs, q.mu * mo[y]);
+                    e.mom[i0 + y * THREADS] = mv;
+                    u[y] = nesterov_u(q, u[y], mv);
+                }
+                raw[at[y]] = u[y];
+                s += (double)u[y] * u[y];
+            }
+        }
+    };
+    if (q.dtype == PCX_F32) fetch(float());
+    else if (q.dtype == PCX_BF16) fetch(bf16());
+    else fetch(f16());
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[wave] = s;
+    __syncthreads();
+    if (wave == 0) {  // (64-bit roots and quotients: once)
+        s = 0.;
+#pragma unroll
+        for (int w = 0; w < NSB_WAVES; ++w) s += red[w];
+        const double norm = sqrt(s), inv = 1. / (norm + (double)q.eps);
+        if (threadIdx.x == 0) {
+            red[NSB_WAVES] = q.sx * inv;
+            red[NSB_WAVES + 1] = (double)ns_scale(norm * inv, q.growth);
+        }
+    }
+    __syncthreads();
+    const int lift = (int)red[NSB_WAVES + 1];
+    const float scale = (float)red[NSB_WAVES], more = ldexpf(1.f, lift), unit = ldexpf(1.f / q.sx, -lift);
+    // The wave's tiles of X, in pairs along n: of pair i rows 32 tr[i] of m, columns 32 tc[i] of n and the next 32 (a pair
+    // at an odd end has no second tile: it computes one that is not stored).  And its pair of tiles of A.
+    const int pr = tall ? 1 : pitch, pc = tall ? pitch : 1, row_pairs = (nb + 1) / 2, a_pairs = (mb + 1) / 2;
+    int tr[T / 2], tc[T / 2];
+    f32x16 x[T / 2][2];
+#pragma unroll
+    for (int i = 0; i < T / 2; ++i) {
+        const int pair = wave + NSB_WAVES * i;
+        tr[i] = pair / row_pairs;
+        tc[i] = 2 * (pair % row_pairs);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r0 = 32 * tr[i] + 4 * h, c = 32 * (tc[i] + j) + l32;
+            const float* at = raw + r0 * pr + c * pc;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                x[i][j][k] = r0 + acc_row(k, 0) < m && c < n ? at[acc_row(k, 0) * pr] * scale * more : 0.f;
+        }
+    }
+    const int ar = wave / a_pairs, ac = 2 * (wave % a_pairs);
+    __syncthreads();
+
+    for (int step = 0; step < coef.steps; ++step) {
+        const float a = coef.c[3 * step], b = coef.c[3 * step + 1], c = coef.c[3 * step + 2];
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));  // (addresses are formed anew: kept over the steps, they take the registers of X)
+        const int l32 = lane & 31, h = lane >> 5;
+        if (step) __syncthreads();  // (X^T and B of the last step are read)
+#pragma unroll
+        for (int i = 0; i < T; ++i) {  // X planes: rows of m, K along n
+            if (tr[i / 2] < mb && tc[i / 2] + i % 2 < nb)
+                put_across(X, dx, mp, 32 * tr[i / 2], 32 * (tc[i / 2] + i % 2), l32, h, x[i / 2][i % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        f32x16 g[2], p[2];
+        if (ar < mb) {
+            const LdsRows XR{X, dx, mp};
+            block_product(XR, 32 * ar, XR, 32 * ac, 32 * min(ac + 1, mb - 1), 2 * nb, l32, h, g);
+            const float k = q.sa * unit * unit;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                g[j] *= k;
+                if (ac + j < mb) put_along(A, da, mp, 32 * ar, 32 * (ac + j) + l32, h, g[j]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < T; ++i) {  // X^T planes: rows of n, K along m
+            if (tr[i / 2] < mb && tc[i / 2] + i % 2 < nb)
+                put_along(X, dx, np, 32 * tr[i / 2], 32 * (tc[i / 2] + i % 2) + l32, h, x[i / 2][i % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (ar < mb) {
+            const LdsRows AR{A, da, mp};
+            block_product(AR, 32 * ar, AR, 32 * ac, 32 * min(ac + 1, mb - 1), 2 * mb, l32, h, p);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) g[j] = g[j] * b + p[j] * (c / q.sa);
+        }
+        __syncthreads();
+        if (ar < mb) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (ac + j < mb) put_along(A, da, mp, 32 * ar, 32 * (ac + j) + l32, h, g[j]);
+        }
+        __syncthreads();
+        const LdsRows BR{A, da, mp}, XR{X, dx, np};
+        const float k = 1.f / q.sa;
+#pragma unroll
+        for (int i = 0; i < T / 2; ++i) {
+            if (tr[i] < mb) {
+                block_product(BR, 32 * tr[i], XR, 32 * tc[i], 32 * min(tc[i] + 1, nb - 1), 2 * mb, l32, h, p);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) x[i][j] = x[i][j] * a + p[j] * k;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        const int r0 = 32 * tr[i / 2] + 4 * h, c = 32 * (tc[i / 2] + i % 2) + l32;
+        float* at = raw + r0 * pr + c * pc;
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (r0 + acc_row(k, 0) < m && c < n) at[acc_row(k, 0) * pr] = x[i / 2][i % 2][k] * unit;
+    }
+    __syncthreads();
+    const auto finish = [&](auto kind, auto put) {
+        using V = decltype(kind);
+        V* out = static_cast<V*>(e.out) + (int64_t)bat * total;
+#pragma unroll 8
+        for (int i = threadIdx.x; i < total; i += 64 * NSB_WAVES) {
+            const int r = (int)((i + 0.5f) * by_cols), c = i - r * e.cols;
+            out[i] = put(out + i, raw[r * pitch + c]);
+        }
+    };
+    if (q.is_step) finish(float(), [&](const float* w, float v) { return fmaf(q.decay, *w, -e.step * v); });
+    else if (q.dtype == PCX_F32) finish(float(), [](const float*, float v) { return v; });
+    else if (q.dtype == PCX_BF16) finish(bf16(), [](const bf16*, float v) { return (bf16)v; });
+    else finish(f16(), [](const f16*, float v) { return (f16)v; });
 }
 
 // ---------------------------------------------------------------- host
@@ -709,7 +958,7 @@ int ns_config(const NsTable& t, int phase) {
     if (force >= 0) return force;
     return 0;
 }
-constexpr int NS_TM[5] = {64, 128, 256, 128, 64}, NS_TN[5] = {64, 128, 128, 128, 64}, NS_PER_CU[5] = {3, 1, 1, 2, 4};
+constexpr int NS_TM[2] = {64, 128}, NS_TN[2] = {64, 128}, NS_PER_CU[2] = {3, 2};
 
 struct NsPlan {
     NsUnits un;
@@ -829,10 +1078,7 @@ template <int PHASE, int WM, int WN, int NB> int ns_product_as(const NsTable& t,
 template <int PHASE> int ns_product(const NsTable& t, const NsArgs& q, hipStream_t s) {
     const NsPlan p = ns_plan(t, PHASE);
     if (p.cfg == 0) return ns_product_as<PHASE, 1, 1, 3>(t, p, q, s);
-    if (p.cfg == 1) return ns_product_as<PHASE, 2, 2, 3>(t, p, q, s);
-    if (p.cfg == 3) return ns_product_as<PHASE, 2, 2, 2>(t, p, q, s);
-    if (p.cfg == 4) return ns_product_as<PHASE, 1, 1, 2>(t, p, q, s);
-    return ns_product_as<PHASE, 4, 2, 3>(t, p, q, s);
+    return ns_product_as<PHASE, 2, 2, 2>(t, p, q, s);
 }
 
 int ns_scales(NsArgs& q, const float* coef, int steps) {
@@ -845,8 +1091,42 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
     return PCX_OK;
 }
 
+// pairs of tiles along the long side, and the bytes of a matrix's planes in LDS if one block holds it (0 if not): at most
+// two pairs a wave, and one of A's
+int ns_block_pairs(const NsMat& e) {
+    return ((std::min(e.rows, e.cols) + 31) / 32) * ((std::max(e.rows, e.cols) + 63) / 64);
+}
+int ns_block_bytes(const NsMat& e) {
+    if (std::min(e.rows, e.cols) > 128 || std::max(e.rows, e.cols) > 1024 || ns_block_pairs(e) > 2 * NSB_WAVES) return 0;
+    const int64_t mp = round_up(std::min(e.rows, e.cols), 32), np = round_up(std::max(e.rows, e.cols), 32);
+    const int64_t bytes = 4 * (mp * np + (int64_t)mp * mp);
+    return bytes <= NSB_LDS ? (int)bytes : 0;
+}
+
+template <int T> int ns_block_as(const NsTable& t, const NsUnits& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
+    if (sm > 64 * 1024)
+        (void)hipFuncSetAttribute((const void*)ns_block_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+    ns_block_kernel<T><<<n, 64 * NSB_WAVES, sm, s>>>(t, un, q, c);
+    PCX_LAUNCH_CHECK("ns_block_kernel");
+    return PCX_OK;
+}
+
 int ns_run(const NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
     NsUnits un{};
+    int most = 0, pairs = 0;
+    for (int i = 0; i < t.count && most >= 0; ++i) {
+        const int bytes = ns_block_bytes(t.e[i]);
+        most = bytes ? std::max(most, bytes) : -1;
+        pairs = std::max(pairs, ns_block_pairs(t.e[i]));
+    }
+    if (most > 0) {  // every matrix of the launch fits a block
+        NsCoef c{};
+        c.steps = steps;
+        memcpy(c.c, coef, 3 * steps * sizeof(float));
+        const unsigned n = ns_blocks(t, un, [](const NsMat&) { return (int64_t)1; });
+        if (pairs <= NSB_WAVES) return ns_block_as<2>(t, un, q, c, n, most, s);
+        return ns_block_as<4>(t, un, q, c, n, most, s);
+    }
     unsigned n = ns_blocks(t, un, [](const NsMat& e) { return (int64_t)e.parts; });
     ns_norm_kernel<<<n, 256, 0, s>>>(t, un, q);
     PCX_LAUNCH_CHECK("ns_norm_kernel");
@@ -897,7 +1177,7 @@ bool ns_shape_ok(int64_t batch, int64_t rows, int64_t cols) {
 }
 
 int ns_check(const char* what, int steps, const float* coef, float eps) {
-    PCX_CHECK_ARG(steps >= 1 && steps <= 64, "%s: 1 to 64 steps (got %d)", what, steps);
+    PCX_CHECK_ARG(steps >= 1 && steps <= NS_STEPS, "%s: 1 to %d steps (got %d)", what, NS_STEPS, steps);
     PCX_CHECK_ARG(coef, "%s: no coefficients", what);
     for (int i = 0; i < 3 * steps; ++i) PCX_CHECK_ARG(isfinite(coef[i]), "%s: coefficient %d is not finite", what, i);
     PCX_CHECK_ARG(eps > 0.f && isfinite(eps), "%s: eps must be positive (got %g)", what, (double)eps);
