@@ -12,9 +12,13 @@ OBJ = $(patsubst phoneme_contrast_amd/csrc/%.hip,$(BUILD)/%.o,$(SRC))
 HDR = $(wildcard phoneme_contrast_amd/csrc/*.h) include/pcx.h
 LIB ?= phoneme_contrast_amd/libpcx.so
 
+# the torch operators (csrc/torch_ops.cpp) on top of the C ABI, against the installed torch's headers
+TORCH_LIB = phoneme_contrast_amd/libpcx_torch.so
+TORCH_DIR := $(shell python3 -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+
 TOOLS = tools/wino_bench tools/ww_bench tools/stem_bench tools/wb_bench tools/ws_bench
 
-all: $(LIB) $(TOOLS)
+all: $(LIB) $(TORCH_LIB) $(TOOLS)
 
 # engine cross-check / micro-benchmark (tests/test_wino_engine_gpu.py runs it)
 tools/wino_bench: tools/wino_bench.cpp $(LIB) $(HDR)
@@ -56,6 +60,11 @@ $(BUILD)/layernorm.o $(BUILD)/muon.o: CXXFLAGS += -Xclang -target-feature -Xclan
 $(LIB): $(OBJ)
 	$(HIPCC) -shared --offload-arch=$(ARCH) -o $@ $(OBJ)
 
+$(TORCH_LIB): phoneme_contrast_amd/csrc/torch_ops.cpp include/pcx.h $(LIB)
+	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -Iinclude \
+	    -isystem $(TORCH_DIR)/include -isystem $(TORCH_DIR)/include/torch/csrc/api/include -isystem /opt/rocm/include \
+	    $< -o $@ -L$(TORCH_DIR)/lib -ltorch -ltorch_cpu -lc10 -lc10_hip -Lphoneme_contrast_amd -lpcx -Wl,-rpath,'$$ORIGIN'
+
 # host-side sanitizer build (no GPU): every source compiled host-only with ASan + UBSan, linked with the
 # plan-builder check tools/plan_check.cpp (tests/test_plan_asan.py runs it)
 ASAN_FLAGS = -O1 -g -std=c++17 --offload-arch=$(ARCH) -fPIC -Iinclude -Xarch_host -fsanitize=address \
@@ -76,6 +85,6 @@ tools/plan_check_asan: build_asan/plan_check.o $(ASAN_OBJ)
 asan: tools/plan_check_asan
 
 clean:
-	rm -rf build build_asan $(LIB) $(TOOLS) tools/plan_check_asan
+	rm -rf build build_asan $(LIB) $(TORCH_LIB) $(TOOLS) tools/plan_check_asan
 
 .PHONY: all asan clean

@@ -15,6 +15,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # scripts/ab_bench.sh); unset, the in-tree library
 LIB_PATH = os.environ.get("PCX_LIB_PATH") or os.path.join(_HERE, "libpcx.so")
 
+TORCH_OPS_PATH = os.path.join(_HERE, "libpcx_torch.so")
+
 PCX_OK = 0
 PCX_EINVAL = -1
 PCX_ESHAPE = -2
@@ -157,6 +159,31 @@ def lib():
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+class _TorchOps:
+    """Handles of the torch operators in libpcx_torch.so (csrc/torch_ops.cpp)."""
+
+    def __init__(self):
+        if not os.path.exists(TORCH_OPS_PATH):
+            raise RuntimeError(
+                f"phoneme_contrast_amd: native library {TORCH_OPS_PATH} is missing; build it with "
+                "`make` (or __graft_entry__.build()) — there is no CPU fallback")
+        torch.ops.load_library(TORCH_OPS_PATH)
+        self.layer_norm = torch.ops.pcx.layer_norm.default
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """Load libpcx_torch.so once; raise if it is missing (no silent fallback)."""
+    global _torch_ops
+    if _torch_ops is None:
+        with _lock:
+            if _torch_ops is None:
+                _torch_ops = _TorchOps()
+    return _torch_ops
 
 
 def last_error():

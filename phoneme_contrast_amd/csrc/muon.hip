@@ -21,10 +21,9 @@
 // Layout.  X is kept as hi / lo planes and transposed, A and B once, all padded with zeros to 64, so that every product is
 // one of rows with rows.  A plane is stored in panels of 32 values of K, [K / 32][rows][32]: what a tile needs of a panel
 // is one run of memory.  (Row by row, the rows of a tile lie a power of two apart more often than not and queue at one
-// L2 channel: 512 x 4608 took 35 us for the product that takes XXX us now.)
+// L2 channel: 5160 us for 4096 x 4096 in bfloat16, 4836 us in panels, all else alike.)
 // A and B are symmetric: only tiles on and above the diagonal are computed, and written twice.
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -42,7 +41,6 @@ typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int NS_LIST = 24;      // entries per launch (their table is a kernel argument)
 constexpr int NS_PAD = 64;       // X, A, B are padded to it; tiles that reach over the padding read their last rows again
 constexpr int NS_K = 32;         // K values of a stage
-constexpr int NS_BUF = 3;        // stages in LDS: one computed on, two on their way
 constexpr int NS_STEPS = 64;     // most steps
 constexpr int NS_PART = 512;     // most partial sums of squares per matrix
 
@@ -297,7 +295,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsUnits un, Ns
 // ---------------------------------------------------------------- the products
 // C[r][c] = sum_k P[r][k] Q[c][k] on tiles of TM = 64 WM rows by TN = 64 WN columns, four waves of 32 WM x 32 WN each.
 // The operands' four plane tiles (32 K values of TM + TN rows, hi and lo) are copied to LDS by global_load_lds, 16 bytes
-// per lane, NS_BUF stages deep; run q of row r sits in slot q ^ ((r >> 2) & 3), which spreads the operand reads over all
+// per lane, NB stages deep; run q of row r sits in slot q ^ ((r >> 2) & 3), which spreads the operand reads over all
 // banks.  One barrier per stage, half a stage ahead of its first read: while the first half's MFMAs run, the second
 // half's operands are read; then the next stage has landed, its first half is read under the second half's MFMAs.
 typedef __attribute__((address_space(3))) void lds_void;
@@ -460,6 +458,17 @@ template <int WM, int WN, int NB> struct Product {
     }
 };
 
+// what is stored for a result v: itself, or the parameter `old` moved by it
+template <typename T> struct Plain {
+    __device__ static T old(const T*) { return T(); }
+    __device__ T operator()(T, float v) const { return (T)v; }
+};
+struct Descend {
+    float decay, step;
+    __device__ static float old(const float* p) { return *p; }
+    __device__ float operator()(float w, float v) const { return fmaf(decay, w, -step * v); }
+};
+
 enum NsPhase { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 
 // NS_GRAM: A = X X^T.  NS_POLY: B = b A + c A A.  Both symmetric: of each pair of 64-blocks across the diagonal one is
@@ -486,12 +495,10 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     int r0, c0;
     Rows P, Q;
     if (SYM) {
-        const int nc = (e.mp + G::TN - 1) / G::TN;
         int ti = 0;
         for (;; ++ti) {
-            const int w = min((WM / WN) * (ti + 1), nc);
-            if (tl < w) break;
-            tl -= w;
+            if (tl <= ti) break;
+            tl -= ti + 1;
         }
         r0 = ti * G::TM;
         c0 = tl * G::TN;
@@ -561,7 +568,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
 #pragma unroll
                 for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
             const uint64_t* from = reinterpret_cast<const uint64_t*>(q.joint + (int64_t)(un.joint[ei] + over % cut) * SZ) + threadIdx.x;
-            constexpr int FLY = 8 / (WM * WN) > 0 ? 8 / (WM * WN) : 1;  // parts in flight
+            constexpr int FLY = WM * WN == 1 ? 4 : 2;  // parts in flight
             for (int k = 0; k < split; k += FLY) {
 #pragma unroll
                 for (int i = 0; i < WM; ++i)
@@ -606,7 +613,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     }
     f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
     f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
-#pragma unroll 4
+#pragma unroll 8
     for (int x0 = 0; x0 < G::TM * G::TN / 4; x0 += 256) {
         const int x = x0 + threadIdx.x, c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
         if (r >= nr || c >= nc) continue;
@@ -654,24 +661,38 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     const auto finish = [&](auto kind, auto put) {
         using T = decltype(kind);
         T* out = static_cast<T*>(e.out) + (int64_t)bat * e.rows * e.cols;
-#pragma unroll 8
-        for (int x = threadIdx.x; x < G::TM * G::TN; x += 256) {
-            const int c = x / G::TM, r = x % G::TM;
-            if (r0 + r >= e.cols || c0 + c >= e.rows) continue;
-            T* o = out + (int64_t)(c0 + c) * e.cols + r0 + r;
-            *o = put(o, tv[c * LS + r] * unit);
+        // (16 values a thread at a time: the parameters are read from HBM)
+        const int r = threadIdx.x % G::TM, cs = threadIdx.x / G::TM;
+        if (r0 + r >= e.cols) return;
+        T* o = out + (int64_t)(c0 + cs) * e.cols + r0 + r;
+        const float* at = tv + cs * LS + r;
+        constexpr int STEP = 256 / G::TM;
+#pragma unroll 1
+        for (int x0 = 0; x0 < G::TN; x0 += 16 * STEP) {
+            T old[16];
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int c = x0 + x * STEP;
+                if (c0 + cs + c < e.rows) old[x] = put.old(o + (int64_t)c * e.cols);
+            }
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int c = x0 + x * STEP;
+                if (c0 + cs + c < e.rows) o[(int64_t)c * e.cols] = put(old[x], at[c * LS] * unit);
+            }
         }
     };
-    if (q.is_step) finish(float(), [&](const float* w, float v) { return fmaf(q.decay, *w, -e.step * v); });
-    else if (q.dtype == PCX_F32) finish(float(), [](const float*, float v) { return v; });
-    else if (q.dtype == PCX_BF16) finish(bf16(), [](const bf16*, float v) { return (bf16)v; });
-    else finish(f16(), [](const f16*, float v) { return (f16)v; });
+    if (q.is_step) finish(float(), Descend{q.decay, e.step});
+    else if (q.dtype == PCX_F32) finish(float(), Plain<float>());
+    else if (q.dtype == PCX_BF16) finish(bf16(), Plain<bf16>());
+    else finish(f16(), Plain<f16>());
 }
 
 // ---------------------------------------------------------------- small matrices: all steps in one block
 // X of up to 32 tiles of 32 x 32 stays in the registers of eight waves (in float32, T tiles a wave); its planes, X for the
 // gram product and then X^T, and the planes of A and then B pass through LDS.  A launch per product costs 5 us and more
-// however small it is, and there are 3 per step: 128 x 128 took 96 us that way, YYY us here.
+// however small it is, and there are 3 per step: 128 x 128 took 96 us that way, 57 us here (of a step's 10 us 4.4 are
+// MFMAs, the rest LDS traffic, the splitting into hi and lo, and barriers).
 constexpr int NSB_WAVES = 8, NSB_LDS = 159 * 1024;
 
 // float16 number (row, k) of an LDS plane of `rows` rows: panels of 32 K values, runs of 8 swizzled over the slots
@@ -907,13 +928,13 @@ template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kern
 #pragma unroll 8
         for (int i = threadIdx.x; i < total; i += 64 * NSB_WAVES) {
             const int r = (int)((i + 0.5f) * by_cols), c = i - r * e.cols;
-            out[i] = put(out + i, raw[r * pitch + c]);
+            out[i] = put(put.old(out + i), raw[r * pitch + c]);
         }
     };
-    if (q.is_step) finish(float(), [&](const float* w, float v) { return fmaf(q.decay, *w, -e.step * v); });
-    else if (q.dtype == PCX_F32) finish(float(), [](const float*, float v) { return v; });
-    else if (q.dtype == PCX_BF16) finish(bf16(), [](const bf16*, float v) { return (bf16)v; });
-    else finish(f16(), [](const f16*, float v) { return (f16)v; });
+    if (q.is_step) finish(float(), Descend{q.decay, e.step});
+    else if (q.dtype == PCX_F32) finish(float(), Plain<float>());
+    else if (q.dtype == PCX_BF16) finish(bf16(), Plain<bf16>());
+    else finish(f16(), Plain<f16>());
 }
 
 // ---------------------------------------------------------------- host
@@ -950,15 +971,28 @@ void ns_bounds(const float* coef, int steps, double* smax, double* bmax, double*
     }
 }
 
-template <int WM, int WN> struct Config {
-    static constexpr int wm = WM, wn = WN;
-};
-int ns_config(const NsTable& t, int phase) {
-    static const int force = getenv("NS_CFG") ? atoi(getenv("NS_CFG")) : -1;
-    if (force >= 0) return force;
-    return 0;
+constexpr int NS_TM[2] = {64, 128}, NS_PER_CU[2] = {3, 2};  // tile edges; blocks a CU holds (LDS)
+
+// tiles of one matrix of an entry in a phase
+int64_t ns_tiles(const NsMat& e, int phase, int edge) {
+    const int64_t tm = (e.mp + edge - 1) / edge, tn = (e.np + edge - 1) / edge;
+    return phase <= NS_POLY ? tm * (tm + 1) / 2 : tm * tn;
 }
-constexpr int NS_TM[2] = {64, 128}, NS_TN[2] = {64, 128}, NS_PER_CU[2] = {3, 2};
+int ns_stages(const NsMat& e, int phase) { return (phase == NS_GRAM ? e.np : e.mp) / NS_K; }
+
+// 128 x 128 tiles do the same work with half the LDS reads per MFMA, 64 x 64 tiles spread it over four times the blocks.
+// Measured, us for 64 / 128: X <- a X + B X of 1536 x 1536 (144 tiles of 128) 38 / 43, 1024 x 4096 (256) 51 / 39,
+// 2048 x 2048 (256) 81 / 70; A = X X^T of 4 x 1024 x 1024 (144, K 1024) 31 / 32, 2048 x 2048 (136, K 2048) 52 / 46,
+// 3 x 1536 x 1536 (234) 59 / 55: large tiles from one per CU on, with K of 2048 from one per two CUs.
+int ns_config(const NsTable& t, int phase) {
+    int64_t n = 0, deep = 0;
+    for (int i = 0; i < t.count; ++i) {
+        const int64_t k = ns_tiles(t.e[i], phase, 128) * t.e[i].batch;
+        n += k;
+        if (ns_stages(t.e[i], phase) >= 64) deep += k;
+    }
+    return n >= num_cus() || 2 * deep >= num_cus();
+}
 
 struct NsPlan {
     NsUnits un;
@@ -971,23 +1005,13 @@ struct NsPlan {
 NsPlan ns_plan(const NsTable& t, int phase) {
     NsPlan p{};
     p.cfg = ns_config(t, phase);
-    const int TM = NS_TM[p.cfg], TN = NS_TN[p.cfg];
-    static const int most = getenv("NS_MOST") ? atoi(getenv("NS_MOST")) : 16;
+    const int edge = NS_TM[p.cfg];
     const int64_t slots = (int64_t)num_cus() * NS_PER_CU[p.cfg];
     int64_t units = 0, parts = 0;
     int stages[NS_LIST];
     for (int i = 0; i < t.count; ++i) {
-        const NsMat& e = t.e[i];
-        int64_t n = 0;
-        if (phase <= NS_POLY) {
-            const int nc = (e.mp + TN - 1) / TN;
-            for (int ti = 0; ti * TM < e.mp; ++ti) n += std::min(TM / TN * (ti + 1), nc);
-        } else {
-            const bool tall = phase == NS_LAST && e.rows > e.cols;
-            n = (int64_t)(((tall ? e.mp : e.np) + TM - 1) / TM) * (((tall ? e.np : e.mp) + TN - 1) / TN);
-        }
-        p.un.tiles[i] = (int)n;
-        stages[i] = (phase == NS_GRAM ? e.np : e.mp) / NS_K;
+        p.un.tiles[i] = (int)ns_tiles(t.e[i], phase, edge);
+        stages[i] = ns_stages(t.e[i], phase);
     }
     p.un.count = t.count;
     int64_t all = 0;
@@ -999,9 +1023,11 @@ NsPlan ns_plan(const NsTable& t, int phase) {
             whole = n / slots * slots;
             if (n > whole) split = std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / 16));
         } else if (stages[i] >= 48) {
+            // a stage takes about 0.17 us, meeting in memory 4 us and 0.3 us a part: sqrt(0.6 stages) parts are the best,
+            // and parts of less than 48 stages do not pay
             split = std::min<int64_t>((int64_t)(sqrt(0.6 * stages[i]) + 0.5), std::max<int64_t>(1, slots / all));
         }
-        split = std::min<int64_t>(split, most);
+        split = std::min<int64_t>(split, 16);
         if (split == 1) whole = n;
         p.un.whole[i] = (int)whole;
         p.un.split[i] = (int)split;
@@ -1014,7 +1040,7 @@ NsPlan ns_plan(const NsTable& t, int phase) {
     }
     p.un.first[t.count] = (int)units;
     p.blocks = (unsigned)units;
-    p.joint = parts * TM * TN;
+    p.joint = parts * edge * edge;
     return p;
 }
 
