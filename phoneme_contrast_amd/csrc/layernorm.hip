@@ -10,8 +10,8 @@
 // rows far from zero), and the backward sums dw / db over the rows of its block in registers, so x and dy are read
 // once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
 //
-// A row belongs to 1 ... 64 lanes of a wave, to a block of 256 threads or to one of 1024 (the fewest that leave a
-// thread at most 32 values): sub-wave rows need no barrier, and wider ones one barrier per reduction.  Rows of up to
+// A row belongs to 1 ... 64 lanes of a wave or to a block of just the waves it needs: sub-wave rows need no barrier, and
+// wider ones one barrier per reduction.  Rows of up to
 // 32 values are computed in 64 bits from x itself: at D = 2 the three terms of dx cancel to eps / (var + eps) of
 // their size, which 32-bit statistics do not resolve, and such rows are short of bytes, not of arithmetic.
 #include "kernels.h"
@@ -51,27 +51,32 @@ template <typename T> struct Pack<T, 1> {
     typedef T type;
 };
 
-template <int V, typename T> __device__ __forceinline__ void load_v(const T* p, float* v) {
+template <typename T, int V> using pack = typename Pack<T, V>::type;
+
+template <int V, typename T> __device__ __forceinline__ pack<T, V> load_raw(const T* p) {
+    return *reinterpret_cast<const pack<T, V>*>(p);
+}
+template <typename T, int V> __device__ __forceinline__ void widen(const pack<T, V>& t, float* v) {
     if constexpr (V == 1) {
-        v[0] = (float)p[0];
+        v[0] = (float)t;
     } else {
-        constexpr int N = V * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;  // (float weights of 16-bit rows: two loads)
 #pragma unroll
-        for (int k = 0; k < V / N; ++k) {
-            const typename Pack<T, N>::type t = *reinterpret_cast<const typename Pack<T, N>::type*>(p + k * N);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[k * N + j] = (float)t[j];
-        }
+        for (int j = 0; j < V; ++j) v[j] = (float)t[j];
     }
+}
+template <int V, typename T> __device__ __forceinline__ void load_v(const T* p, float* v) {
+    constexpr int N = V * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;  // (float weights of 16-bit rows: two loads)
+#pragma unroll
+    for (int k = 0; k < V / N; ++k) widen<T, N>(load_raw<N>(p + k * N), v + k * N);
 }
 template <int V, typename T> __device__ __forceinline__ void store_v(T* p, const float* v) {
     if constexpr (V == 1) {
         p[0] = (T)v[0];
     } else {
-        typename Pack<T, V>::type t;
+        pack<T, V> t;
 #pragma unroll
         for (int j = 0; j < V; ++j) t[j] = (T)v[j];
-        *reinterpret_cast<typename Pack<T, V>::type*>(p) = t;
+        *reinterpret_cast<pack<T, V>*>(p) = t;
     }
 }
 // V weights; without any the pointer is some readable row of the same length, and the values are not used
@@ -81,10 +86,10 @@ template <int V, typename W> __device__ __forceinline__ void load_w(const void* 
     for (int j = 0; j < V; ++j) v[j] = has ? v[j] : none;
 }
 
-// sums over the lanes of a row; BLOCK = 0: tpr lanes of a wave, else the whole block through `red` (one barrier; the
-// caller alternates between two `red` buffers, so a buffer is rewritten only behind the other's barrier)
-template <int BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float (*red)[16]) {
-    if constexpr (BLOCK == 0) {
+// sums over the lanes of a row: tpr lanes of a wave, or (BLOCK) all waves of the block through `red` with one barrier; the
+// caller alternates between two `red` buffers, so a buffer is rewritten only behind the other's barrier
+template <bool BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float (*red)[16]) {
+    if constexpr (!BLOCK) {
         for (int o = tpr >> 1; o > 0; o >>= 1) {
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
@@ -100,36 +105,64 @@ template <int BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[N
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float s = 0.f;
-#pragma unroll
-            for (int w = 0; w < BLOCK / 64; ++w) s += red[i][w];
+            for (int w = 0; w < tpr / 64; ++w) s += red[i][w];
             v[i] = s;
         }
     }
 }
 
-template <typename T, int V, int E, int BLOCK>
-__global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_fwd_kernel(LnArgs a) {
+// A block goes from row to row: the next row is on its way while this one is summed, and the weights stay in registers
+// (read again per row they are as many bytes from L2 as the row itself).
+template <typename T, int V, int E, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
+    constexpr bool KEEP = E <= (V > 1 ? 16 : 8), AHEAD = KEEP;  // (what the registers of 1024 threads hold)
     __shared__ float red[2][1][16];
-    const int tpr = BLOCK ? BLOCK : a.tpr;
-    const int lane = threadIdx.x & (tpr - 1);
-    const int rpb = (BLOCK ? BLOCK : 256) / tpr;
+    const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
+    const int lane = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (unsigned)(tpr - 1));
+    const int64_t rpb = BLOCK ? 1 : 256 / tpr, stride = gridDim.x * rpb;
     const float invd = 1.f / (float)a.D;
-    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
-        const int64_t r = r0 + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
-        const bool on = r < a.rows;  // (a whole sub-wave row; the others of its wave go on)
-        const T* x = static_cast<const T*>(a.x) + (on ? r : 0) * a.xs;
-        float v[NC][V];
-        float s[1] = {0.f};
+    float w[KEEP ? NC : 1][V], b[KEEP ? NC : 1][V];
+    const auto weights = [&](int c, float* wv, float* bv) {
+        const int d = (lane + c * tpr) * V;
+        if (d < a.D) {
+            if (a.wf32) {
+                load_w<V, float>(a.w, a.hw, d, wv, 1.f);
+                load_w<V, float>(a.b, a.hb, d, bv, 0.f);
+            } else {
+                load_w<V, T>(a.w, a.hw, d, wv, 1.f);
+                load_w<V, T>(a.b, a.hb, d, bv, 0.f);
+            }
+        }
+    };
+    const auto fetch = [&](int64_t r, pack<T, V> (&raw)[NC]) {
+        const T* x = static_cast<const T*>(a.x) + (r < a.rows ? r : 0) * a.xs;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = (lane + c * tpr) * V;
-            if (on && d < a.D) load_v<V>(x + d, v[c]);
+            if (d < a.D) raw[c] = load_raw<V>(x + d);
+        }
+    };
+    int64_t r = (int64_t)blockIdx.x * rpb + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
+    pack<T, V> next[NC];
+    if constexpr (AHEAD) fetch(r, next);
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) weights(c, w[c], b[c]);
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += stride, r += stride) {
+        float v[NC][V];
+        float s[1] = {0.f};
+        if constexpr (!AHEAD) fetch(r, next);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if ((lane + c * tpr) * V < a.D) widen<T, V>(next[c], v[c]);
             else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) v[c][j] = 0.f;
             }
         }
+        if (AHEAD && r0 + stride < a.rows) fetch(r + stride, next);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -149,66 +182,79 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_fwd_kernel(LnArgs a) {
         }
         row_sum<BLOCK, 1>(s, tpr, red[1]);
         const float rstd = 1.f / sqrtf(fmaf(s[0], invd, a.eps));
-        if (!on) continue;
+        if (r >= a.rows) continue;  // (a whole sub-wave row; the others of its wave go on)
         T* y = static_cast<T*>(a.y) + r * a.D;
-        auto finish = [&](auto kind) {
-            using W = decltype(kind);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = (lane + c * tpr) * V;
-                if (d < a.D) {
-                    float w[V], b[V];
-                    load_w<V, W>(a.w, a.hw, d, w, 1.f);
-                    load_w<V, W>(a.b, a.hb, d, b, 0.f);
+        for (int c = 0; c < NC; ++c) {
+            const int d = (lane + c * tpr) * V, k = KEEP ? c : 0;
+            if (d < a.D) {
+                if constexpr (!KEEP) weights(c, w[0], b[0]);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[j], b[j]);
-                    store_v<V>(y + d, v[c]);
-                }
-                if constexpr (V == 1)  // (single values: few weights in flight, or the registers spill)
-                    if (c % 4 == 3) asm volatile("" ::: "memory");
+                for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[k][j], b[k][j]);
+                store_v<V>(y + d, v[c]);
             }
-        };
-        if (a.wf32) finish(float());
-        else finish(T());
+            if constexpr (!KEEP)  // (few weights in flight, or the registers spill)
+                if (c % 4 == 3) asm volatile("" ::: "memory");
+        }
         if (a.stat && lane == 0) a.stat[r] = make_float2(mean, rstd);
     }
 }
 
-template <typename T, int V, int E, int BLOCK>
-__global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(LnArgs a) {
+template <typename T, int V, int E, bool BLOCK>
+__global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
-    constexpr bool COLS = E <= 16;  // (32 values a thread leave no registers for two sums each: ln_long_cols_kernel)
+    constexpr bool AHEAD = E <= 8 || sizeof(T) == 2;  // (16 float32 values a thread leave no registers for the next row)
     __shared__ float red[2][2][16];
     extern __shared__ __attribute__((aligned(16))) float cols[];  // sub-wave rows: [4 waves][D] of dw, then of db
-    const int tpr = BLOCK ? BLOCK : a.tpr;
-    const int lane = threadIdx.x & (tpr - 1);
-    const int rpb = (BLOCK ? BLOCK : 256) / tpr;
+    const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
+    const int lane = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (unsigned)(tpr - 1));
+    const int64_t rpb = BLOCK ? 1 : 256 / tpr, stride = gridDim.x * rpb;
     const float invd = 1.f / (float)a.D;
-    float sw[NC][V], sb[NC][V], w[NC][V];
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int d = (lane + c * tpr) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) sw[c][j] = sb[c][j] = w[c][j] = 0.f;
-        if (d < a.D) {
-            if (a.wf32) load_w<V, float>(a.w, a.hw, d, w[c], 1.f);
-            else load_w<V, T>(a.w, a.hw, d, w[c], 1.f);
-        }
-    }
-    int par = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += (int64_t)gridDim.x * rpb) {
-        const int64_t r = r0 + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
-        const bool on = r < a.rows;
-        const T* x = static_cast<const T*>(a.x) + (on ? r : 0) * a.xs;
-        const T* dy = static_cast<const T*>(a.dy) + (on ? r : 0) * a.dys;
-        const float2 st = on ? a.stat[r] : make_float2(0.f, 0.f);
-        float xh[NC][V], g[NC][V];
+    int64_t r = (int64_t)blockIdx.x * rpb + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
+    pack<T, V> nx[NC], ng[NC];
+    float2 nst;
+    const auto fetch = [&](int64_t row) {
+        const int64_t q = row < a.rows ? row : 0;
+        const T* x = static_cast<const T*>(a.x) + q * a.xs;
+        const T* dy = static_cast<const T*>(a.dy) + q * a.dys;
+        nst = a.stat[q];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = (lane + c * tpr) * V;
-            if (on && d < a.D) {
-                load_v<V>(x + d, xh[c]);
-                load_v<V>(dy + d, g[c]);
+            if (d < a.D) {
+                nx[c] = load_raw<V>(x + d);
+                ng[c] = load_raw<V>(dy + d);
+            }
+        }
+    };
+    if constexpr (AHEAD) fetch(r);
+    float sw[NC][V], sb[NC][V], w[AHEAD ? NC : 1][V];
+    const auto weight = [&](int c, float* wv) {
+        const int d = (lane + c * tpr) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) wv[j] = 0.f;
+        if (d < a.D) {
+            if (a.wf32) load_w<V, float>(a.w, a.hw, d, wv, 1.f);
+            else load_w<V, T>(a.w, a.hw, d, wv, 1.f);
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sw[c][j] = sb[c][j] = 0.f;
+        if constexpr (AHEAD) weight(c, w[c]);
+    }
+    int par = 0;
+    for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += stride, r += stride) {
+        const bool on = r < a.rows;
+        if constexpr (!AHEAD) fetch(r);
+        const float2 st = nst;
+        float xh[NC][V], g[NC][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (on && (lane + c * tpr) * V < a.D) {
+                widen<T, V>(nx[c], xh[c]);
+                widen<T, V>(ng[c], g[c]);
             } else {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
@@ -217,20 +263,22 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(LnArgs a) {
                 }
             }
         }
+        if (AHEAD && r0 + stride < a.rows) fetch(r + stride);
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) {
+            const int k = AHEAD ? c : 0;
+            if constexpr (!AHEAD) weight(c, w[0]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 xh[c][j] = (xh[c][j] - st.x) * st.y;
-                if constexpr (COLS) {
-                    sb[c][j] += g[c][j];
-                    sw[c][j] = fmaf(g[c][j], xh[c][j], sw[c][j]);
-                }
-                g[c][j] *= w[c][j];
+                sb[c][j] += g[c][j];
+                sw[c][j] = fmaf(g[c][j], xh[c][j], sw[c][j]);
+                g[c][j] *= w[k][j];
                 s[0] += g[c][j];
                 s[1] = fmaf(g[c][j], xh[c][j], s[1]);
             }
+        }
         if (!a.dx) continue;  // (the same for the whole grid)
         row_sum<BLOCK, 2>(s, tpr, red[par]);
         par ^= 1;
@@ -247,9 +295,9 @@ __global__ __launch_bounds__(BLOCK ? BLOCK : 256) void ln_bwd_kernel(LnArgs a) {
             }
         }
     }
-    if (!COLS || !a.part) return;
+    if (!a.part) return;
     float* pw = a.part + (int64_t)blockIdx.x * 2 * a.D;
-    if constexpr (BLOCK != 0) {
+    if constexpr (BLOCK) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int d = (lane + c * tpr) * V;
@@ -342,7 +390,78 @@ template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow
     }
 }
 
-// partial dw, db of rows of more than 16384 values: a thread owns a column, a block a slab of rows
+// Rows that no block holds in registers (behind 8192 values without 16-byte loads, behind 16384 in the backward): read
+// again for each sum, from L2, where a row stays meanwhile.
+template <typename T> __global__ __launch_bounds__(1024) void ln_long_fwd_kernel(LnArgs a) {
+    __shared__ float red[2][1][16];
+    const float invd = 1.f / (float)a.D;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + r * a.xs;
+        float s[1] = {0.f};
+#pragma unroll 8
+        for (int d = threadIdx.x; d < a.D; d += 1024) s[0] += (float)x[d];
+        row_sum<true, 1>(s, 1024, red[0]);
+        const float mean = s[0] * invd;
+        s[0] = 0.f;
+#pragma unroll 8
+        for (int d = threadIdx.x; d < a.D; d += 1024) {
+            const float u = (float)x[d] - mean;
+            s[0] = fmaf(u, u, s[0]);
+        }
+        row_sum<true, 1>(s, 1024, red[1]);
+        const float rstd = 1.f / sqrtf(fmaf(s[0], invd, a.eps));
+        T* y = static_cast<T*>(a.y) + r * a.D;
+        const auto finish = [&](auto kind) {
+            using W = decltype(kind);
+#pragma unroll 4
+            for (int d = threadIdx.x; d < a.D; d += 1024) {
+                float w[1], b[1];
+                load_w<1, W>(a.w, a.hw, d, w, 1.f);
+                load_w<1, W>(a.b, a.hb, d, b, 0.f);
+                y[d] = (T)fmaf(((float)x[d] - mean) * rstd, w[0], b[0]);
+            }
+        };
+        if (a.wf32) finish(float());
+        else finish(T());
+        if (a.stat && threadIdx.x == 0) a.stat[r] = make_float2(mean, rstd);
+    }
+}
+template <typename T> __global__ __launch_bounds__(1024) void ln_long_bwd_kernel(LnArgs a) {
+    __shared__ float red[2][2][16];
+    const float invd = 1.f / (float)a.D;
+    int par = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + r * a.xs;
+        const T* dy = static_cast<const T*>(a.dy) + r * a.dys;
+        const float2 st = a.stat[r];
+        const auto go = [&](auto kind) {
+            using W = decltype(kind);
+            float s[2] = {0.f, 0.f};
+#pragma unroll 4
+            for (int d = threadIdx.x; d < a.D; d += 1024) {
+                float w[1];
+                load_w<1, W>(a.w, a.hw, d, w, 1.f);
+                const float g = (float)dy[d] * w[0];
+                s[0] += g;
+                s[1] = fmaf(g, ((float)x[d] - st.x) * st.y, s[1]);
+            }
+            row_sum<true, 2>(s, 1024, red[par]);
+            const float c1 = s[0] * invd, c2 = s[1] * invd;
+            T* dx = static_cast<T*>(a.dx) + r * a.D;
+#pragma unroll 4
+            for (int d = threadIdx.x; d < a.D; d += 1024) {
+                float w[1];
+                load_w<1, W>(a.w, a.hw, d, w, 1.f);
+                const float xh = ((float)x[d] - st.x) * st.y;
+                dx[d] = (T)(st.y * ((float)dy[d] * w[0] - fmaf(xh, c2, c1)));
+            }
+        };
+        if (a.wf32) go(float());
+        else go(T());
+        par ^= 1;
+    }
+}
+// their partial dw, db: a thread owns a column, a block a slab of rows
 template <typename T> __global__ __launch_bounds__(256) void ln_long_cols_kernel(LnArgs a, int64_t slab) {
     const int d = blockIdx.x * 256 + threadIdx.x;
     if (d >= a.D) return;
@@ -381,85 +500,101 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_cols_kernel(con
 
 // ---------------------------------------------------------------- host
 struct LnPick {
-    int tpr, ept, block;  // block 0: sub-wave rows
+    int tpr, ept;   // lanes of a row, values of a lane
+    bool block;     // a block per row (tpr threads), else rows within waves
 };
 
-// the fewest threads that leave at most 32 values to each -- 16 in the backward, which holds two sums per column, and
-// 8 without 16-byte loads, where each value has an address of its own in flight
-LnPick ln_pick(int D, int V, bool bwd) {
-    LnPick p{64, V, 0};
+// Rows within a wave up to 64 lanes of 8 values (16 with 16-byte loads); behind that a block per row, of as many waves as
+// leave 8 values to a thread while that is up to 512 threads (1024 of single loads), 16 up to 1024, then 32.
+LnPick ln_pick(int D, int V) {
     if (D <= 64 * V) {
+        LnPick p{64, V, false};
         while (p.tpr > 1 && (p.tpr / 2) * V >= D) p.tpr /= 2;
         return p;
     }
-    const int cap = V == 1 ? 8 : bwd ? 16 : 32;
-    for (int e = 8; e <= cap; e *= 2)
-        if (D <= 64 * e) return {64, e, 0};
-    for (int e = 8; e <= cap; e *= 2)
-        if (D <= 256 * e) return {256, e, 256};
-    return {1024, D <= 1024 * 16 ? 16 : 32, 1024};
+    for (int e = 8; e <= (V > 1 ? 16 : 8); e *= 2)
+        if (e >= V && D <= 64 * e) return {64, e, false};
+    const auto threads = [&](int e) { return ((D + e - 1) / e + 63) / 64 * 64; };
+    if (threads(8) <= (V > 1 ? 512 : 1024)) return {threads(8), 8, true};
+    if (threads(16) <= 1024) return {threads(16), 16, true};
+    return {threads(32), 32, true};
 }
 
-// blocks of the backward's row pass: its partial sums are 8 D bytes per block, written and read once, next to the
-// rows' own 3 tensors; two blocks per CU unless a block would get fewer than 8 passes of rows
-int ln_bwd_blocks(int64_t rows, int D, int V) {
-    const bool narrow = D <= LN_NARROW;
-    int rpb, cap;
-    if (narrow) {
+int64_t ln_rows_per_block(int D, int V) {
+    if (D <= LN_NARROW) {
         int tpr = 1;
         while (tpr < D) tpr *= 2;
-        rpb = 256 / tpr;
-        cap = 256;
-    } else {
-        const LnPick p = ln_pick(D, V, true);
-        rpb = p.block ? 1 : 256 / p.tpr;
-        cap = p.block == 1024 ? 256 : 512;
+        return 256 / tpr;
     }
-    const int64_t passes = (rows + rpb - 1) / rpb;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(cap, (passes + 7) / 8));
+    const LnPick p = ln_pick(D, V);
+    return p.block ? 1 : 256 / p.tpr;
 }
 
-template <typename T, int V, int E, int BLOCK, bool BWD> int ln_go(const LnArgs& a, int blocks, hipStream_t s) {
+// as many blocks as give every block the same number of passes over rows, `most` or fewer
+int ln_even(int64_t passes, int64_t most) {
+    const int64_t each = (passes + most - 1) / most;
+    return (int)((passes + each - 1) / each);
+}
+
+// The forward keeps 1536 threads of a CU busy.  The backward's partial sums are 8 D bytes per block, written and read
+// once, next to the rows' own 3 tensors: 1024 threads a CU, and no block with fewer than 8 passes.
+int ln_fwd_blocks(int64_t rows, int D, int V) {
+    const int64_t rpb = ln_rows_per_block(D, V), passes = (rows + rpb - 1) / rpb;
+    const int threads = D > LN_NARROW && ln_pick(D, V).block ? ln_pick(D, V).tpr : 256;
+    return ln_even(passes, (int64_t)num_cus() * std::max(1, 1536 / threads));
+}
+int ln_bwd_blocks(int64_t rows, int D, int V) {
+    const int64_t rpb = ln_rows_per_block(D, V), passes = (rows + rpb - 1) / rpb;
+    const int threads = D > LN_NARROW && ln_pick(D, V).block ? ln_pick(D, V).tpr : 256;
+    const int64_t most = std::min<int64_t>((int64_t)num_cus() * std::max(1, 1024 / threads), (passes + 7) / 8);
+    return ln_even(passes, std::max<int64_t>(1, std::min<int64_t>(512, most)));
+}
+
+template <typename T, int V, int E, bool BLOCK, bool BWD> int ln_go(const LnArgs& a, int blocks, hipStream_t s) {
+    const int threads = BLOCK ? a.tpr : 256;
     if constexpr (BWD) {
-        const size_t sm = BLOCK == 0 && a.part ? (size_t)4 * a.D * sizeof(float) : 0;
-        if constexpr (E > 16) {
-            if (a.part) {
-                const int64_t slab = (a.rows + blocks - 1) / blocks;
-                ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
-                PCX_LAUNCH_CHECK("ln_long_cols_kernel");
-            }
-            if (!a.dx) return PCX_OK;
-        }
-        ln_bwd_kernel<T, V, E, BLOCK><<<blocks, BLOCK ? BLOCK : 256, sm, s>>>(a);
+        const size_t sm = !BLOCK && a.part ? (size_t)4 * a.D * sizeof(float) : 0;
+        ln_bwd_kernel<T, V, E, BLOCK><<<blocks, threads, sm, s>>>(a);
         PCX_LAUNCH_CHECK("ln_bwd_kernel");
     } else {
-        ln_fwd_kernel<T, V, E, BLOCK><<<blocks, BLOCK ? BLOCK : 256, 0, s>>>(a);
+        ln_fwd_kernel<T, V, E, BLOCK><<<blocks, threads, 0, s>>>(a);
         PCX_LAUNCH_CHECK("ln_fwd_kernel");
     }
     return PCX_OK;
 }
 
+template <typename T, bool BWD> int ln_long(const LnArgs& a, int blocks, hipStream_t s) {
+    if constexpr (BWD) {
+        if (a.part) {
+            const int64_t slab = (a.rows + blocks - 1) / blocks;
+            ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
+            PCX_LAUNCH_CHECK("ln_long_cols_kernel");
+        }
+        if (!a.dx) return PCX_OK;
+        ln_long_bwd_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_long_bwd_kernel");
+    } else {
+        ln_long_fwd_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_long_fwd_kernel");
+    }
+    return PCX_OK;
+}
+
 template <typename T, int V, bool BWD> int ln_dispatch(LnArgs a, int blocks, hipStream_t s) {
-    const LnPick p = ln_pick(a.D, V, BWD);
+    const LnPick p = ln_pick(a.D, V);
     a.tpr = p.tpr;
-    if (p.block == 0) {
-        if (p.ept == V) return ln_go<T, V, V, 0, BWD>(a, blocks, s);
+    if (!p.block) {
+        if (p.ept == V) return ln_go<T, V, V, false, BWD>(a, blocks, s);
         if constexpr (V < 8)
-            if (p.ept == 8) return ln_go<T, V, 8, 0, BWD>(a, blocks, s);
-        if constexpr (V > 1)
-            if (p.ept == 16) return ln_go<T, V, 16, 0, BWD>(a, blocks, s);
-        if constexpr (V > 1 && !BWD) return ln_go<T, V, 32, 0, BWD>(a, blocks, s);
+            if (p.ept == 8) return ln_go<T, V, 8, false, BWD>(a, blocks, s);
+        if constexpr (V > 1) return ln_go<T, V, 16, false, BWD>(a, blocks, s);
     }
-    if (p.block == 256) {
-        if constexpr (V == 1 || BWD)
-            if (p.ept == 8) return ln_go<T, V, 8, 256, BWD>(a, blocks, s);
-        if constexpr (V > 1)
-            if (p.ept == 16) return ln_go<T, V, 16, 256, BWD>(a, blocks, s);
-        if constexpr (V > 1 && !BWD) return ln_go<T, V, 32, 256, BWD>(a, blocks, s);
+    if (p.ept == 8) return ln_go<T, V, 8, true, BWD>(a, blocks, s);
+    if constexpr (V > 1) {
+        if (p.ept == 16) return ln_go<T, V, 16, true, BWD>(a, blocks, s);
+        if constexpr (!BWD) return ln_go<T, V, 32, true, false>(a, blocks, s);
     }
-    if constexpr (V == 1 || BWD)
-        if (p.ept == 16) return ln_go<T, V, 16, 1024, BWD>(a, blocks, s);
-    return ln_go<T, V, 32, 1024, BWD>(a, blocks, s);
+    return ln_long<T, BWD>(a, blocks, s);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -518,16 +653,7 @@ LnArgs ln_args(const LayerNormArgs& q) {
 int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s) {
     const LnArgs a = ln_args(q);
     const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
-    int rpb = 1;
-    if (a.D <= LN_NARROW) {
-        int tpr = 1;
-        while (tpr < a.D) tpr *= 2;
-        rpb = 256 / tpr;
-    } else {
-        const LnPick p = ln_pick(a.D, V, false);
-        rpb = p.block ? 1 : 256 / p.tpr;
-    }
-    const int blocks = (int)std::min<int64_t>(1 << 20, (a.rows + rpb - 1) / rpb);
+    const int blocks = ln_fwd_blocks(a.rows, a.D, V);
     const int bv = V > 1 ? blocks : 0;
     if (q.dtype == PCX_F32) return ln_run<float>(a, false, blocks, bv, s);
     if (q.dtype == PCX_BF16) return ln_run<bf16>(a, false, blocks, bv, s);
