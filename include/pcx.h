@@ -168,6 +168,8 @@ typedef struct pcx_net_config {
     int hidden_dims[4];   /* deep only */
     int use_residual;     /* deep only */
     int conv_bf16;        /* deep only: conv operands rounded to bf16, float32 accumulation (0: fp32) */
+    int proj_norm;        /* norm behind the projection: 0 BatchNorm1d, 1 layer norm (each embedding by itself: no
+                             running statistics in bn_stats, and a training batch of one is allowed) */
 } pcx_net_config;
 
 /* The cnn_deep convolution engine as a standalone op (src/models/phoneme_cnn.py:146-304 convs):

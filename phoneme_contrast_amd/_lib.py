@@ -44,7 +44,7 @@ class NetConfig(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("in_channels", ctypes.c_int),
                 ("embedding_dim", ctypes.c_int), ("use_attention", ctypes.c_int),
                 ("hidden_dims", ctypes.c_int * 4), ("use_residual", ctypes.c_int),
-                ("conv_bf16", ctypes.c_int)]
+                ("conv_bf16", ctypes.c_int), ("proj_norm", ctypes.c_int)]
 
 
 class MuonMatrix(ctypes.Structure):

@@ -258,6 +258,11 @@ int build_deep(Plan& p) {
     p.dh = p.carve("dh", (size_t)B * D * 4);
     p.dpooled = p.carve("dpooled", (size_t)B * K * 4);
     p.proj_part = p.carve("proj_part", proj_part_floats(B, D, K) * 4);
+    if (p.cfg.proj_norm) {
+        p.z = p.carve("z", (size_t)B * D * 4);
+        p.lnstat = p.carve("lnstat", (size_t)B * 8);
+        p.lnws = p.carve("lnws", layernorm_bwd_ws(B, D, 4));
+    }
     p.wt = p.carve("wt", (size_t)K * D * 4);
     p.hp_dwa = p.carve("hp_dwa", (size_t)K * B * 4);
     p.hp_dba = p.carve("hp_dba", (size_t)B * 4);
@@ -267,7 +272,7 @@ int build_deep(Plan& p) {
     if (p.cfg.use_attention) p.stages.push_back(d.ia);
     for (int i = 3; i >= 0; --i) p.stages.push_back(d.blk[i].pidx);
     p.stages.push_back(0);
-    p.nbn = bnidx + 1;
+    p.nbn = p.cfg.proj_norm ? bnidx : bnidx + 1;
     p.ndrop = 4;
     for (int i = 0; i < 4; ++i) p.drop_ch[i] = d.h[i];
     p.deep = dp;
@@ -634,9 +639,11 @@ int deep_forward(const Plan& p, const float* const* P, float* const* bnstat, int
         j.bias = P[ip + 1];
         j.gamma = P[ip + 2];
         j.beta = P[ip + 3];
-        j.rmean = bnp(d.bn_proj, 0);
-        j.rvar = bnp(d.bn_proj, 1);
-        j.nbt = nb(d.bn_proj);
+        if (!p.cfg.proj_norm) {
+            j.rmean = bnp(d.bn_proj, 0);
+            j.rvar = bnp(d.bn_proj, 1);
+            j.nbt = nb(d.bn_proj);
+        }
         j.momentum = 0.1f;
         j.eps = 1e-5f;
         j.train = train;
@@ -644,6 +651,7 @@ int deep_forward(const Plan& p, const float* const* P, float* const* bnstat, int
         j.cf = at<float4>(ws, p.cfp);
         j.emb = emb;
         j.norm = at<float>(ws, p.norm);
+        proj_layer_norm(p, j, ws);
         Scope sc(&p.prof, s, "proj_fwd");
         RC(launch_proj_fwd(j, s));
     }
@@ -684,6 +692,7 @@ int deep_backward(const Plan& p, const float* const* P, const float* x, const fl
         j.dgamma = G[ip + 2];
         j.dbeta = G[ip + 3];
         j.part = at<float>(ws, p.proj_part);
+        proj_layer_norm(p, j, ws);
         Scope sc(&p.prof, s, "proj_bwd");
         RC(launch_proj_bwd(j, s));
     }

@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256) void bn1d_fwd_kernel(ProjArgs a) {
     }
 }
 
-// e = z / max(||z||, 1e-12), z = h*s + t ; one wave per row
+// e = z / max(||z||, 1e-12), z = h*s + t (BatchNorm1d) or given (layer norm); one wave per row
 __global__ __launch_bounds__(256) void normalize_fwd_kernel(ProjArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -442,8 +442,12 @@ __global__ __launch_bounds__(256) void normalize_fwd_kernel(ProjArgs a) {
         int d = lane + 64 * k;
         z[k] = 0.f;
         if (d < a.D) {
-            float4 cf = a.cf[d];
-            z[k] = fmaf(a.h[b * a.D + d], cf.x, cf.y);
+            if (a.z) {
+                z[k] = a.z[b * a.D + d];
+            } else {
+                float4 cf = a.cf[d];
+                z[k] = fmaf(a.h[b * a.D + d], cf.x, cf.y);
+            }
             ss = fmaf(z[k], z[k], ss);
         }
     }
@@ -503,7 +507,7 @@ __global__ __launch_bounds__(256) void bn1d_bwd_kernel(ProjArgs a) {
     }
 }
 
-// dh = BN1d backward ; dpooled = dh @ W
+// dh = BN1d backward (layer norm: given) ; dpooled = dh @ W
 __global__ __launch_bounds__(256) void proj_bwd_data_kernel(ProjArgs a) {
     extern __shared__ __attribute__((aligned(16))) float sd[];  // [PR][D]
     const int b0 = blockIdx.x * PR, tid = threadIdx.x;
@@ -513,9 +517,13 @@ __global__ __launch_bounds__(256) void proj_bwd_data_kernel(ProjArgs a) {
         float v = 0.f;
         if (r < nr) {
             int64_t o = (int64_t)(b0 + r) * a.D + d;
-            float4 c = a.cfb[d];
-            v = c.x * (a.dzp[o] - c.y - (a.h[o] - c.w) * c.z);
-            a.dh[o] = v;
+            if (a.z) {
+                v = a.dh[o];
+            } else {
+                float4 c = a.cfb[d];
+                v = c.x * (a.dzp[o] - c.y - (a.h[o] - c.w) * c.z);
+                a.dh[o] = v;
+            }
         }
         sd[e] = v;
     }
@@ -643,24 +651,49 @@ int launch_head_pool_bwd(HeadPoolArgs a, hipStream_t s) {
     return PCX_OK;
 }
 
+#define RC_(x)                  \
+    do {                        \
+        int _rc = (x);          \
+        if (_rc) return _rc;    \
+    } while (0)
+
+static LayerNormArgs proj_layernorm(const ProjArgs& a) {
+    LayerNormArgs q{};
+    q.dtype = q.wdtype = PCX_F32;
+    q.rows = a.B;
+    q.D = a.D;
+    q.eps = a.eps;
+    q.x = a.h;
+    q.xs = a.D;
+    q.w = a.gamma;
+    q.b = a.beta;
+    q.y = a.z;
+    q.stat = a.lnstat;
+    q.dy = a.dzp;
+    q.dys = a.D;
+    q.dx = a.dh;
+    q.dw = a.dgamma;
+    q.db = a.dbeta;
+    q.ws = a.lnws;
+    return q;
+}
+
 int launch_proj_fwd(ProjArgs a, hipStream_t s) {
     PCX_CHECK_ARG(a.D <= 256, "projection: embedding_dim %d > 256 unsupported", a.D);
     size_t sm = (size_t)PR * a.K * sizeof(float);
     (void)hipFuncSetAttribute((const void*)proj_fwd_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
     proj_fwd_kernel<<<ceil_div(a.B, PR), 256, sm, s>>>(a);
     PCX_LAUNCH_CHECK("proj_fwd_kernel");
-    bn1d_fwd_kernel<<<a.D, 256, 0, s>>>(a);
-    PCX_LAUNCH_CHECK("bn1d_fwd_kernel");
+    if (a.z) {
+        RC_(launch_layernorm_fwd(proj_layernorm(a), s));
+    } else {
+        bn1d_fwd_kernel<<<a.D, 256, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("bn1d_fwd_kernel");
+    }
     normalize_fwd_kernel<<<ceil_div(a.B, 4), 256, 0, s>>>(a);
     PCX_LAUNCH_CHECK("normalize_fwd_kernel");
     return PCX_OK;
 }
-
-#define RC_(x)                  \
-    do {                        \
-        int _rc = (x);          \
-        if (_rc) return _rc;    \
-    } while (0)
 
 int proj_wg_nslice(int B) { return std::max(1, std::min(64, B / 64)); }
 size_t proj_part_floats(int B, int D, int K) { return (size_t)proj_wg_nslice(B) * D * (K + 1); }
@@ -668,8 +701,12 @@ size_t proj_part_floats(int B, int D, int K) { return (size_t)proj_wg_nslice(B) 
 int launch_proj_bwd(ProjArgs a, hipStream_t s) {
     normalize_bwd_kernel<<<ceil_div(a.B, 4), 256, 0, s>>>(a);
     PCX_LAUNCH_CHECK("normalize_bwd_kernel");
-    bn1d_bwd_kernel<<<a.D, 256, 0, s>>>(a);
-    PCX_LAUNCH_CHECK("bn1d_bwd_kernel");
+    if (a.z) {
+        RC_(launch_layernorm_bwd(proj_layernorm(a), s));
+    } else {
+        bn1d_bwd_kernel<<<a.D, 256, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("bn1d_bwd_kernel");
+    }
     size_t sm = (size_t)PR * a.D * sizeof(float);
     (void)hipFuncSetAttribute((const void*)proj_bwd_data_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sm);
     proj_bwd_data_kernel<<<ceil_div(a.B, PR), 256, sm, s>>>(a);

@@ -358,9 +358,14 @@ struct ProjArgs {
     float* dgamma;
     float* dbeta;
     float* part;           // [proj_part_floats] weight / bias gradient partials
+    // layer norm in place of BatchNorm1d (gamma, beta, dgamma, dbeta are its weight and bias): rmean .. cf, cfb unused
+    float* z;              // [B][D] its output (non-NULL selects it)
+    float* lnstat;         // [B][2]
+    void* lnws;            // layernorm_bwd_ws bytes
 };
 int proj_wg_nslice(int B);
 size_t proj_part_floats(int B, int D, int K);
+size_t layernorm_bwd_ws(int64_t rows, int D, int es);
 int launch_proj_fwd(ProjArgs a, hipStream_t s);
 int launch_proj_bwd(ProjArgs a, hipStream_t s);
 int launch_transpose(const float* in, float* out, int rows, int cols, hipStream_t s);
@@ -384,7 +389,6 @@ struct LayerNormArgs {
     void* db;              // [D] or NULL
     void* ws;              // layernorm_bwd_ws bytes
 };
-size_t layernorm_bwd_ws(int64_t rows, int D, int es);
 int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s);
 int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s);
 

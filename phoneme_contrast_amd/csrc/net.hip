@@ -138,6 +138,11 @@ int build_small(Plan& p) {
     p.dh = p.carve("dh", (size_t)B * D * 4);
     p.dpooled = p.carve("dpooled", (size_t)B * K * 4);
     p.proj_part = p.carve("proj_part", proj_part_floats(B, D, K) * 4);
+    if (p.cfg.proj_norm) {
+        p.z = p.carve("z", (size_t)B * D * 4);
+        p.lnstat = p.carve("lnstat", (size_t)B * 8);
+        p.lnws = p.carve("lnws", layernorm_bwd_ws(B, D, 4));
+    }
     p.wt = p.carve("wt", (size_t)K * D * 4);
     p.hp_dz = p.carve("hp_dz", (size_t)K * B * 4);
     p.hp_dzx = p.carve("hp_dzx", (size_t)K * B * 4);
@@ -148,7 +153,7 @@ int build_small(Plan& p) {
     p.stages = {p.cfg.use_attention ? 26 : 24};
     if (p.cfg.use_attention) p.stages.push_back(24);
     for (int l = 6; l >= 1; --l) p.stages.push_back(p_conv_w(l));
-    p.nbn = 7;
+    p.nbn = p.cfg.proj_norm ? 6 : 7;
     p.ndrop = 3;
     p.drop_ch[0] = 32; p.drop_ch[1] = 64; p.drop_ch[2] = 128;
     return PCX_OK;
@@ -279,9 +284,11 @@ int small_forward(const Plan& p, const float* const* P, float* const* bnstat, in
         j.bias = P[ip + 1];
         j.gamma = P[ip + 2];
         j.beta = P[ip + 3];
-        j.rmean = bnstat[12];
-        j.rvar = bnstat[13];
-        j.nbt = nbt ? nbt[6] : nullptr;
+        if (!p.cfg.proj_norm) {
+            j.rmean = bnstat[12];
+            j.rvar = bnstat[13];
+            j.nbt = nbt ? nbt[6] : nullptr;
+        }
         j.momentum = mom;
         j.eps = eps;
         j.train = train;
@@ -289,6 +296,7 @@ int small_forward(const Plan& p, const float* const* P, float* const* bnstat, in
         j.cf = at<float4>(ws, p.cfp);
         j.emb = emb;
         j.norm = at<float>(ws, p.norm);
+        proj_layer_norm(p, j, ws);
         { Scope sc(&p.prof, s, "proj_fwd"); RC(launch_proj_fwd(j, s)); }
     }
     return PCX_OK;
@@ -327,6 +335,7 @@ int small_backward(const Plan& p, const float* const* P, const float* x, const f
         j.dgamma = G[ip + 2];
         j.dbeta = G[ip + 3];
         j.part = at<float>(ws, p.proj_part);
+        proj_layer_norm(p, j, ws);
         { Scope sc(&p.prof, s, "proj_bwd"); RC(launch_proj_bwd(j, s)); }
     }
     p.buckets.mark(ip, s);
@@ -534,6 +543,7 @@ using pcx::Plan;
 extern "C" void* pcx_net_create(const pcx_net_config* cfg, int64_t B, int64_t F, int64_t T) {
     using namespace pcx;
     if (!cfg) { set_error("pcx_net_create: NULL config"); return nullptr; }
+    if (cfg->proj_norm != 0 && cfg->proj_norm != 1) { set_error("pcx_net_create: proj_norm %d (0 or 1)", cfg->proj_norm); return nullptr; }
     if (cfg->in_channels != 1) { set_error("pcx_net_create: in_channels must be 1 (MFCC input)"); return nullptr; }
     if (B < 1 || F < 1 || T < 1 || B * F * T > ((int64_t)1 << 40)) {
         set_error("pcx_net_create: bad input shape [%lld,1,%lld,%lld]", (long long)B, (long long)F, (long long)T);
@@ -596,7 +606,7 @@ extern "C" int pcx_net_forward(const void* plan, const float* const* params, flo
     PCX_CHECK_ARG(plan && params && bn_stats && x && emb && ws, "pcx_net_forward: NULL argument");
     const Plan* p = static_cast<const Plan*>(plan);
     if (ws_bytes < p->total) { set_error("pcx_net_forward: workspace too small"); return PCX_EWORKSPACE; }
-    if (train && p->B < 2) {
+    if (train && p->B < 2 && !p->cfg.proj_norm) {
         set_error("Expected more than 1 value per channel when training, got input size [1, %d]", p->D);
         return PCX_EINVAL;
     }

@@ -15,6 +15,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .layers import LayerNorm
 
 
 # ----------------------------------------------------------------------------- registry
@@ -211,7 +212,7 @@ class _NativeNet(BaseModel):
         for p in self.parameters():
             if p.device != x.device or p.dtype != torch.float32:
                 raise RuntimeError(f"{type(self).__name__}: parameters must be float32 on {x.device}")
-        if self.training and x.shape[0] == 1:
+        if self.training and x.shape[0] == 1 and self.projection_norm == "batch":
             raise ValueError("Expected more than 1 value per channel when training, got input size "
                              f"torch.Size([1, {self.embedding_dim}])")
         x = x.contiguous().float()
@@ -288,6 +289,14 @@ class SpatialAttention(nn.Module):
         self.conv = nn.Conv2d(in_channels, 1, kernel_size=1)
 
 
+def _projection(cin, dim, norm):
+    """Linear + BatchNorm1d, or (MI355X addition, config["projection_norm"] = "layer") Linear + layer norm: each embedding
+    normalised by itself, so it depends on no other sample of the batch, no running statistics and no rank."""
+    if norm not in ("batch", "layer"):
+        raise ValueError(f"projection_norm {norm!r} (batch | layer)")
+    return nn.Sequential(nn.Linear(cin, dim), nn.BatchNorm1d(dim) if norm == "batch" else LayerNorm(dim))
+
+
 def _double_conv(cin, cout, p, pool):
     """conv-BN-ReLU x2 (+ MaxPool2d(2)) + Dropout2d, child indices as the reference's blocks."""
     layers = [nn.Conv2d(cin, cout, 3, padding=1), nn.BatchNorm2d(cout), nn.ReLU(inplace=True),
@@ -301,7 +310,7 @@ def _double_conv(cin, cout, p, pool):
 @model_registry.register("phoneme_cnn")
 class PhonemeNet(_NativeNet):
     """cnn_small (reference src/models/phoneme_cnn.py:10-126): 3 conv blocks 1->32->64->128,
-    SpatialAttention, global average pool, Linear+BatchNorm1d, L2 normalisation."""
+    SpatialAttention, global average pool, Linear+BatchNorm1d (or layer norm), L2 normalisation."""
 
     _kind = 0
 
@@ -311,6 +320,7 @@ class PhonemeNet(_NativeNet):
         self.embedding_dim = config.get("embedding_dim", 128)
         self.use_attention = config.get("use_attention", True)
         self.dropout_rate = config.get("dropout_rate", 0.1)
+        self.projection_norm = config.get("projection_norm", "batch")
         self._build_network()
         self._initialize_weights()
 
@@ -324,8 +334,7 @@ class PhonemeNet(_NativeNet):
         if self.use_attention:
             self.attention = SpatialAttention(128)
         self.global_pool = nn.AdaptiveAvgPool2d(1)
-        self.projection = nn.Sequential(nn.Linear(128, self.embedding_dim),
-                                        nn.BatchNorm1d(self.embedding_dim))
+        self.projection = _projection(128, self.embedding_dim, self.projection_norm)
 
     def _net_config(self):
         cfg = _lib.NetConfig()
@@ -333,6 +342,7 @@ class PhonemeNet(_NativeNet):
         cfg.in_channels = self.in_channels
         cfg.embedding_dim = self.embedding_dim
         cfg.use_attention = 1 if self.use_attention else 0
+        cfg.proj_norm = 1 if self.projection_norm == "layer" else 0
         return cfg
 
 
@@ -356,7 +366,7 @@ class ResidualBlock(nn.Module):
 @model_registry.register("phoneme_cnn_deep")
 class PhonemeNetDeep(_NativeNet):
     """cnn_deep (reference src/models/phoneme_cnn.py:187-304): 7x7 stem + MaxPool(3,2,1), four
-    ResidualBlocks (strides 1,2,2,2), SpatialAttention, pool, Linear+BatchNorm1d, normalize."""
+    ResidualBlocks (strides 1,2,2,2), SpatialAttention, pool, Linear+BatchNorm1d (or layer norm), normalize."""
 
     _kind = 1
 
@@ -366,6 +376,7 @@ class PhonemeNetDeep(_NativeNet):
         self.embedding_dim = config.get("embedding_dim", 128)
         self.use_attention = config.get("use_attention", True)
         self.dropout_rate = config.get("dropout_rate", 0.2)
+        self.projection_norm = config.get("projection_norm", "batch")
         self.hidden_dims = list(config.get("hidden_dims", [64, 128, 256, 512]))
         self.use_residual = config.get("use_residual", True)
         # MI355X addition: "bf16" runs every convolution on bf16 operands with float32 accumulation
@@ -396,8 +407,7 @@ class PhonemeNetDeep(_NativeNet):
         if self.use_attention:
             self.attention = SpatialAttention(h[-1])
         self.global_pool = nn.AdaptiveAvgPool2d(1)
-        self.projection = nn.Sequential(nn.Linear(h[-1], self.embedding_dim),
-                                        nn.BatchNorm1d(self.embedding_dim))
+        self.projection = _projection(h[-1], self.embedding_dim, self.projection_norm)
 
     def _net_config(self):
         cfg = _lib.NetConfig()
@@ -405,6 +415,7 @@ class PhonemeNetDeep(_NativeNet):
         cfg.in_channels = self.in_channels
         cfg.embedding_dim = self.embedding_dim
         cfg.use_attention = 1 if self.use_attention else 0
+        cfg.proj_norm = 1 if self.projection_norm == "layer" else 0
         for i, d in enumerate(self.hidden_dims[:4]):
             cfg.hidden_dims[i] = d
         cfg.use_residual = 1 if self.use_residual else 0

@@ -32,7 +32,7 @@ from phoneme_contrast_amd.data import (GpuContrastiveBatches, GpuEvalBatches, Sh
 from phoneme_contrast_amd.features import GpuViewBuilder, build_feature_extractor  # noqa: E402
 from phoneme_contrast_amd.losses import GlobalSupervisedContrastiveLoss, get_loss_fn  # noqa: E402
 from phoneme_contrast_amd.models import model_registry  # noqa: E402
-from phoneme_contrast_amd.optim import FusedAdam  # noqa: E402
+from phoneme_contrast_amd.optim import FusedAdam, FusedMuon  # noqa: E402
 from phoneme_contrast_amd.samplers import ContrastiveBatchSampler  # noqa: E402
 from phoneme_contrast_amd.trainer import ContrastiveTrainer  # noqa: E402
 from phoneme_contrast_amd.transforms import build_augmentation_pipeline  # noqa: E402
@@ -95,7 +95,12 @@ def setup_model(cfg, device, world=1):
     model = model_registry.create(cfg.model.type, dict(cfg.model)).to(device)
     ddp.broadcast_module(model)
     wd = cfg.training.get("weight_decay", 0)
-    if cfg.accel.get("fused_adam", True):
+    kind = cfg.accel.get("optimizer", "adam")
+    if kind not in ("adam", "muon"):
+        raise ValueError(f"accel.optimizer {kind!r} (adam | muon)")
+    if kind == "muon":
+        optimizer = FusedMuon(model.parameters(), lr=cfg.training.learning_rate, weight_decay=wd)
+    elif cfg.accel.get("fused_adam", True):
         optimizer = FusedAdam(model.parameters(), lr=cfg.training.learning_rate, weight_decay=wd)
     else:
         optimizer = torch.optim.Adam(model.parameters(), lr=cfg.training.learning_rate, weight_decay=wd)
