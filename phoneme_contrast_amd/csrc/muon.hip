@@ -1056,6 +1056,30 @@ template <typename F> unsigned ns_blocks(const NsTable& t, NsUnits& un, F per) {
     return (unsigned)n;
 }
 
+// pairs of tiles along the long side, and the bytes of a matrix's planes in LDS if one block holds it (0 if not): at most
+// two pairs a wave, and one of A's
+int ns_block_pairs(const NsMat& e) {
+    return ((std::min(e.rows, e.cols) + 31) / 32) * ((std::max(e.rows, e.cols) + 63) / 64);
+}
+int ns_block_bytes(const NsMat& e) {
+    if (std::min(e.rows, e.cols) > 128 || std::max(e.rows, e.cols) > 1024 || ns_block_pairs(e) > 2 * NSB_WAVES) return 0;
+    const int64_t mp = round_up(std::min(e.rows, e.cols), 32), np = round_up(std::max(e.rows, e.cols), 32);
+    const int64_t bytes = 4 * (mp * np + (int64_t)mp * mp);
+    return bytes <= NSB_LDS ? (int)bytes : 0;
+}
+
+// the launch's matrices in blocks of their own: bytes of LDS and pairs of the largest; false if one does not fit
+bool ns_in_blocks(const NsTable& t, int* bytes, int* pairs) {
+    *bytes = *pairs = 0;
+    for (int i = 0; i < t.count; ++i) {
+        const int b = ns_block_bytes(t.e[i]);
+        if (!b) return false;
+        *bytes = std::max(*bytes, b);
+        *pairs = std::max(*pairs, ns_block_pairs(t.e[i]));
+    }
+    return true;
+}
+
 // One launch table's workspace: partial sums and unit of every matrix, counters and partial products of split tiles,
 // then the planes.  Fills in the places; returns its size.
 int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
@@ -1065,6 +1089,8 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
         mats += t.e[i].batch;
     }
     t.mats = (int)mats;
+    int bytes, pairs;
+    if (ns_in_blocks(t, &bytes, &pairs)) return 256;  // (nothing passes through memory)
     for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
         const NsPlan p = ns_plan(t, ph);
         counters = std::max(counters, p.counters);
@@ -1117,18 +1143,6 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
     return PCX_OK;
 }
 
-// pairs of tiles along the long side, and the bytes of a matrix's planes in LDS if one block holds it (0 if not): at most
-// two pairs a wave, and one of A's
-int ns_block_pairs(const NsMat& e) {
-    return ((std::min(e.rows, e.cols) + 31) / 32) * ((std::max(e.rows, e.cols) + 63) / 64);
-}
-int ns_block_bytes(const NsMat& e) {
-    if (std::min(e.rows, e.cols) > 128 || std::max(e.rows, e.cols) > 1024 || ns_block_pairs(e) > 2 * NSB_WAVES) return 0;
-    const int64_t mp = round_up(std::min(e.rows, e.cols), 32), np = round_up(std::max(e.rows, e.cols), 32);
-    const int64_t bytes = 4 * (mp * np + (int64_t)mp * mp);
-    return bytes <= NSB_LDS ? (int)bytes : 0;
-}
-
 template <int T> int ns_block_as(const NsTable& t, const NsUnits& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
     if (sm > 64 * 1024)
         (void)hipFuncSetAttribute((const void*)ns_block_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
@@ -1139,13 +1153,8 @@ template <int T> int ns_block_as(const NsTable& t, const NsUnits& un, const NsAr
 
 int ns_run(const NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
     NsUnits un{};
-    int most = 0, pairs = 0;
-    for (int i = 0; i < t.count && most >= 0; ++i) {
-        const int bytes = ns_block_bytes(t.e[i]);
-        most = bytes ? std::max(most, bytes) : -1;
-        pairs = std::max(pairs, ns_block_pairs(t.e[i]));
-    }
-    if (most > 0) {  // every matrix of the launch fits a block
+    int most, pairs;
+    if (ns_in_blocks(t, &most, &pairs)) {
         NsCoef c{};
         c.steps = steps;
         memcpy(c.c, coef, 3 * steps * sizeof(float));

@@ -39,7 +39,8 @@ def test_orthogonalize_refuses_before_any_launch():
     # growing steps: the bound follows the iteration
     assert call(steps=3, c=coef(*(3.0, 0, 0) * 3)) == _lib.PCX_EINVAL
     assert lib.pcx_orthogonalize_workspace_bytes(1, 0, 4) == 0 and lib.pcx_orthogonalize_workspace_bytes(0, 4, 4) == 0
-    assert lib.pcx_orthogonalize_workspace_bytes(3, 100, 40) > lib.pcx_orthogonalize_workspace_bytes(1, 100, 40) > 0
+    assert lib.pcx_orthogonalize_workspace_bytes(3, 400, 300) > lib.pcx_orthogonalize_workspace_bytes(1, 400, 300) > 0
+    assert lib.pcx_orthogonalize_workspace_bytes(3, 100, 40) > 0
 
 
 def test_muon_step_refuses_before_any_launch():
