@@ -103,7 +103,8 @@ int pcx_adam_step(float* p, const float* g, float* m, float* v, int64_t n, int64
  * Statistics, sums and products are in float32 (rows of up to 32 values: float64); each output is rounded once.
  * The forward writes stats [rows][2] = {mean, 1 / sqrt(var + eps)} for the backward, or keeps nothing when it is
  * NULL (rows of up to 32 values never write it: the backward forms them from x).  The backward computes any of
- * dx, dw = sum_rows dy xhat and db = sum_rows dy (NULL: not wanted; dw, db in wdtype; workspace needed for them).
+ * dx, dw = sum_rows dy xhat and db = sum_rows dy (NULL: not wanted; dw, db in wdtype; workspace for them, of 0 bytes
+ * for few rows).
  * Deterministic. */
 size_t pcx_layernorm_workspace_bytes(int dtype, int64_t rows, int64_t D);
 int pcx_layernorm_forward(int dtype, int wdtype, int64_t rows, int64_t D, const void* x, int64_t x_stride,

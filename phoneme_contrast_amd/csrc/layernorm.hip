@@ -26,10 +26,11 @@ typedef _Float16 f16;
 
 constexpr int LN_MAX = 32768;    // 1024 threads x 32 values
 constexpr int LN_NARROW = 32;    // rows up to here: 64-bit arithmetic, one value per lane
+constexpr int LN_ALONE = 8192;   // rows up to here: a single block writes dw and db itself
 
 struct LnArgs {
     int64_t rows;
-    int D, tpr, wf32;            // tpr: lanes of a sub-wave row; wf32: w and b are float32 (else x's type)
+    int D, tpr, wf32, cf32;      // tpr: lanes of a sub-wave row; wf32, cf32: w and b, dw and db are float32 (else x's type)
     float eps;
     const void* x;
     int64_t xs;                  // row strides in elements
@@ -41,7 +42,10 @@ struct LnArgs {
     const void* dy;
     int64_t dys;
     void* dx;                    // NULL: not wanted
-    float* part;                 // [blocks][2][D] partial dw, db; NULL: not wanted
+    bool cols;                   // dw, db wanted
+    float* part;                 // [blocks][2][D] partial dw, db; NULL: one block, which writes them itself
+    void* dw;
+    void* db;
 };
 
 template <typename T, int V> struct Pack {
@@ -84,6 +88,18 @@ template <int V, typename W> __device__ __forceinline__ void load_w(const void* 
     load_v<V>(static_cast<const W*>(w) + d, v);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = has ? v[j] : none;
+}
+
+// a block's sum of column d (pass 0: dw, 1: db)
+template <typename T> __device__ __forceinline__ void put_column(const LnArgs& a, int pass, int d, float v) {
+    if (a.part) {
+        a.part[((int64_t)blockIdx.x * 2 + pass) * a.D + d] = v;
+        return;
+    }
+    void* out = pass ? a.db : a.dw;
+    if (!out) return;
+    if (a.cf32) static_cast<float*>(out)[d] = v;
+    else static_cast<T*>(out)[d] = (T)v;
 }
 
 // sums over the lanes of a row: tpr lanes of a wave, or (BLOCK) all waves of the block through `red` with one barrier; the
@@ -295,8 +311,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
             }
         }
     }
-    if (!a.part) return;
-    float* pw = a.part + (int64_t)blockIdx.x * 2 * a.D;
+    if (!a.cols) return;
     if constexpr (BLOCK) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -304,8 +319,8 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
             if (d < a.D) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    pw[d + j] = sw[c][j];
-                    pw[a.D + d + j] = sb[c][j];
+                    put_column<T>(a, 0, d + j, sw[c][j]);
+                    put_column<T>(a, 1, d + j, sb[c][j]);
                 }
             }
         }
@@ -326,7 +341,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
             }
             __syncthreads();
             for (int d = threadIdx.x; d < a.D; d += 256)
-                pw[pass * a.D + d] = (cols[d] + cols[a.D + d]) + (cols[2 * a.D + d] + cols[3 * a.D + d]);
+                put_column<T>(a, pass, d, (cols[d] + cols[a.D + d]) + (cols[2 * a.D + d] + cols[3 * a.D + d]));
             __syncthreads();
         }
     }
@@ -374,8 +389,7 @@ template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow
         }
     }
     if constexpr (BWD) {
-        if (!a.part) return;
-        float* pw = a.part + (int64_t)blockIdx.x * 2 * a.D;
+        if (!a.cols) return;
 #pragma unroll
         for (int pass = 0; pass < 2; ++pass) {
             double t = pass ? sb : sw;
@@ -383,8 +397,8 @@ template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow
             if ((threadIdx.x & 63) < (unsigned)tpr && in) cols[threadIdx.x >> 6][d] = t;
             __syncthreads();
             if (threadIdx.x < (unsigned)a.D)
-                pw[pass * a.D + threadIdx.x] = (float)((cols[0][threadIdx.x] + cols[1][threadIdx.x]) +
-                                                       (cols[2][threadIdx.x] + cols[3][threadIdx.x]));
+                put_column<T>(a, pass, threadIdx.x, (float)((cols[0][threadIdx.x] + cols[1][threadIdx.x]) +
+                                                            (cols[2][threadIdx.x] + cols[3][threadIdx.x])));
             __syncthreads();
         }
     }
@@ -553,7 +567,7 @@ int ln_bwd_blocks(int64_t rows, int D, int V) {
 template <typename T, int V, int E, bool BLOCK, bool BWD> int ln_go(const LnArgs& a, int blocks, hipStream_t s) {
     const int threads = BLOCK ? a.tpr : 256;
     if constexpr (BWD) {
-        const size_t sm = !BLOCK && a.part ? (size_t)4 * a.D * sizeof(float) : 0;
+        const size_t sm = !BLOCK && a.cols ? (size_t)4 * a.D * sizeof(float) : 0;
         ln_bwd_kernel<T, V, E, BLOCK><<<blocks, threads, sm, s>>>(a);
         PCX_LAUNCH_CHECK("ln_bwd_kernel");
     } else {
@@ -565,7 +579,7 @@ template <typename T, int V, int E, bool BLOCK, bool BWD> int ln_go(const LnArgs
 
 template <typename T, bool BWD> int ln_long(const LnArgs& a, int blocks, hipStream_t s) {
     if constexpr (BWD) {
-        if (a.part) {
+        if (a.cols) {
             const int64_t slab = (a.rows + blocks - 1) / blocks;
             ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
             PCX_LAUNCH_CHECK("ln_long_cols_kernel");
@@ -627,7 +641,7 @@ bool ln_vectors(const LnArgs& a, int es) {
 size_t layernorm_bwd_ws(int64_t rows, int D, int es) {
     if (rows <= 0 || D <= 0) return 0;
     const int n = std::max(ln_bwd_blocks(rows, D, 1), ln_bwd_blocks(rows, D, 16 / es));
-    return (size_t)n * 2 * D * sizeof(float);
+    return n > 1 || D > LN_ALONE ? (size_t)n * 2 * D * sizeof(float) : 0;
 }
 
 LnArgs ln_args(const LayerNormArgs& q) {
@@ -662,14 +676,18 @@ int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s) {
 
 int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s) {
     LnArgs a = ln_args(q);
-    a.part = q.dw || q.db ? static_cast<float*>(q.ws) : nullptr;
+    a.cols = q.dw || q.db;
+    a.dw = q.dw;
+    a.db = q.db;
+    a.cf32 = q.wdtype == PCX_F32;
     const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
     const int blocks = ln_bwd_blocks(a.rows, a.D, V);
+    if (blocks > 1 || a.D > LN_ALONE) a.part = static_cast<float*>(q.ws);
     const int bv = V > 1 ? blocks : 0;
     int rc = q.dtype == PCX_F32 ? ln_run<float>(a, true, blocks, bv, s)
              : q.dtype == PCX_BF16 ? ln_run<bf16>(a, true, blocks, bv, s)
                                    : ln_run<f16>(a, true, blocks, bv, s);
-    if (rc || !a.part) return rc;
+    if (rc || !a.cols || !a.part) return rc;
     const int cb = ceil_div(2 * (int64_t)a.D, 32);
     if (q.wdtype == PCX_F32)
         ln_cols_kernel<float><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<float*>(q.dw), static_cast<float*>(q.db));
@@ -722,9 +740,9 @@ extern "C" int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64
     PCX_CHECK_ARG(rows >= 1, "layernorm_backward: no rows");
     PCX_CHECK_ARG(x && dy && stats, "layernorm_backward: NULL buffer");
     if (!dx && !dw && !db) return PCX_OK;
-    if ((dw || db) && (!ws || ws_bytes < pcx_layernorm_workspace_bytes(dtype, rows, D))) {
-        set_error("layernorm_backward: workspace of %zu bytes, %zu needed", ws_bytes,
-                  pcx_layernorm_workspace_bytes(dtype, rows, D));
+    const size_t need = pcx_layernorm_workspace_bytes(dtype, rows, D);
+    if ((dw || db) && need && (!ws || ws_bytes < need)) {
+        set_error("layernorm_backward: workspace of %zu bytes, %zu needed", ws_bytes, need);
         return PCX_EWORKSPACE;
     }
     LayerNormArgs q{};

@@ -343,7 +343,7 @@ template <int WM, int WN, int NB> struct Product {
     static constexpr int TM = 64 * WM, TN = 64 * WN;
     static constexpr int PB = TM * 64, QB = TN * 64;        // bytes of a plane's tile
     static constexpr int STAGE = 2 * (PB + QB);
-    static constexpr int LDS = NB * STAGE > (TM + 1) * TN * 4 ? NB * STAGE : (TM + 1) * TN * 4;  // (the epilogue's tile)
+    static constexpr int LDS = NB * STAGE > (TM + 4) * TN * 4 ? NB * STAGE : (TM + 4) * TN * 4;  // (the epilogue's tile)
     static constexpr int COPIES = 2 * (WM + WN);            // of a wave and stage
 
     static constexpr int READS = 2 * (WM + WN), MFMAS = 3 * WM * WN;
@@ -595,7 +595,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     }
     // The tile goes through LDS, [column][row], so that both passes over it touch whole lines of memory: along the rows
     // first, where the old values are added, then across.
-    constexpr int LS = G::TM + 1;
+    constexpr int LS = G::TM + 4;  // (float4 along the rows; 16 lanes apart by columns share a bank, never 8)
     float* tv = reinterpret_cast<float*>(sm);
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -607,7 +607,9 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
             for (int j = 0; j < WN; ++j) {
                 float* at = tv + ((wave >> 1) * 32 * WN + 32 * j + (lane & 31)) * LS + (wave & 1) * 32 * WM + 32 * i;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) at[acc_row(x, lane >> 5)] = acc[i][j][x] * k;
+                for (int g = 0; g < 4; ++g)
+                    st4(at + acc_row(4 * g, lane >> 5), make_float4(acc[i][j][4 * g] * k, acc[i][j][4 * g + 1] * k,
+                                                                    acc[i][j][4 * g + 2] * k, acc[i][j][4 * g + 3] * k));
             }
         __syncthreads();
     }
@@ -619,7 +621,8 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
         if (r >= nr || c >= nc) continue;
         if (SYM && (r0 + r) / 64 < (c0 + c) / 64) continue;  // (the mirrored block writes it)
         float* at = tv + c * LS + r;
-        float v[4] = {at[0], at[1], at[2], at[3]};
+        const float4 was = ld4(at);
+        float v[4] = {was.x, was.y, was.z, was.w};
         const int64_t o = at_panel(c0 + c, r0 + r, orow);
         if (PHASE != NS_GRAM) {
             const f16x4 oh = EARLY ? eh[EARLY ? x0 / 256 : 0] : *reinterpret_cast<const f16x4*>(oldh + o);
@@ -634,10 +637,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
             *reinterpret_cast<f16x4*>(outh + o) = h;
             *reinterpret_cast<f16x4*>(outl + o) = l;
         }
-        if (PHASE >= NS_POLY) {
-#pragma unroll
-            for (int y = 0; y < 4; ++y) at[y] = v[y];
-        }
+        if (PHASE >= NS_POLY) st4(at, make_float4(v[0], v[1], v[2], v[3]));
     }
     __syncthreads();
     if (PHASE != NS_LAST) {

@@ -122,7 +122,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             size_t nws = 0;
             if (need_w || need_b) {
                 nws = pcx_layernorm_workspace_bytes(dt, rows, D);
-                ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
+                if (nws) ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
             }
             check_status(pcx_layernorm_backward(dt, wdt, rows, D, xr.const_data_ptr(), xs, address(w), (float)eps,
                                                 stats.const_data_ptr<float>(), dyr.const_data_ptr(), dys,

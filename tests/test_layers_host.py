@@ -19,7 +19,7 @@ def test_c_entry_points_refuse_before_any_launch():
     def fwd(dt=0, wdt=0, rows=4, D=8, x=buf, xs=8, eps=1e-5, y=buf):
         return lib.pcx_layernorm_forward(dt, wdt, rows, D, x, xs, None, None, eps, y, None, None)
 
-    def bwd(dt=0, wdt=0, rows=4, D=8, xs=8, dys=8, stats=buf, dx=buf, dw=buf, ws=buf, nws=1 << 20, eps=1e-5):
+    def bwd(dt=0, wdt=0, rows=4000, D=8, xs=8, dys=8, stats=buf, dx=buf, dw=buf, ws=buf, nws=1 << 20, eps=1e-5):
         return lib.pcx_layernorm_backward(dt, wdt, rows, D, buf, xs, None, eps, stats, buf, dys, dx, dw, None, ws, nws, None)
     for rc in (fwd(dt=3), fwd(dt=-1), fwd(dt=0, wdt=1), fwd(dt=1, wdt=2), fwd(rows=-1), fwd(D=0), fwd(D=32769), fwd(x=None),
                fwd(y=None), fwd(xs=7), fwd(eps=0.0), fwd(eps=-1.0), fwd(eps=float("nan")), fwd(eps=float("inf")),
