@@ -22,7 +22,11 @@
 // one of rows with rows.  A plane is stored in panels of 32 values of K, [K / 32][rows][32]: what a tile needs of a panel
 // is one run of memory.  (Row by row, the rows of a tile lie a power of two apart more often than not and queue at one
 // L2 channel: 5160 us for 4096 x 4096 in bfloat16, 4836 us in panels, all else alike.)
-// A and B are symmetric: only tiles on and above the diagonal are computed, and written twice.
+// A and B are symmetric: only tiles on and below the diagonal are computed, and written twice.
+//
+// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.93 ms, which are 0.52 PFLOP/s of
+// the three products' definition and 1.05 PFLOP/s executed (three terms, half of the tiles of A and B).  Small ones: the
+// latency of a product launch (fetching addresses, filling LDS, the epilogue's passes), 5 to 8 us of which 2 to 3 compute.
 #include <math.h>
 
 #include <algorithm>
@@ -688,6 +692,150 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     else finish(f16(), Plain<f16>());
 }
 
+// ---------------------------------------------------------------- products of few tiles
+// 32 x 32 tiles, all waves of a block on one of them, each on every W-th stage of K: nothing is shared between waves, so
+// operands go from memory straight to registers, three stages ahead, with no barrier until the waves' sums meet in LDS.
+// Four times the blocks of 64 x 64 tiles and a quarter of the epilogue for each, for launches that are all latency.
+constexpr int NSF_WAVES = 8;
+
+template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_kernel(NsTable t, NsUnits un, NsArgs q) {
+    constexpr bool SYM = PHASE <= NS_POLY;
+    constexpr int W = NSF_WAVES, LS = 36, AHEAD = 3;
+    __shared__ __attribute__((aligned(16))) float tv[W][32 * LS];
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
+    const NsMat& e = t.e[ei];
+    const unsigned rel = blockIdx.x - un.first[ei], tiles = un.tiles[ei];
+    const int bat = e.batch == 1 ? 0 : rel / tiles;
+    int tl = rel - bat * tiles;
+    const Planes p = planes_of(q, e, bat);
+    const bool tall = PHASE == NS_LAST && e.rows > e.cols;
+    int r0, c0;
+    Rows P, Q;
+    if (SYM) {
+        int ti = 0;
+        for (; tl > ti; ++ti) tl -= ti + 1;
+        r0 = ti * 32;
+        c0 = tl * 32;
+        const f16* hi = PHASE == NS_GRAM ? p.x(q.src, 0) : p.a(0);
+        const f16* lo = PHASE == NS_GRAM ? p.x(q.src, 1) : p.a(1);
+        P = Rows{hi, lo, r0, e.mp};
+        Q = Rows{hi, lo, c0, e.mp};
+    } else {
+        const int tc = (tall ? e.np : e.mp) / 32, tr = (unsigned)tl / (unsigned)tc;
+        r0 = tr * 32;
+        c0 = (tl - tr * tc) * 32;
+        const Rows B{p.b(0), p.b(1), tall ? r0 : c0, e.mp};
+        const Rows X{p.xt(q.src, 0), p.xt(q.src, 1), tall ? c0 : r0, e.np};
+        P = tall ? B : X;
+        Q = tall ? X : B;
+    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int stages = (PHASE == NS_GRAM ? e.np : e.mp) / NS_K;
+    // each thread's four values of the result: rows r .. r + 3 of column c
+    const int c = (threadIdx.x & 255) >> 3, r = (threadIdx.x & 7) * 4;
+    const bool mine = threadIdx.x < 256;
+    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
+    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
+    const int64_t o = at_panel(c0 + c, r0 + r, tall ? e.np : e.mp);
+    f16x4 oh{}, ol{};
+    if (PHASE != NS_GRAM) {
+        oh = *reinterpret_cast<const f16x4*>(oldh + o);
+        ol = *reinterpret_cast<const f16x4*>(oldl + o);
+    }
+    const float unit = q.unit[e.mat + bat];
+
+    const unsigned off = (lane & 31) * 64 + (lane >> 5) * 16;
+    const char* base[4] = {uniform(P.hi + P.first * 32), uniform(P.lo + P.first * 32), uniform(Q.hi + Q.first * 32),
+                           uniform(Q.lo + Q.first * 32)};
+    const int64_t kp = (int64_t)P.rows * 64, kq = (int64_t)Q.rows * 64;
+    f16x8 f[AHEAD][2][4];  // [stage][half][P hi, P lo, Q hi, Q lo]
+    const auto fetch = [&](int s, f16x8 (&g)[2][4]) {
+        const int k = min(s, stages - 1);  // (behind the end: not used)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                g[h][y] = *reinterpret_cast<const f16x8*>(base[y] + k * (y < 2 ? kp : kq) + off + 32 * h);
+    };
+    f32x16 a0{}, a1{}, a2{};
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) fetch(wave + i * W, f[i]);
+    for (int s = wave; s < stages; s += AHEAD * W) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (s + i * W < stages) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    a0 = mfma16(f[i][h][0], f[i][h][3], a0);
+                    a1 = mfma16(f[i][h][1], f[i][h][2], a1);
+                    a2 = mfma16(f[i][h][0], f[i][h][2], a2);
+                }
+            }
+            if (s + (i + AHEAD) * W < stages) fetch(s + (i + AHEAD) * W, f[i]);
+        }
+    }
+    a2 += a0 + a1;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        st4(&tv[wave][(lane & 31) * LS + acc_row(4 * g, lane >> 5)],
+            make_float4(a2[4 * g], a2[4 * g + 1], a2[4 * g + 2], a2[4 * g + 3]));
+    __syncthreads();
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (mine) {
+        const int used = min(W, stages);
+        for (int w = 0; w < used; ++w) {
+            const float4 x = ld4(&tv[w][c * LS + r]);
+            v[0] += x.x;
+            v[1] += x.y;
+            v[2] += x.z;
+            v[3] += x.w;
+        }
+        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? q.c / q.sa : 1.f / q.sa;
+        const float fo = PHASE == NS_POLY ? q.b : q.a;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] = PHASE == NS_GRAM ? v[y] * k : fmaf(fo, (float)oh[y] + (float)ol[y], v[y] * k);
+    }
+    if (PHASE != NS_LAST) {
+        f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
+        f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
+        f16x4 h, l;
+        split4(v, h, l);
+        if (mine) {
+            *reinterpret_cast<f16x4*>(outh + o) = h;
+            *reinterpret_cast<f16x4*>(outl + o) = l;
+        }
+        if (SYM && r0 == c0) return;  // (the same for the block)
+        __syncthreads();
+        if (mine) st4(&tv[0][c * LS + r], make_float4(v[0], v[1], v[2], v[3]));
+        __syncthreads();
+        if (!mine) return;
+        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - q.src, 0) : outh;
+        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - q.src, 1) : outl;
+        const float w[4] = {tv[0][r * LS + c], tv[0][(r + 1) * LS + c], tv[0][(r + 2) * LS + c], tv[0][(r + 3) * LS + c]};
+        split4(w, h, l);
+        const int64_t oa = at_panel(r0 + c, c0 + r, PHASE == NS_APPLY ? e.np : e.mp);
+        *reinterpret_cast<f16x4*>(acrh + oa) = h;
+        *reinterpret_cast<f16x4*>(acrl + oa) = l;
+        return;
+    }
+    if (!mine || c0 + c >= e.rows) return;
+    const auto finish = [&](auto kind, auto put) {
+        using T = decltype(kind);
+        T* out = static_cast<T*>(e.out) + (int64_t)bat * e.rows * e.cols + (int64_t)(c0 + c) * e.cols + r0 + r;
+        T old[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+            if (r0 + r + y < e.cols) old[y] = put.old(out + y);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+            if (r0 + r + y < e.cols) out[y] = put(old[y], v[y] * unit);
+    };
+    if (q.is_step) finish(float(), Descend{q.decay, e.step});
+    else if (q.dtype == PCX_F32) finish(float(), Plain<float>());
+    else if (q.dtype == PCX_BF16) finish(bf16(), Plain<bf16>());
+    else finish(f16(), Plain<f16>());
+}
+
 // ---------------------------------------------------------------- small matrices: all steps in one block
 // X of up to 32 tiles of 32 x 32 stays in the registers of eight waves (in float32, T tiles a wave); its planes, X for the
 // gram product and then X^T, and the planes of A and then B pass through LDS.  A launch per product costs 5 us and more
@@ -971,7 +1119,7 @@ void ns_bounds(const float* coef, int steps, double* smax, double* bmax, double*
     }
 }
 
-constexpr int NS_TM[2] = {64, 128}, NS_PER_CU[2] = {3, 2};  // tile edges; blocks a CU holds (LDS)
+constexpr int NS_TM[3] = {64, 128, 32}, NS_PER_CU[3] = {3, 2, 1};  // of NsConfig: tile edges; blocks a CU holds
 
 // tiles of one matrix of an entry in a phase
 int64_t ns_tiles(const NsMat& e, int phase, int edge) {
@@ -984,19 +1132,28 @@ int ns_stages(const NsMat& e, int phase) { return (phase == NS_GRAM ? e.np : e.m
 // Measured, us for 64 / 128: X <- a X + B X of 1536 x 1536 (144 tiles of 128) 38 / 43, 1024 x 4096 (256) 51 / 39,
 // 2048 x 2048 (256) 81 / 70; A = X X^T of 4 x 1024 x 1024 (144, K 1024) 31 / 32, 2048 x 2048 (136, K 2048) 52 / 46,
 // 3 x 1536 x 1536 (234) 59 / 55: large tiles from one per CU on, with K of 2048 from one per two CUs.
-int ns_config(const NsTable& t, int phase) {
-    int64_t n = 0, deep = 0;
+// 32 x 32 tiles are for launches that are all latency.  us for 32 / 64: A A of 512 x 512 (36 tiles of 64) 6.3 / 8.2,
+// B X of 512 x 512 (64) 7.9 / 9.6, X X^T of 512 x 2048 (36, 64 stages) 11.5 / 12.4 but of 512 x 4608 (144 stages)
+// 20.4 / 16.9, A A of 6 x 333 x 333 (126) 11.3 / 8.2: up to a 64 x 64 tile per four CUs and 64 stages.
+enum NsConfig { NS_TILE64, NS_TILE128, NS_TILE32 };
+NsConfig ns_config(const NsTable& t, int phase) {
+    int64_t n = 0, small = 0, deep = 0;
+    int most = 0;
     for (int i = 0; i < t.count; ++i) {
         const int64_t k = ns_tiles(t.e[i], phase, 128) * t.e[i].batch;
+        const int stages = ns_stages(t.e[i], phase);
         n += k;
-        if (ns_stages(t.e[i], phase) >= 64) deep += k;
+        small += ns_tiles(t.e[i], phase, 64) * t.e[i].batch;
+        most = std::max(most, stages);
+        if (stages >= 64) deep += k;
     }
-    return n >= num_cus() || 2 * deep >= num_cus();
+    if (4 * small <= num_cus() && most <= 64) return NS_TILE32;
+    return n >= num_cus() || 2 * deep >= num_cus() ? NS_TILE128 : NS_TILE64;
 }
 
 struct NsPlan {
     NsUnits un;
-    int cfg;
+    NsConfig cfg;
     unsigned blocks;
     int64_t counters, joint;  // split tiles, floats of their parts
 };
@@ -1027,7 +1184,7 @@ NsPlan ns_plan(const NsTable& t, int phase) {
             // and parts of less than 48 stages do not pay
             split = std::min<int64_t>((int64_t)(sqrt(0.6 * stages[i]) + 0.5), std::max<int64_t>(1, slots / all));
         }
-        split = std::min<int64_t>(split, 16);
+        split = p.cfg == NS_TILE32 ? 1 : std::min<int64_t>(split, 16);  // (there the waves share K)
         if (split == 1) whole = n;
         p.un.whole[i] = (int)whole;
         p.un.split[i] = (int)split;
@@ -1129,7 +1286,12 @@ template <int PHASE, int WM, int WN, int NB> int ns_product_as(const NsTable& t,
 }
 template <int PHASE> int ns_product(const NsTable& t, const NsArgs& q, hipStream_t s) {
     const NsPlan p = ns_plan(t, PHASE);
-    if (p.cfg == 0) return ns_product_as<PHASE, 1, 1, 3>(t, p, q, s);
+    if (p.cfg == NS_TILE32) {
+        ns_few_kernel<PHASE><<<p.blocks, 64 * NSF_WAVES, 0, s>>>(t, p.un, q);
+        PCX_LAUNCH_CHECK("ns_few_kernel");
+        return PCX_OK;
+    }
+    if (p.cfg == NS_TILE64) return ns_product_as<PHASE, 1, 1, 3>(t, p, q, s);
     return ns_product_as<PHASE, 2, 2, 2>(t, p, q, s);
 }
 
