@@ -5,7 +5,6 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -74,6 +73,16 @@ Tensor forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t D, dou
     return y;
 }
 
+// The gradient as a function of x, w and dy: it is not differentiable, and says so when asked to be.
+struct LayerNormGradient : torch::autograd::Function<LayerNormGradient> {
+    static variable_list forward(AutogradContext*, at::TensorList all, int64_t n) {
+        return variable_list(all.begin(), all.begin() + n);
+    }
+    static variable_list backward(AutogradContext*, const variable_list&) {
+        TORCH_CHECK(false, "layer_norm: its gradient is not differentiable");
+    }
+};
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
     // (an absent tensor has no edge: needs_input_grad counts x and those that are there)
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
@@ -132,13 +141,17 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
                                                 nws ? ws.mutable_data_ptr() : nullptr, nws, stream_of(x)),
                          "pcx_layernorm_backward");
         }
-        variable_list out{dx, dw, db};
-        if (at::GradMode::is_enabled()) {  // create_graph: the gradient is not differentiable, and says so when asked to be
-            auto no = std::make_shared<torch::autograd::DelayedError>("layer_norm: its gradient is not differentiable", 3);
-            out = (*no)(std::move(out));
+        if (at::GradMode::is_enabled()) {  // create_graph
+            variable_list all;
+            for (const Tensor& t : {dx, dw, db, x, w, grads[0]})
+                if (t.defined()) all.push_back(t);
+            const int64_t n = dx.defined() + dw.defined() + db.defined();
+            const variable_list out = LayerNormGradient::apply(at::TensorList(all), n);
+            int64_t k = 0;
+            for (Tensor* t : {&dx, &dw, &db})
+                if (t->defined()) *t = out[k++];
         }
-        out.resize(5);
-        return out;
+        return {dx, dw, db, Tensor(), Tensor()};
     }
 };
 

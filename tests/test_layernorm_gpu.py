@@ -307,3 +307,47 @@ def test_refusals_on_the_device():
             bad()
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         layer_norm(x, 8, torch.ones(8))
+
+
+def test_autograd_contract():
+    """A second derivative is refused, an input changed before its backward pass is noticed, a result may be changed."""
+    from phoneme_contrast_amd.layers import layer_norm
+    x, w, b, dy = (t.cuda() for t in inputs(6, 40, torch.float32, torch.float32, 15))
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    (gx,) = torch.autograd.grad(layer_norm(x, 40, w, b), [x], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(gx.square().sum(), [x])
+    plain = torch.autograd.grad(layer_norm(x, 40, w, b), leaves, dy)
+    y = layer_norm(x, 40, w, b)
+    y.mul_(2.0)
+    for a, c in zip(plain, torch.autograd.grad(y, leaves, dy)):
+        assert torch.equal(2 * a, c)  # (a power of two goes through every rounding)
+    for t in (x, w):
+        h, y = t * 1, None
+        y = layer_norm(h if t is x else x, 40, h if t is w else w, b)
+        h.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(y, [x], dy)
+    with torch.inference_mode():
+        assert torch.equal(layer_norm(x, 40, w, b), layer_norm(x.detach(), 40, w, b))
+    twice = layer_norm(x, 40, w, w)  # one tensor in both places: its gradient is the sum
+    assert torch.equal(torch.autograd.grad(twice, [w], dy)[0], plain[1] + plain[2])
+
+
+@pytest.mark.parametrize("D", [128, 8192, 8193, 16384, 16392, 32768])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_writes_stay_inside_their_tensors(D, t):
+    """Rows between guards, input and gradient in views of wider buffers off 16-byte alignment."""
+    from phoneme_contrast_amd.layers import layer_norm
+    x, w, b, dy = inputs(3, D, TYPES[t], TYPES[t], 16)
+    wide = torch.full((3, 2 * D + 6), 3.0, dtype=TYPES[t])
+    wide[:, 1:D + 1], wide[:, D + 3:2 * D + 3] = x, dy
+    wide = wide.cuda()
+    before = wide.clone()
+    vx, vdy = wide[:, 1:D + 1].requires_grad_(True), wide[:, D + 3:2 * D + 3]
+    wd, bd = w.cuda().requires_grad_(True), b.cuda().requires_grad_(True)
+    y = layer_norm(vx, D, wd, bd)
+    got = [y.detach(), *torch.autograd.grad(y, [vx, wd, bd], vdy)]
+    assert torch.equal(wide.detach(), before)
+    for a, r, tol, what in zip(got, *reference(x, w, b, dy, 1e-5), ("y", "dx", "dw", "db")):
+        close(a, r, tol, what)
