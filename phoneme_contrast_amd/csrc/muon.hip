@@ -1181,7 +1181,7 @@ NsPlan ns_plan(const NsTable& t, int phase) {
             if (n > whole) split = std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / 16));
         } else if (stages[i] >= 48) {
             // a stage takes about 0.17 us, meeting in memory 4 us and 0.3 us a part: sqrt(0.6 stages) parts are the best,
-            // and parts of less than 48 stages do not pay
+            // and no meeting pays for K of less than 48 stages
             split = std::min<int64_t>((int64_t)(sqrt(0.6 * stages[i]) + 0.5), std::max<int64_t>(1, slots / all));
         }
         split = p.cfg == NS_TILE32 ? 1 : std::min<int64_t>(split, 16);  // (there the waves share K)

@@ -280,7 +280,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
 
     with k = 0.2 sqrt(max(rows, cols)) (adjust "rms": the size of an Adam update, so that its learning rate and decay
     serve), sqrt(max(1, rows / cols)) ("spectral") or 1 (None).  A weight of more than two axes is the matrix of its
-    first axis against the rest.  All tensors float32, contiguous and on one GPU, no weight twice."""
+    first axis against the rest.  All tensors float32, contiguous and on one GPU; no parameter or buffer shares memory
+    with another tensor of the call (a gradient may appear twice)."""
     params, grads, buffers = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(buffers):
         raise ValueError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(buffers)} momentum buffers")
@@ -291,7 +292,7 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
         return
     dev = params[0].device
     mats = (_lib.MuonMatrix * len(params))()
-    written = set()
+    spans = []
     for i, (p, g, m) in enumerate(zip(params, grads, buffers)):
         _lib.require_gpu(p, g, m, what="muon_step")
         if p.dim() < 2 or p.numel() == 0:
@@ -303,13 +304,17 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
                 raise ValueError(f"muon_step: {name} {i} must be contiguous float32")
             if t.device != dev:
                 raise RuntimeError(f"muon_step: {name} {i} is on {t.device}, parameter 0 on {dev}")
-        written.update((p.data_ptr(), m.data_ptr()))
+            spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel(), name != "gradient"))
         rows, cols = _matrix_shape(p)
         e = mats[i]
         e.param, e.grad, e.momentum, e.rows, e.cols = p.data_ptr(), g.data_ptr(), m.data_ptr(), rows, cols
         e.scale = _update_scale(adjust, rows, cols)
-    if len(written) != 2 * len(params):
-        raise ValueError("muon_step: a parameter or momentum buffer appears twice")
+    any_end = written_end = 0  # (gradients are read again once the buffers are written: only they may share memory)
+    for start, end, is_written in sorted(spans):
+        if start < written_end or (is_written and start < any_end):
+            raise ValueError("muon_step: a parameter or momentum buffer shares memory with another tensor of the call")
+        any_end = max(any_end, end)
+        written_end = max(written_end, end) if is_written else written_end
     _muon_launch(mats, len(params), params[0], lr, momentum, nesterov, weight_decay, grad_scale, ns_steps, coef, eps)
 
 

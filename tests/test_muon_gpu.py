@@ -365,3 +365,57 @@ def test_step_in_a_captured_graph():
         torch.cuda.synchronize()
         for a, b in zip(p + m, p2 + m2):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("batch,rows,cols", [
+    (3, 1100, 2100), (3, 2100, 1100),  # 128 x 128 tiles over ragged edges, in every product
+    (1, 1856, 1856),                   # more 64 x 64 tiles than the card holds at a time: the last ones in parts
+    (1, 2900, 2900),                   # the same of 128 x 128 tiles
+    (1, 600, 5000), (1, 5000, 600),    # parts of a long K
+    (40, 150, 90), (7, 40, 3000)])     # many small ones, and short sides of a long K
+def test_every_way_to_cut_the_products(batch, rows, cols):
+    from phoneme_contrast_amd.optim import orthogonalize
+    x = torch.stack([gradient(rows, cols, 50 + i) for i in range(batch)])
+    out = orthogonalize(x.cuda())
+    for i in sorted({0, batch - 1}):
+        close(out[i], x[i].double(), steps=5)
+    assert torch.equal(out, orthogonalize(x.cuda()))
+
+
+def test_memory_shared_between_the_tensors_of_a_step():
+    from phoneme_contrast_amd.optim import muon_step
+    flat = torch.randn(400, device="cuda")
+    p, g, m = flat[:72].view(8, 9), flat[72:144].view(8, 9), flat[144:216].view(8, 9)
+    near = flat[180:252].view(8, 9)  # half of m
+    before = flat.clone()
+    for ps, gs, ms in (([p], [m], [m]), ([p], [p], [m]), ([p], [near], [m]), ([p, near], [g, g], [m, flat[300:372].view(8, 9)]),
+                       ([p], [g], [g]), ([p], [g], [flat[36:108].view(8, 9)])):
+        with pytest.raises(ValueError, match="shares memory"):
+            muon_step(ps, gs, ms, lr=0.1)
+    assert torch.equal(flat, before)
+    q, n = flat[216:288].view(8, 9), flat[288:360].view(8, 9)
+    ref = [reference_step(a, g, b, 0.1, 0.95, True, 0.0, "rms") for a, b in ((p, m), (q, n))]
+    muon_step([p, q], [g, g], [m, n], lr=0.1)  # neighbours, and one gradient for two
+    for a, (r, _, tol) in zip((p, q), ref):
+        assert (a.cpu().double() - r).norm().item() <= tol
+    assert torch.equal(g, before[72:144].view(8, 9)) and torch.equal(flat[360:], before[360:])
+
+
+def test_writes_stay_inside_their_tensors():
+    """Views between guards of a flat buffer, at offsets off every alignment but float32's."""
+    from phoneme_contrast_amd.optim import muon_step
+    for rows, cols in ((31, 65), (130, 700), (700, 130), (1, 9)):
+        n = rows * cols
+        flat = torch.full((3 * n + 100,), 7.0, device="cuda")
+        views = [flat[17 + i * (n + 13):17 + i * (n + 13) + n].view(rows, cols) for i in range(3)]
+        p, g, m = (gradient(rows, cols, s) for s in range(3))
+        for v, t in zip(views, (p, g, m)):
+            v.copy_(t)
+        ref, _, tol = reference_step(p, g, m, 0.1, 0.95, True, 0.0, "rms")
+        muon_step([views[0]], [views[1]], [views[2]], lr=0.1)
+        assert (views[0].cpu().double() - ref).norm().item() <= tol
+        assert torch.equal(views[1].cpu(), g)
+        guard = torch.ones_like(flat, dtype=torch.bool)
+        for i in range(3):
+            guard[17 + i * (n + 13):17 + i * (n + 13) + n] = False
+        assert (flat[guard] == 7.0).all()
