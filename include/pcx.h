@@ -120,8 +120,11 @@ int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64_t D, const
  * in [0, 1] beyond 8 are refused.  The short side is at most 16384, the long one 2^20, a matrix 2^31 values.
  * Deterministic.
  *
- * pcx_orthogonalize: `batch` matrices [rows][cols] of one type, any strides (in elements) -> out [batch][rows][cols].
- * pcx_muon_step: for every matrix of the list (float32, contiguous, none twice)
+ * Workspaces start on 256 bytes.
+ *
+ * pcx_orthogonalize: `batch` matrices [rows][cols] of one type, any strides (in elements) -> out [batch][rows][cols],
+ * apart from x.
+ * pcx_muon_step: for every matrix of the list (float32, contiguous; params and momenta apart from all other tensors)
  *   momentum <- mu momentum + (1 - mu) grad_scale grad
  *   u = nesterov ? (1 - mu) grad_scale grad + mu momentum : momentum
  *   param <- (1 - lr weight_decay) param - lr scale orthogonalized(u)

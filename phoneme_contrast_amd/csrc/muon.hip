@@ -1434,8 +1434,8 @@ extern "C" int pcx_orthogonalize(int dtype, int64_t batch, int64_t rows, int64_t
     NsTable t{};
     ns_single(t, batch, rows, cols);
     const int64_t need = ns_place(t, q, ws);
-    if (!ws || (int64_t)ws_bytes < need) {
-        set_error("orthogonalize: workspace of %zu bytes, %lld needed", ws_bytes, (long long)need);
+    if (!ws || ((uintptr_t)ws & 255) || (int64_t)ws_bytes < need) {
+        set_error("orthogonalize: workspace of %zu bytes, %lld on a 256-byte boundary needed", ws_bytes, (long long)need);
         return PCX_EWORKSPACE;
     }
     NsMat& e = t.e[0];
@@ -1478,8 +1478,8 @@ extern "C" int pcx_muon_step(const pcx_muon_matrix* mats, int n, float lr, float
         for (int i = 0; i < t.count; ++i)
             PCX_CHECK_ARG(t.e[i].x && t.e[i].out && t.e[i].mom, "muon_step: NULL buffer of matrix %d", at + i);
         const int64_t need = ns_place(t, q, ws);
-        if (!ws || (int64_t)ws_bytes < need) {
-            set_error("muon_step: workspace of %zu bytes, %lld needed", ws_bytes, (long long)need);
+        if (!ws || ((uintptr_t)ws & 255) || (int64_t)ws_bytes < need) {
+            set_error("muon_step: workspace of %zu bytes, %lld on a 256-byte boundary needed", ws_bytes, (long long)need);
             return PCX_EWORKSPACE;
         }
     }

@@ -171,6 +171,8 @@ class FusedAdam(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
+        if any(("ns_steps" in g) != isinstance(self, FusedMuon) for g in state_dict["param_groups"]):
+            raise ValueError(f"{type(self).__name__}: this is the state of another optimizer")
         super().load_state_dict(state_dict)
         self._flat = [None] * len(self.param_groups)
 
@@ -452,8 +454,3 @@ class FusedMuon(FusedAdam):
                     voff += k
                 off += k
         return torch.optim.Optimizer.state_dict(self)
-
-    def load_state_dict(self, state_dict):
-        if any("ns_steps" not in g for g in state_dict["param_groups"]):
-            raise ValueError("FusedMuon: this is the state of another optimizer")
-        super().load_state_dict(state_dict)

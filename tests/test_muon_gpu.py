@@ -419,3 +419,22 @@ def test_writes_stay_inside_their_tensors():
         for i in range(3):
             guard[17 + i * (n + 13):17 + i * (n + 13) + n] = False
         assert (flat[guard] == 7.0).all()
+
+
+def test_states_of_the_two_optimizers_are_told_apart():
+    from phoneme_contrast_amd.optim import FusedAdam, FusedMuon
+    a, b = small_model(1), small_model(1)
+    oa, ob = FusedAdam(a.parameters()), FusedMuon(b.parameters())
+    for mdl, o in ((a, oa), (b, ob)):
+        set_grads(mdl, 0)
+        o.step()
+    for o, other in ((oa, ob), (ob, oa)):
+        before = [t.clone() for t in (a if o is oa else b).parameters()]
+        with pytest.raises(ValueError, match="another optimizer"):
+            o.load_state_dict(other.state_dict())
+        for p, q in zip(before, (a if o is oa else b).parameters()):
+            assert torch.equal(p, q)
+        o.load_state_dict(o.state_dict())
+    plain = torch.optim.Adam([torch.nn.Parameter(p.detach().clone()) for p in a.parameters()])
+    oa.load_state_dict(plain.state_dict())
+    plain.load_state_dict(oa.state_dict())

@@ -84,3 +84,14 @@ def test_which_parameters_are_matrices():
     assert not any(_is_matrix(torch.empty(s)) for s in ((5,), (1, 512, 1, 1), (7, 1), (0, 4), ()))
     assert _update_scale("rms", 64, 576) == pytest.approx(0.2 * 24) and _update_scale("spectral", 64, 16) == 2.0
     assert _update_scale("spectral", 16, 64) == 1.0 and _update_scale(None, 3, 4) == 1.0
+
+
+def test_workspaces_off_their_boundary_are_refused():
+    from phoneme_contrast_amd import _lib
+    lib = _lib.lib()
+    c = coef(3.0, -4.0, 2.0)
+    arr = (_lib.MuonMatrix * 1)((BUF, BUF, BUF, 8, 9, 1.0))
+    for ws in (BUF + 128, BUF + 1):
+        assert lib.pcx_orthogonalize(0, 1, 8, 8, BUF, 64, 8, 1, BUF, 1, c, 1e-7, ws, 1 << 30, None) == _lib.PCX_EWORKSPACE
+        assert lib.pcx_muon_step(arr, 1, 0.1, 0.9, 1, 0.0, 1.0, 1, c, 1e-7, ws, 1 << 30, None) == _lib.PCX_EWORKSPACE
+        assert "boundary" in _lib.last_error()
