@@ -27,6 +27,7 @@
 // What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.93 ms, which are 0.52 PFLOP/s of
 // the three products' definition and 1.05 PFLOP/s executed (three terms, half of the tiles of A and B).  Small ones: the
 // latency of a product launch (fetching addresses, filling LDS, the epilogue's passes), 5 to 8 us of which 2 to 3 compute.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -68,7 +69,7 @@ struct NsTable {
 // Work units of a product launch, per entry: its tiles in order, the first `whole` over all of K, the others in `split`
 // parts each (joined by whichever unit of a tile ends last, in part order).
 struct NsUnits {
-    int first[NS_LIST + 1];      // units of the launch up to each entry
+    int first[NS_LIST];          // units of the launch up to each entry; behind the last, more than there are
     int tiles[NS_LIST];          // tiles of one matrix of the entry
     int whole[NS_LIST];          // of the entry's tiles times batch
     int split[NS_LIST];
@@ -123,10 +124,13 @@ __device__ __forceinline__ Planes planes_of(const NsArgs& q, const NsMat& e, int
     return p;
 }
 
+// (all of the table at once: searched in a loop, each look waits for the one before)
 __device__ __forceinline__ int find_entry(const int* first, int count, int blk) {
+    if (count == 1) return 0;
     int i = 0;
-    while (i + 1 < count && blk >= first[i + 1]) ++i;
-    return i;
+#pragma unroll
+    for (int k = 1; k < NS_LIST; ++k) i += blk >= first[k];
+    return __builtin_amdgcn_readfirstlane(i);
 }
 
 // blocks go to the 8 XCDs in turn: block b of n works as unit xcd_order(b, n), which gives each XCD (its own L2) adjacent
@@ -572,7 +576,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
 #pragma unroll
                 for (int j = 0; j < WN; ++j) acc[i][j] = f32x16{};
             const uint64_t* from = reinterpret_cast<const uint64_t*>(q.joint + (int64_t)(un.joint[ei] + over % cut) * SZ) + threadIdx.x;
-            constexpr int FLY = WM * WN == 1 ? 4 : 2;  // parts in flight
+            constexpr int FLY = WM * WN == 1 ? 5 : 2;  // parts in flight (8 would cost a CU its third block: 17 -> 19 us at 512 x 4608)
             for (int k = 0; k < split; k += FLY) {
 #pragma unroll
                 for (int i = 0; i < WM; ++i)
@@ -1181,7 +1185,8 @@ NsPlan ns_plan(const NsTable& t, int phase) {
             if (n > whole) split = std::max<int64_t>(1, std::min<int64_t>(slots / (n - whole), stages[i] / 16));
         } else if (stages[i] >= 48) {
             // a stage takes about 0.17 us, meeting in memory 4 us and 0.3 us a part: sqrt(0.6 stages) parts are the best,
-            // and no meeting pays for K of less than 48 stages
+            // and no meeting pays for K of less than 48 stages.  (More parts of the longest K in a list, up to as many
+            // units as the card holds: 22.8 us against 20.9 for X X^T of the deep network's weights.)
             split = std::min<int64_t>((int64_t)(sqrt(0.6 * stages[i]) + 0.5), std::max<int64_t>(1, slots / all));
         }
         split = p.cfg == NS_TILE32 ? 1 : std::min<int64_t>(split, 16);  // (there the waves share K)
@@ -1195,7 +1200,7 @@ NsPlan ns_plan(const NsTable& t, int phase) {
         parts += (n - whole) * split;
         units += whole + (n - whole) * split;
     }
-    p.un.first[t.count] = (int)units;
+    for (int i = t.count; i < NS_LIST; ++i) p.un.first[i] = INT_MAX;
     p.blocks = (unsigned)units;
     p.joint = parts * edge * edge;
     return p;
@@ -1209,7 +1214,7 @@ template <typename F> unsigned ns_blocks(const NsTable& t, NsUnits& un, F per) {
         un.first[i] = (int)n;
         n += per(t.e[i]) * t.e[i].batch;
     }
-    un.first[t.count] = (int)n;
+    for (int i = t.count; i < NS_LIST; ++i) un.first[i] = INT_MAX;
     return (unsigned)n;
 }
 
