@@ -111,7 +111,7 @@ struct Planes {
 };
 // value (row, k) of a plane of `rows` rows
 __device__ __forceinline__ int64_t at_panel(int row, int k, int rows) {
-    return ((int64_t)(k >> 5) * rows + row) * 32 + (k & 31);
+    return ((int64_t)(k >> 3) * rows + row) * 8 + (k & 7);
 }
 __host__ __device__ inline int64_t plane_bytes(int mp, int np) {
     return 2 * (8 * (int64_t)mp * np + 4 * (int64_t)mp * mp);
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsUnits un, Ns
     }
     __syncthreads();
     for (int k = threadIdx.x; k < 64 * 16; k += 256) {
-        const int r = (k >> 3) & 63, c = (k & 7) * 4 + (k >> 9) * 32;
+        const int r = (k >> 1) & 63, c = (k & 1) * 4 + (k >> 7) * 8;
         f16x4 h, l, ht, lt;
         const float va[4] = {tile[r][c], tile[r][c + 1], tile[r][c + 2], tile[r][c + 3]};
         const float vt[4] = {tile[c][r], tile[c + 1][r], tile[c + 2][r], tile[c + 3][r]};
@@ -351,24 +351,24 @@ template <int WM, int WN, int NB> struct Product {
     static constexpr int TM = 64 * WM, TN = 64 * WN;
     static constexpr int PB = TM * 64, QB = TN * 64;        // bytes of a plane's tile
     static constexpr int STAGE = 2 * (PB + QB);
-    static constexpr int LDS = NB * STAGE > (TM + 4) * TN * 4 ? NB * STAGE : (TM + 4) * TN * 4;  // (the epilogue's tile)
+    static constexpr int LDS = NB * STAGE > (TM + 8) * TN * 4 ? NB * STAGE : (TM + 8) * TN * 4;  // (the epilogue's tile)
     static constexpr int COPIES = 2 * (WM + WN);            // of a wave and stage
 
     static constexpr int READS = 2 * (WM + WN), MFMAS = 3 * WM * WN;
 
     // operand t of a stage's half, this lane's 8 values
     __device__ static const char* operand_at(const char* st, int half) {
-        const int lane = threadIdx.x & 63, l32 = lane & 31, run = 2 * half + (lane >> 5);
-        return st + l32 * 64 + 16 * (run ^ ((l32 >> 2) & 3));  // (rows differ by multiples of 32 between the operands)
+        const int lane = threadIdx.x & 63;
+        return st + (2 * half + (lane >> 5)) * TM * 16 + (lane & 31) * 16;
     }
     template <int T> __device__ static void read(const char* at, Frags<WM, WN>& f) {
         const int wave = threadIdx.x >> 6;
-        const char* p = at + (wave & 1) * 2048 * WM;
-        const char* c = at + 2 * PB + (wave >> 1) * 2048 * WN;
-        if constexpr (T < WM) f.ph[T] = *reinterpret_cast<const f16x8*>(p + 2048 * T);
-        else if constexpr (T < WM + WN) f.ql[T - WM] = *reinterpret_cast<const f16x8*>(c + QB + 2048 * (T - WM));
-        else if constexpr (T < 2 * WM + WN) f.pl[T - WM - WN] = *reinterpret_cast<const f16x8*>(p + PB + 2048 * (T - WM - WN));
-        else f.qh[T - 2 * WM - WN] = *reinterpret_cast<const f16x8*>(c + 2048 * (T - 2 * WM - WN));
+        const char* p = at + (wave & 1) * 512 * WM;
+        const char* c = at + 2 * PB + (wave >> 1) * 512 * WN;
+        if constexpr (T < WM) f.ph[T] = *reinterpret_cast<const f16x8*>(p + 512 * T);
+        else if constexpr (T < WM + WN) f.ql[T - WM] = *reinterpret_cast<const f16x8*>(c + QB + 512 * (T - WM));
+        else if constexpr (T < 2 * WM + WN) f.pl[T - WM - WN] = *reinterpret_cast<const f16x8*>(p + PB + 512 * (T - WM - WN));
+        else f.qh[T - 2 * WM - WN] = *reinterpret_cast<const f16x8*>(c + 512 * (T - 2 * WM - WN));
     }
     // MFMA t of a half: the small terms first, neighbours in different accumulators
     template <int T> __device__ static void mfma(const Frags<WM, WN>& f, f32x16 (&acc)[WM][WN]) {
@@ -406,23 +406,17 @@ template <int WM, int WN, int NB> struct Product {
         const unsigned lds0 = (unsigned)(uintptr_t)(lds_void*)sm;
         unsigned offp[WM], offq[WN];  // (rows behind the planes' last: that one again, for sums that nobody stores)
 #pragma unroll
-        for (int i = 0; i < WM; ++i) {  // this wave's 16-row groups wave, wave + 4, ...
-            const int r = (wave + 4 * i) * 16 + (lane >> 2);
-            offp[i] = (unsigned)(min(r, P.rows - P.first - 1) * 64 + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
-        }
+        for (int i = 0; i < WM; ++i) offp[i] = (unsigned)(wave * P.rows + min(64 * i + lane, P.rows - P.first - 1)) * 16;
 #pragma unroll
-        for (int i = 0; i < WN; ++i) {
-            const int r = (wave + 4 * i) * 16 + (lane >> 2);
-            offq[i] = (unsigned)(min(r, Q.rows - Q.first - 1) * 64 + 16 * ((lane & 3) ^ ((r >> 2) & 3)));
-        }
-        const char* base[4] = {uniform(P.hi + P.first * 32), uniform(P.lo + P.first * 32), uniform(Q.hi + Q.first * 32),
-                               uniform(Q.lo + Q.first * 32)};
+        for (int i = 0; i < WN; ++i) offq[i] = (unsigned)(wave * Q.rows + min(64 * i + lane, Q.rows - Q.first - 1)) * 16;
+        const char* base[4] = {uniform(P.hi + P.first * 8), uniform(P.lo + P.first * 8), uniform(Q.hi + Q.first * 8),
+                               uniform(Q.lo + Q.first * 8)};
         // copy T of this wave for a stage
         const auto copy = [&](auto t, int s, int buf) {
             constexpr int T = decltype(t)::value, pl = T / (WM + WN), x = T % (WM + WN);
-            const unsigned at = lds0 + (unsigned)(buf * STAGE + wave * 1024);
-            if constexpr (x < WM) copy16(base[pl] + (int64_t)s * P.rows * 64, offp[x], at + pl * PB + x * 4096);
-            else copy16(base[2 + pl] + (int64_t)s * Q.rows * 64, offq[x - WM], at + 2 * PB + pl * QB + (x - WM) * 4096);
+            const unsigned at = lds0 + (unsigned)(buf * STAGE + wave * TM * 16);
+            if constexpr (x < WM) copy16(base[pl] + (int64_t)s * P.rows * 64, offp[x], at + pl * PB + x * 1024);
+            else copy16(base[2 + pl] + (int64_t)s * Q.rows * 64, offq[x - WM], at + 2 * PB + pl * QB + (x - WM) * 1024);
         };
         const int n = s1 - s0;
         copies(copy, s0, 0);
@@ -535,7 +529,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     if (EARLY) {
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-            const int x = threadIdx.x + 256 * y, c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
+            const int x = threadIdx.x + 256 * y, c = x / 2 % G::TN, r = x % 2 * 4 + x / (2 * G::TN) * 8;
             const int64_t o = at_panel(c0 + c, r0 + r, orow);  // (64 x 64: nothing reaches over the padding)
             eh[y] = *reinterpret_cast<const f16x4*>(oldh + o);
             el[y] = *reinterpret_cast<const f16x4*>(oldl + o);
@@ -603,7 +597,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     }
     // The tile goes through LDS, [column][row], so that both passes over it touch whole lines of memory: along the rows
     // first, where the old values are added, then across.
-    constexpr int LS = G::TM + 4;  // (float4 along the rows; 16 lanes apart by columns share a bank, never 8)
+    constexpr int LS = G::TM + 8;  // (two float4 of a column, then the next: 8 columns share no bank)
     float* tv = reinterpret_cast<float*>(sm);
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -625,7 +619,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
 #pragma unroll 8
     for (int x0 = 0; x0 < G::TM * G::TN / 4; x0 += 256) {
-        const int x = x0 + threadIdx.x, c = x / 8 % G::TN, r = x % 8 * 4 + x / (8 * G::TN) * 32;
+        const int x = x0 + threadIdx.x, c = x / 2 % G::TN, r = x % 2 * 4 + x / (2 * G::TN) * 8;
         if (r >= nr || c >= nc) continue;
         if (SYM && (r0 + r) / 64 < (c0 + c) / 64) continue;  // (the mirrored block writes it)
         float* at = tv + c * LS + r;
@@ -653,7 +647,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
         f16* acrl = PHASE == NS_APPLY ? p.xt(1 - q.src, 1) : outl;
 #pragma unroll 4
         for (int x = threadIdx.x; x < G::TM * G::TN / 4; x += 256) {
-            const int r = x / 8 % G::TM, c = x % 8 * 4 + x / (8 * G::TM) * 32;
+            const int r = x / 2 % G::TM, c = x % 2 * 4 + x / (2 * G::TM) * 8;
             if (r >= nr || c >= nc) continue;
             if (SYM && (r0 + r) / 64 <= (c0 + c) / 64) continue;
             const float* at = tv + c * LS + r;
@@ -704,7 +698,7 @@ constexpr int NSF_WAVES = 8;
 
 template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_kernel(NsTable t, NsUnits un, NsArgs q) {
     constexpr bool SYM = PHASE <= NS_POLY;
-    constexpr int W = NSF_WAVES, LS = 36, AHEAD = 3;
+    constexpr int W = NSF_WAVES, LS = 40, AHEAD = 3;
     __shared__ __attribute__((aligned(16))) float tv[W][32 * LS];
     const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
@@ -736,7 +730,7 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int stages = (PHASE == NS_GRAM ? e.np : e.mp) / NS_K;
     // each thread's four values of the result: rows r .. r + 3 of column c
-    const int c = (threadIdx.x & 255) >> 3, r = (threadIdx.x & 7) * 4;
+    const int c = (threadIdx.x >> 1) & 31, r = (threadIdx.x & 1) * 4 + (threadIdx.x >> 6 & 3) * 8;
     const bool mine = threadIdx.x < 256;
     const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
     const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
@@ -748,9 +742,9 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
     }
     const float unit = q.unit[e.mat + bat];
 
-    const unsigned off = (lane & 31) * 64 + (lane >> 5) * 16;
-    const char* base[4] = {uniform(P.hi + P.first * 32), uniform(P.lo + P.first * 32), uniform(Q.hi + Q.first * 32),
-                           uniform(Q.lo + Q.first * 32)};
+    const unsigned offp = ((lane & 31) + (lane >> 5) * P.rows) * 16, offq = ((lane & 31) + (lane >> 5) * Q.rows) * 16;
+    const char* base[4] = {uniform(P.hi + P.first * 8), uniform(P.lo + P.first * 8), uniform(Q.hi + Q.first * 8),
+                           uniform(Q.lo + Q.first * 8)};
     const int64_t kp = (int64_t)P.rows * 64, kq = (int64_t)Q.rows * 64;
     f16x8 f[AHEAD][2][4];  // [stage][half][P hi, P lo, Q hi, Q lo]
     const auto fetch = [&](int s, f16x8 (&g)[2][4]) {
@@ -759,7 +753,7 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int y = 0; y < 4; ++y)
-                g[h][y] = *reinterpret_cast<const f16x8*>(base[y] + k * (y < 2 ? kp : kq) + off + 32 * h);
+                g[h][y] = *reinterpret_cast<const f16x8*>(base[y] + k * (y < 2 ? kp : kq) + h * (y < 2 ? kp : kq) / 2 + (y < 2 ? offp : offq));
     };
     f32x16 a0{}, a1{}, a2{};
 #pragma unroll
