@@ -48,6 +48,7 @@ constexpr int NS_PAD = 64;       // X, A, B are padded to it; tiles that reach o
 constexpr int NS_K = 32;         // K values of a stage
 constexpr int NS_STEPS = 64;     // most steps
 constexpr int NS_PART = 512;     // most partial sums of squares per matrix
+constexpr int NS_ROUND = 768;    // tiles up to here are on the card together, or nearly so
 
 struct NsMat {
     const void* x;               // orthogonalize: the matrices; step: gradients
@@ -484,10 +485,12 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     const NsMat& e = t.e[ei];
     const unsigned rel = blockIdx.x - un.first[ei], whole = un.whole[ei], split = un.split[ei], tiles = un.tiles[ei];
     const unsigned cut = tiles * e.batch - whole;
-    // split tiles in part order, and adjacent ones to one XCD: its units then share their K range
+    // Adjacent units to one XCD: split tiles in part order share their K range there, whole tiles their rows (X <- a X + B X
+    // of 512 x 4608 20.3 -> 17.5 us; units in turn give each XCD one column of tiles and all of X).  Where the tiles fill the
+    // card more than once, in turn is better: 372 us against 397 at 4096 x 4096.
     const int over = rel < whole ? -1 : xcd_order(rel - whole, cut * split);
     const int part = over < 0 ? 0 : (unsigned)over / cut;
-    const unsigned tile = over < 0 ? rel : whole + over - part * cut;
+    const unsigned tile = over < 0 ? (whole <= NS_ROUND ? xcd_order(rel, whole) : rel) : whole + over - part * cut;
     const int bat = e.batch == 1 ? 0 : tile / tiles;
     int tl = tile - bat * tiles;
     const Planes p = planes_of(q, e, bat);
@@ -1126,27 +1129,27 @@ int64_t ns_tiles(const NsMat& e, int phase, int edge) {
 }
 int ns_stages(const NsMat& e, int phase) { return (phase == NS_GRAM ? e.np : e.mp) / NS_K; }
 
-// 128 x 128 tiles do the same work with half the LDS reads per MFMA, 64 x 64 tiles spread it over four times the blocks.
-// Measured, us for 64 / 128: X <- a X + B X of 1536 x 1536 (144 tiles of 128) 38 / 43, 1024 x 4096 (256) 51 / 39,
-// 2048 x 2048 (256) 81 / 70; A = X X^T of 4 x 1024 x 1024 (144, K 1024) 31 / 32, 2048 x 2048 (136, K 2048) 52 / 46,
-// 3 x 1536 x 1536 (234) 59 / 55: large tiles from one per CU on, with K of 2048 from one per two CUs.
+// 128 x 128 tiles do the same work with half the LDS reads per MFMA and half the traffic from L2, 64 x 64 tiles spread it
+// over four times the blocks.  us for 64 / 128 of X <- a X + B X (tiles of 128, stages of K): 1024 x 4096 (256, 32) 45 / 39,
+// 4 x 1024 x 1024 (256, 32) 45 / 38, 16 x 256 x 1024 (256, 8) 21 / 21, 768 x 6144 (288, 24) 39 / 41, 4 x 512 x 4608
+// (576, 16) 61 / 52; of X X^T: 4 x 1024 x 1024 (144, 32) 26 / 29, 3 x 1536 x 1536 (234, 48) 54 / 54, 8 x 1024 x 1024
+// (288, 32) 50 / 47, 32 x 512 x 512 (320, 16) 44 / 30.  Large tiles from one per CU on if K is long, else from five per
+// four CUs, counted by the longest: the deep network's weights (310 tiles, worth 258 of the longest) take 26 / 30.
 // 32 x 32 tiles are for launches that are all latency.  us for 32 / 64: A A of 512 x 512 (36 tiles of 64) 6.3 / 8.2,
 // B X of 512 x 512 (64) 7.9 / 9.6, X X^T of 512 x 2048 (36, 64 stages) 11.5 / 12.4 but of 512 x 4608 (144 stages)
 // 20.4 / 16.9, A A of 6 x 333 x 333 (126) 11.3 / 8.2: up to a 64 x 64 tile per four CUs and 64 stages.
 enum NsConfig { NS_TILE64, NS_TILE128, NS_TILE32 };
 NsConfig ns_config(const NsTable& t, int phase) {
-    int64_t n = 0, small = 0, deep = 0;
-    int most = 0;
+    int64_t small = 0, work = 0, most = 0;  // 64 x 64 tiles; stages of all 128 x 128 tiles, and of one
     for (int i = 0; i < t.count; ++i) {
-        const int64_t k = ns_tiles(t.e[i], phase, 128) * t.e[i].batch;
-        const int stages = ns_stages(t.e[i], phase);
-        n += k;
+        const int64_t stages = ns_stages(t.e[i], phase);
         small += ns_tiles(t.e[i], phase, 64) * t.e[i].batch;
+        work += ns_tiles(t.e[i], phase, 128) * t.e[i].batch * stages;
         most = std::max(most, stages);
-        if (stages >= 64) deep += k;
     }
     if (4 * small <= num_cus() && most <= 64) return NS_TILE32;
-    return n >= num_cus() || 2 * deep >= num_cus() ? NS_TILE128 : NS_TILE64;
+    const int64_t each = num_cus() * most;
+    return 4 * work >= 5 * each || (most >= 32 && work >= each) ? NS_TILE128 : NS_TILE64;
 }
 
 struct NsPlan {
