@@ -43,7 +43,7 @@ typedef _Float16 f16;
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int NS_LIST = 24;      // entries per launch (their table is a kernel argument)
+constexpr int NS_LIST = 16;      // entries per launch (their table is the first kernel's argument)
 constexpr int NS_PAD = 64;       // X, A, B are padded to it; tiles that reach over the padding read their last rows again
 constexpr int NS_K = 32;         // K values of a stage
 constexpr int NS_STEPS = 64;     // most steps
@@ -67,16 +67,19 @@ struct NsTable {
     int count, mats;
 };
 
-// Work units of a product launch, per entry: its tiles in order, the first `whole` over all of K, the others in `split`
-// parts each (joined by whichever unit of a tile ends last, in part order).
-struct NsUnits {
-    int first[NS_LIST];          // units of the launch up to each entry; behind the last, more than there are
+// Work units of a launch up to each entry; behind the last, more than there are.
+struct NsFirst {
+    int first[NS_LIST];
+    int count;
+};
+// Those of a product, per entry: its tiles in order, the first `whole` over all of K, the others in `split` parts each
+// (joined by whichever unit of a tile ends last, in part order).
+struct NsUnits : NsFirst {
     int tiles[NS_LIST];          // tiles of one matrix of the entry
     int whole[NS_LIST];          // of the entry's tiles times batch
     int split[NS_LIST];
     int tail[NS_LIST];           // first counter of the entry's split tiles
     int joint[NS_LIST];          // first of their parts' sums
-    int count;
 };
 
 struct NsCoef {
@@ -97,8 +100,25 @@ struct NsArgs {
     float eps;
     float sx, sa;                // S of X (of a matrix that starts near 1) and of A, B
     double growth;               // most that all steps together enlarge a small singular value
-    float a, b, c;               // this step's coefficients
-    int src;                     // which X buffer the step reads
+};
+
+// What all launches of a list need.  The first is given it and leaves it in the workspace: the others' arguments stay short
+// (a launch of 3 KB of arguments costs the host 4.3 us, of 64 bytes 2.8).
+struct NsJob {
+    NsTable t;
+    NsArgs q;
+    NsFirst norm, split;
+    NsUnits product[4];          // by phase
+};
+static_assert(sizeof(NsJob) <= 4096, "a kernel's arguments");
+// (in the constant address space, as arguments are: scalar loads wherever they stand)
+__device__ __forceinline__ const NsJob& job_at(const void* p) {
+    return *(const NsJob*)(const __attribute__((address_space(4))) NsJob*)(uintptr_t)p;
+}
+
+struct NsStep {
+    float a, b, c;
+    int src;                     // which X buffer it reads
 };
 
 // planes of one matrix, in float16 numbers from its workspace: X hi, lo, X^T hi, lo (two buffers), A hi, lo, B hi, lo
@@ -167,10 +187,16 @@ __device__ __forceinline__ float nesterov_u(const NsArgs& q, float g, float m) {
 }
 
 // ---------------------------------------------------------------- u, and the sums of its squares (in float64: no range)
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsTable t, NsUnits un, NsArgs q) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsJob job) {
     __shared__ double red[4];
-    if (blockIdx.x == 0)
+    const NsTable& t = job.t;
+    const NsArgs& q = job.q;
+    const NsFirst& un = job.norm;
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < (int)(sizeof(NsJob) / 4); i += 256)
+            reinterpret_cast<unsigned*>(q.ws)[i] = reinterpret_cast<const unsigned*>(&job)[i];
         for (int i = threadIdx.x; i < q.ndone; i += 256) q.done[i] = 0;
+    }
     const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
     const int bat = (blockIdx.x - un.first[ei]) / e.parts, blk = (blockIdx.x - un.first[ei]) % e.parts;
@@ -225,7 +251,10 @@ __device__ __forceinline__ int ns_scale(double fro, double growth) {
 }
 
 // ---------------------------------------------------------------- X = u S / (|u| + eps) as planes, both ways round
-__global__ __launch_bounds__(256) void ns_split_kernel(NsTable t, NsUnits un, NsArgs q) {
+__global__ __launch_bounds__(256) void ns_split_kernel(const void* job) {
+    const NsTable& t = job_at(job).t;
+    const NsArgs& q = job_at(job).q;
+    const NsFirst& un = job_at(job).split;
     __shared__ float tile[64][65];
     __shared__ double red[4];
     __shared__ double scale_s;
@@ -476,7 +505,10 @@ enum NsPhase { NS_GRAM = 0, NS_POLY = 1, NS_APPLY = 2, NS_LAST = 3 };
 
 // NS_GRAM: A = X X^T.  NS_POLY: B = b A + c A A.  Both symmetric: of each pair of 64-blocks across the diagonal one is
 // computed and written twice.  NS_APPLY: X <- a X + B X, both ways round.  NS_LAST: that to the caller's matrices.
-template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) void ns_product_kernel(NsTable t, NsUnits un, NsArgs q) {
+template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) void ns_product_kernel(const void* job, NsStep st) {
+    const NsTable& t = job_at(job).t;
+    const NsArgs& q = job_at(job).q;
+    const NsUnits& un = job_at(job).product[PHASE];
     using G = Product<WM, WN, NB>;
     constexpr bool SYM = PHASE <= NS_POLY;
     extern __shared__ __attribute__((aligned(16))) char sm[];
@@ -507,8 +539,8 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
         }
         r0 = ti * G::TM;
         c0 = tl * G::TN;
-        const f16* hi = PHASE == NS_GRAM ? p.x(q.src, 0) : p.a(0);
-        const f16* lo = PHASE == NS_GRAM ? p.x(q.src, 1) : p.a(1);
+        const f16* hi = PHASE == NS_GRAM ? p.x(st.src, 0) : p.a(0);
+        const f16* lo = PHASE == NS_GRAM ? p.x(st.src, 1) : p.a(1);
         P = Rows{hi, lo, r0, e.mp};
         Q = Rows{hi, lo, c0, e.mp};
     } else {
@@ -517,14 +549,14 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
         r0 = tr * G::TM;
         c0 = (tl - tr * tc) * G::TN;
         const Rows B{p.b(0), p.b(1), tall ? r0 : c0, e.mp};
-        const Rows X{p.xt(q.src, 0), p.xt(q.src, 1), tall ? c0 : r0, e.np};
+        const Rows X{p.xt(st.src, 0), p.xt(st.src, 1), tall ? c0 : r0, e.np};
         P = tall ? B : X;
         Q = tall ? X : B;
     }
     const int stages = (int)((PHASE == NS_GRAM ? e.np : e.mp) / NS_K);
     // the old values of small tiles are on their way during the product (these are latency, not throughput)
-    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
-    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
+    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(st.src, 0) : p.x(st.src, 0);
+    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(st.src, 1) : p.x(st.src, 1);
     const int orow = tall ? e.np : e.mp;  // rows of the old values' and the output's planes: the product's columns
     const int nr = min(G::TM, (SYM || tall ? e.mp : e.np) - r0), nc = min(G::TN, (SYM ? e.mp : tall ? e.np : e.mp) - c0);
     constexpr bool EARLY = WM * WN == 1 && PHASE != NS_GRAM;
@@ -604,7 +636,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     float* tv = reinterpret_cast<float*>(sm);
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? q.c / q.sa : 1.f / q.sa;
+        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? st.c / q.sa : 1.f / q.sa;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < WM; ++i)
@@ -618,8 +650,8 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
             }
         __syncthreads();
     }
-    f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
-    f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
+    f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - st.src, 0);
+    f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - st.src, 1);
 #pragma unroll 8
     for (int x0 = 0; x0 < G::TM * G::TN / 4; x0 += 256) {
         const int x = x0 + threadIdx.x, c = x / 2 % G::TN, r = x % 2 * 4 + x / (2 * G::TN) * 8;
@@ -632,7 +664,7 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
         if (PHASE != NS_GRAM) {
             const f16x4 oh = EARLY ? eh[EARLY ? x0 / 256 : 0] : *reinterpret_cast<const f16x4*>(oldh + o);
             const f16x4 ol = EARLY ? el[EARLY ? x0 / 256 : 0] : *reinterpret_cast<const f16x4*>(oldl + o);
-            const float f = PHASE == NS_POLY ? q.b : q.a;
+            const float f = PHASE == NS_POLY ? st.b : st.a;
 #pragma unroll
             for (int y = 0; y < 4; ++y) v[y] = fmaf(f, (float)oh[y] + (float)ol[y], v[y]);
         }
@@ -646,8 +678,8 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
     }
     __syncthreads();
     if (PHASE != NS_LAST) {
-        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - q.src, 0) : outh;
-        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - q.src, 1) : outl;
+        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - st.src, 0) : outh;
+        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - st.src, 1) : outl;
 #pragma unroll 4
         for (int x = threadIdx.x; x < G::TM * G::TN / 4; x += 256) {
             const int r = x / 2 % G::TM, c = x % 2 * 4 + x / (2 * G::TM) * 8;
@@ -699,7 +731,10 @@ template <int PHASE, int WM, int WN, int NB> __global__ __launch_bounds__(256) v
 // Four times the blocks of 64 x 64 tiles and a quarter of the epilogue for each, for launches that are all latency.
 constexpr int NSF_WAVES = 8;
 
-template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_kernel(NsTable t, NsUnits un, NsArgs q) {
+template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_kernel(const void* job, NsStep st) {
+    const NsTable& t = job_at(job).t;
+    const NsArgs& q = job_at(job).q;
+    const NsUnits& un = job_at(job).product[PHASE];
     constexpr bool SYM = PHASE <= NS_POLY;
     constexpr int W = NSF_WAVES, LS = 40, AHEAD = 3;
     __shared__ __attribute__((aligned(16))) float tv[W][32 * LS];
@@ -717,8 +752,8 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
         for (; tl > ti; ++ti) tl -= ti + 1;
         r0 = ti * 32;
         c0 = tl * 32;
-        const f16* hi = PHASE == NS_GRAM ? p.x(q.src, 0) : p.a(0);
-        const f16* lo = PHASE == NS_GRAM ? p.x(q.src, 1) : p.a(1);
+        const f16* hi = PHASE == NS_GRAM ? p.x(st.src, 0) : p.a(0);
+        const f16* lo = PHASE == NS_GRAM ? p.x(st.src, 1) : p.a(1);
         P = Rows{hi, lo, r0, e.mp};
         Q = Rows{hi, lo, c0, e.mp};
     } else {
@@ -726,7 +761,7 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
         r0 = tr * 32;
         c0 = (tl - tr * tc) * 32;
         const Rows B{p.b(0), p.b(1), tall ? r0 : c0, e.mp};
-        const Rows X{p.xt(q.src, 0), p.xt(q.src, 1), tall ? c0 : r0, e.np};
+        const Rows X{p.xt(st.src, 0), p.xt(st.src, 1), tall ? c0 : r0, e.np};
         P = tall ? B : X;
         Q = tall ? X : B;
     }
@@ -735,8 +770,8 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
     // each thread's four values of the result: rows r .. r + 3 of column c
     const int c = (threadIdx.x >> 1) & 31, r = (threadIdx.x & 1) * 4 + (threadIdx.x >> 6 & 3) * 8;
     const bool mine = threadIdx.x < 256;
-    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(q.src, 0) : p.x(q.src, 0);
-    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(q.src, 1) : p.x(q.src, 1);
+    const f16* oldh = PHASE == NS_POLY ? p.a(0) : tall ? p.xt(st.src, 0) : p.x(st.src, 0);
+    const f16* oldl = PHASE == NS_POLY ? p.a(1) : tall ? p.xt(st.src, 1) : p.x(st.src, 1);
     const int64_t o = at_panel(c0 + c, r0 + r, tall ? e.np : e.mp);
     f16x4 oh{}, ol{};
     if (PHASE != NS_GRAM) {
@@ -791,14 +826,14 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
             v[2] += x.z;
             v[3] += x.w;
         }
-        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? q.c / q.sa : 1.f / q.sa;
-        const float fo = PHASE == NS_POLY ? q.b : q.a;
+        const float k = PHASE == NS_GRAM ? q.sa * unit * unit : PHASE == NS_POLY ? st.c / q.sa : 1.f / q.sa;
+        const float fo = PHASE == NS_POLY ? st.b : st.a;
 #pragma unroll
         for (int y = 0; y < 4; ++y) v[y] = PHASE == NS_GRAM ? v[y] * k : fmaf(fo, (float)oh[y] + (float)ol[y], v[y] * k);
     }
     if (PHASE != NS_LAST) {
-        f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - q.src, 0);
-        f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - q.src, 1);
+        f16* outh = PHASE == NS_GRAM ? p.a(0) : PHASE == NS_POLY ? p.b(0) : p.x(1 - st.src, 0);
+        f16* outl = PHASE == NS_GRAM ? p.a(1) : PHASE == NS_POLY ? p.b(1) : p.x(1 - st.src, 1);
         f16x4 h, l;
         split4(v, h, l);
         if (mine) {
@@ -810,8 +845,8 @@ template <int PHASE> __global__ __launch_bounds__(64 * NSF_WAVES) void ns_few_ke
         if (mine) st4(&tv[0][c * LS + r], make_float4(v[0], v[1], v[2], v[3]));
         __syncthreads();
         if (!mine) return;
-        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - q.src, 0) : outh;
-        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - q.src, 1) : outl;
+        f16* acrh = PHASE == NS_APPLY ? p.xt(1 - st.src, 0) : outh;
+        f16* acrl = PHASE == NS_APPLY ? p.xt(1 - st.src, 1) : outl;
         const float w[4] = {tv[0][r * LS + c], tv[0][(r + 1) * LS + c], tv[0][(r + 2) * LS + c], tv[0][(r + 3) * LS + c]};
         split4(w, h, l);
         const int64_t oa = at_panel(r0 + c, c0 + r, PHASE == NS_APPLY ? e.np : e.mp);
@@ -918,7 +953,7 @@ __device__ __forceinline__ void put_across(f16* pl, int d, int rows, int r0, int
     }
 }
 
-template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kernel(NsTable t, NsUnits un, NsArgs q, NsCoef coef) {
+template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kernel(NsTable t, NsFirst un, NsArgs q, NsCoef coef) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     __shared__ double red[NSB_WAVES + 2];
     const int ei = find_entry(un.first, un.count, blockIdx.x);
@@ -1204,7 +1239,7 @@ NsPlan ns_plan(const NsTable& t, int phase) {
 }
 
 // Units of the passes over values: `per` blocks to a matrix of an entry.
-template <typename F> unsigned ns_blocks(const NsTable& t, NsUnits& un, F per) {
+template <typename F> unsigned ns_blocks(const NsTable& t, NsFirst& un, F per) {
     int64_t n = 0;
     un.count = t.count;
     for (int i = 0; i < t.count; ++i) {
@@ -1239,7 +1274,7 @@ bool ns_in_blocks(const NsTable& t, int* bytes, int* pairs) {
     return true;
 }
 
-// One launch table's workspace: partial sums and unit of every matrix, counters and partial products of split tiles,
+// One launch table's workspace: the job, partial sums and unit of every matrix, counters and partial products of split tiles,
 // then the planes.  Fills in the places; returns its size.
 int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
     int64_t mats = 0, counters = 0, joint = 0;
@@ -1262,6 +1297,7 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
         return reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(ws) + (uintptr_t)at);
     };
     q.ws = static_cast<char*>(ws);
+    take(sizeof(NsJob));
     q.ndone = (int)counters;
     char* a = take(mats * NS_PART * (int64_t)sizeof(double));
     char* b = take(mats * (int64_t)sizeof(float));
@@ -1278,23 +1314,23 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
     return off;
 }
 
-template <int PHASE, int WM, int WN, int NB> int ns_product_as(const NsTable& t, const NsPlan& p, const NsArgs& q, hipStream_t s) {
+template <int PHASE, int WM, int WN, int NB> int ns_product_as(const NsPlan& p, const void* job, const NsStep& st, hipStream_t s) {
     constexpr int sm = Product<WM, WN, NB>::LDS;
     if (sm > 64 * 1024)
         (void)hipFuncSetAttribute((const void*)ns_product_kernel<PHASE, WM, WN, NB>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-    ns_product_kernel<PHASE, WM, WN, NB><<<p.blocks, 256, sm, s>>>(t, p.un, q);
+    ns_product_kernel<PHASE, WM, WN, NB><<<p.blocks, 256, sm, s>>>(job, st);
     PCX_LAUNCH_CHECK("ns_product_kernel");
     return PCX_OK;
 }
-template <int PHASE> int ns_product(const NsTable& t, const NsArgs& q, hipStream_t s) {
-    const NsPlan p = ns_plan(t, PHASE);
+template <int PHASE> int ns_product(const NsPlan* plans, const void* job, const NsStep& st, hipStream_t s) {
+    const NsPlan& p = plans[PHASE];
     if (p.cfg == NS_TILE32) {
-        ns_few_kernel<PHASE><<<p.blocks, 64 * NSF_WAVES, 0, s>>>(t, p.un, q);
+        ns_few_kernel<PHASE><<<p.blocks, 64 * NSF_WAVES, 0, s>>>(job, st);
         PCX_LAUNCH_CHECK("ns_few_kernel");
         return PCX_OK;
     }
-    if (p.cfg == NS_TILE64) return ns_product_as<PHASE, 1, 1, 3>(t, p, q, s);
-    return ns_product_as<PHASE, 2, 2, 2>(t, p, q, s);
+    if (p.cfg == NS_TILE64) return ns_product_as<PHASE, 1, 1, 3>(p, job, st, s);
+    return ns_product_as<PHASE, 2, 2, 2>(p, job, st, s);
 }
 
 int ns_scales(NsArgs& q, const float* coef, int steps) {
@@ -1307,7 +1343,7 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
     return PCX_OK;
 }
 
-template <int T> int ns_block_as(const NsTable& t, const NsUnits& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
+template <int T> int ns_block_as(const NsTable& t, const NsFirst& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
     if (sm > 64 * 1024)
         (void)hipFuncSetAttribute((const void*)ns_block_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
     ns_block_kernel<T><<<n, 64 * NSB_WAVES, sm, s>>>(t, un, q, c);
@@ -1315,31 +1351,34 @@ template <int T> int ns_block_as(const NsTable& t, const NsUnits& un, const NsAr
     return PCX_OK;
 }
 
-int ns_run(const NsTable& t, NsArgs q, const float* coef, int steps, hipStream_t s) {
-    NsUnits un{};
+int ns_run(const NsTable& t, const NsArgs& q, const float* coef, int steps, hipStream_t s) {
     int most, pairs;
     if (ns_in_blocks(t, &most, &pairs)) {
         NsCoef c{};
         c.steps = steps;
         memcpy(c.c, coef, 3 * steps * sizeof(float));
+        NsFirst un{};
         const unsigned n = ns_blocks(t, un, [](const NsMat&) { return (int64_t)1; });
         if (pairs <= NSB_WAVES) return ns_block_as<2>(t, un, q, c, n, most, s);
         return ns_block_as<4>(t, un, q, c, n, most, s);
     }
-    unsigned n = ns_blocks(t, un, [](const NsMat& e) { return (int64_t)e.parts; });
-    ns_norm_kernel<<<n, 256, 0, s>>>(t, un, q);
+    NsJob job{t, q, {}, {}, {}};
+    NsPlan plans[4];
+    for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
+        plans[ph] = ns_plan(t, ph);
+        job.product[ph] = plans[ph].un;
+    }
+    const unsigned nn = ns_blocks(t, job.norm, [](const NsMat& e) { return (int64_t)e.parts; });
+    const unsigned ns = ns_blocks(t, job.split, [](const NsMat& e) { return (int64_t)(e.mp / 64) * (e.np / 64); });
+    ns_norm_kernel<<<nn, 256, 0, s>>>(job);
     PCX_LAUNCH_CHECK("ns_norm_kernel");
-    n = ns_blocks(t, un, [](const NsMat& e) { return (int64_t)(e.mp / 64) * (e.np / 64); });
-    ns_split_kernel<<<n, 256, 0, s>>>(t, un, q);
+    ns_split_kernel<<<ns, 256, 0, s>>>(q.ws);
     PCX_LAUNCH_CHECK("ns_split_kernel");
     for (int k = 0; k < steps; ++k) {
-        q.a = coef[3 * k];
-        q.b = coef[3 * k + 1];
-        q.c = coef[3 * k + 2];
-        q.src = k & 1;
-        int rc = ns_product<NS_GRAM>(t, q, s);
-        if (!rc) rc = ns_product<NS_POLY>(t, q, s);
-        if (!rc) rc = k + 1 < steps ? ns_product<NS_APPLY>(t, q, s) : ns_product<NS_LAST>(t, q, s);
+        const NsStep st{coef[3 * k], coef[3 * k + 1], coef[3 * k + 2], k & 1};
+        int rc = ns_product<NS_GRAM>(plans, q.ws, st, s);
+        if (!rc) rc = ns_product<NS_POLY>(plans, q.ws, st, s);
+        if (!rc) rc = k + 1 < steps ? ns_product<NS_APPLY>(plans, q.ws, st, s) : ns_product<NS_LAST>(plans, q.ws, st, s);
         if (rc) return rc;
     }
     return PCX_OK;
