@@ -51,8 +51,10 @@ struct LnArgs {
     void* db;
 };
 
+// V values that lie anywhere: rows of an odd length, slices, and strides that are no multiple of 16 bytes take the same
+// 16-byte loads and stores as aligned ones.
 template <typename T, int V> struct Pack {
-    typedef T type __attribute__((ext_vector_type(V)));
+    typedef T type __attribute__((ext_vector_type(V), aligned(alignof(T))));
 };
 template <typename T> struct Pack<T, 1> {
     typedef T type;
@@ -77,14 +79,10 @@ template <int V, typename T> __device__ __forceinline__ void load_v(const T* p, 
     for (int k = 0; k < V / N; ++k) widen<T, N>(load_raw<N>(p + k * N), v + k * N);
 }
 template <int V, typename T> __device__ __forceinline__ void store_v(T* p, const float* v) {
-    if constexpr (V == 1) {
-        p[0] = (T)v[0];
-    } else {
-        pack<T, V> t;
+    pack<T, V> t;
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[j] = (T)v[j];
-        *reinterpret_cast<pack<T, V>*>(p) = t;
-    }
+    for (int j = 0; j < V; ++j) t[j] = (T)v[j];
+    *reinterpret_cast<pack<T, V>*>(p) = t;
 }
 // V weights; without any the pointer is some readable row of the same length, and the values are not used
 template <int V, typename W> __device__ __forceinline__ void load_w(const void* w, bool has, int d, float* v, float none) {
@@ -92,6 +90,20 @@ template <int V, typename W> __device__ __forceinline__ void load_w(const void* 
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = has ? v[j] : none;
 }
+
+// A lane's V values of a row of D in chunk c.  Where the row ends inside them they are its last V instead: the first `skip`
+// belong to the lane before, which does the same with them and stores the same, so only the row's sums leave them out.
+template <int V> struct Place {
+    int d, skip;   // first column, values that are another lane's (all of them behind the row's end)
+    bool whole;    // nobody skips any: the same for all lanes
+    __device__ __forceinline__ Place(int lane, int tpr, int c, int D) {
+        const int at = (lane + c * tpr) * V;
+        whole = (c + 1) * tpr * V <= D;
+        d = whole ? at : min(at, D - V);
+        skip = whole ? 0 : at - d;
+    }
+    __device__ __forceinline__ bool here() const { return whole || skip < V; }
+};
 
 // a block's sum of column d (pass 0: dw, 1: db)
 template <typename T> __device__ __forceinline__ void put_column(const LnArgs& a, int pass, int d, float v) {
@@ -135,7 +147,7 @@ template <bool BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[
 template <typename T, int V, int E, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
-    constexpr bool KEEP = E <= (V > 1 ? 16 : 8), AHEAD = KEEP;  // (what the registers of 1024 threads hold)
+    constexpr bool KEEP = E <= 16, AHEAD = KEEP;  // (what the registers of 1024 threads hold)
     __shared__ float red[2][1][16];
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
     const int lane = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (unsigned)(tpr - 1));
@@ -143,24 +155,19 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
     const float invd = 1.f / (float)a.D;
     float w[KEEP ? NC : 1][V], b[KEEP ? NC : 1][V];
     const auto weights = [&](int c, float* wv, float* bv) {
-        const int d = (lane + c * tpr) * V;
-        if (d < a.D) {
-            if (a.wf32) {
-                load_w<V, float>(a.w, a.hw, d, wv, 1.f);
-                load_w<V, float>(a.b, a.hb, d, bv, 0.f);
-            } else {
-                load_w<V, T>(a.w, a.hw, d, wv, 1.f);
-                load_w<V, T>(a.b, a.hb, d, bv, 0.f);
-            }
+        const int d = Place<V>(lane, tpr, c, a.D).d;
+        if (a.wf32) {
+            load_w<V, float>(a.w, a.hw, d, wv, 1.f);
+            load_w<V, float>(a.b, a.hb, d, bv, 0.f);
+        } else {
+            load_w<V, T>(a.w, a.hw, d, wv, 1.f);
+            load_w<V, T>(a.b, a.hb, d, bv, 0.f);
         }
     };
     const auto fetch = [&](int64_t r, pack<T, V> (&raw)[NC]) {
         const T* x = static_cast<const T*>(a.x) + (r < a.rows ? r : 0) * a.xs;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int d = (lane + c * tpr) * V;
-            if (d < a.D) raw[c] = load_raw<V>(x + d);
-        }
+        for (int c = 0; c < NC; ++c) raw[c] = load_raw<V>(x + Place<V>(lane, tpr, c, a.D).d);
     };
     int64_t r = (int64_t)blockIdx.x * rpb + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
     pack<T, V> next[NC];
@@ -174,29 +181,33 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
         float s[1] = {0.f};
         if constexpr (!AHEAD) fetch(r, next);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if ((lane + c * tpr) * V < a.D) widen<T, V>(next[c], v[c]);
-            else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[c][j] = 0.f;
-            }
-        }
+        for (int c = 0; c < NC; ++c) widen<T, V>(next[c], v[c]);
         if (AHEAD && r0 + stride < a.rows) fetch(r + stride, next);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) {
+            const Place<V> at(lane, tpr, c, a.D);
+            if (at.whole) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) s[0] += v[c][j];
+                for (int j = 0; j < V; ++j) s[0] += v[c][j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[0] += j >= at.skip ? v[c][j] : 0.f;
+            }
+        }
         row_sum<BLOCK, 1>(s, tpr, red[0]);
         const float mean = s[0] * invd;
         s[0] = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            if ((lane + c * tpr) * V < a.D) {
+            const Place<V> at(lane, tpr, c, a.D);
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    v[c][j] -= mean;
-                    s[0] = fmaf(v[c][j], v[c][j], s[0]);
-                }
+            for (int j = 0; j < V; ++j) v[c][j] -= mean;
+            if (at.whole) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[0] = fmaf(v[c][j], v[c][j], s[0]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[0] += j >= at.skip ? v[c][j] * v[c][j] : 0.f;
             }
         }
         row_sum<BLOCK, 1>(s, tpr, red[1]);
@@ -205,13 +216,12 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
         T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d = (lane + c * tpr) * V, k = KEEP ? c : 0;
-            if (d < a.D) {
-                if constexpr (!KEEP) weights(c, w[0], b[0]);
+            const int k = KEEP ? c : 0;
+            if constexpr (!KEEP) weights(c, w[0], b[0]);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[k][j], b[k][j]);
-                store_v<V>(y + d, v[c]);
-            }
+            for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[k][j], b[k][j]);
+            const Place<V> at(lane, tpr, c, a.D);
+            if (at.here()) store_v<V>(y + at.d, v[c]);
             if constexpr (!KEEP)  // (few weights in flight, or the registers spill)
                 if (c % 4 == 3) asm volatile("" ::: "memory");
         }
@@ -222,7 +232,8 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
 template <typename T, int V, int E, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
-    constexpr bool AHEAD = E <= 8 || sizeof(T) == 2;  // (16 float32 values a thread leave no registers for the next row)
+    constexpr bool AHEAD = E <= 8 || sizeof(T) == 2;  // (16 float32 values a thread leave no registers for the next row,
+    constexpr bool KEEP = E <= 8 || (AHEAD && !BLOCK);  // of 16 bits none for the weights in blocks of 1024 threads)
     __shared__ float red[2][2][16];
     extern __shared__ __attribute__((aligned(16))) float cols[];  // sub-wave rows: [4 waves][D] of dw, then of db
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
@@ -239,29 +250,23 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
         nst = a.stat[q];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d = (lane + c * tpr) * V;
-            if (d < a.D) {
-                nx[c] = load_raw<V>(x + d);
-                ng[c] = load_raw<V>(dy + d);
-            }
+            const int d = Place<V>(lane, tpr, c, a.D).d;
+            nx[c] = load_raw<V>(x + d);
+            ng[c] = load_raw<V>(dy + d);
         }
     };
     if constexpr (AHEAD) fetch(r);
-    float sw[NC][V], sb[NC][V], w[AHEAD ? NC : 1][V];
+    float sw[NC][V], sb[NC][V], w[KEEP ? NC : 1][V];
     const auto weight = [&](int c, float* wv) {
-        const int d = (lane + c * tpr) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) wv[j] = 0.f;
-        if (d < a.D) {
-            if (a.wf32) load_w<V, float>(a.w, a.hw, d, wv, 1.f);
-            else load_w<V, T>(a.w, a.hw, d, wv, 1.f);
-        }
+        const int d = Place<V>(lane, tpr, c, a.D).d;
+        if (a.wf32) load_w<V, float>(a.w, a.hw, d, wv, 1.f);
+        else load_w<V, T>(a.w, a.hw, d, wv, 1.f);
     };
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
         for (int j = 0; j < V; ++j) sw[c][j] = sb[c][j] = 0.f;
-        if constexpr (AHEAD) weight(c, w[c]);
+        if constexpr (KEEP) weight(c, w[c]);
     }
     int par = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += stride, r += stride) {
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
         float xh[NC][V], g[NC][V];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            if (on && (lane + c * tpr) * V < a.D) {
+            if (on) {
                 widen<T, V>(nx[c], xh[c]);
                 widen<T, V>(ng[c], g[c]);
             } else {
@@ -286,16 +291,28 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int k = AHEAD ? c : 0;
-            if constexpr (!AHEAD) weight(c, w[0]);
+            const int k = KEEP ? c : 0;
+            if constexpr (!KEEP) weight(c, w[0]);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 xh[c][j] = (xh[c][j] - st.x) * st.y;
                 sb[c][j] += g[c][j];
                 sw[c][j] = fmaf(g[c][j], xh[c][j], sw[c][j]);
                 g[c][j] *= w[k][j];
-                s[0] += g[c][j];
-                s[1] = fmaf(g[c][j], xh[c][j], s[1]);
+            }
+            const Place<V> at(lane, tpr, c, a.D);
+            if (at.whole) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    s[0] += g[c][j];
+                    s[1] = fmaf(g[c][j], xh[c][j], s[1]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    s[0] += j >= at.skip ? g[c][j] : 0.f;
+                    s[1] += j >= at.skip ? g[c][j] * xh[c][j] : 0.f;
+                }
             }
         }
         if (!a.dx) continue;  // (the same for the whole grid)
@@ -306,24 +323,22 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
         T* dx = static_cast<T*>(a.dx) + r * a.D;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d = (lane + c * tpr) * V;
-            if (d < a.D) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[c][j] = st.y * (g[c][j] - fmaf(xh[c][j], c2, c1));
-                store_v<V>(dx + d, g[c]);
-            }
+            for (int j = 0; j < V; ++j) g[c][j] = st.y * (g[c][j] - fmaf(xh[c][j], c2, c1));
+            const Place<V> at(lane, tpr, c, a.D);
+            if (at.here()) store_v<V>(dx + at.d, g[c]);
         }
     }
     if (!a.cols) return;
     if constexpr (BLOCK) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d = (lane + c * tpr) * V;
-            if (d < a.D) {
+            const Place<V> at(lane, tpr, c, a.D);
+            if (at.here()) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    put_column<T>(a, 0, d + j, sw[c][j]);
-                    put_column<T>(a, 1, d + j, sb[c][j]);
+                    put_column<T>(a, 0, at.d + j, sw[c][j]);
+                    put_column<T>(a, 1, at.d + j, sb[c][j]);
                 }
             }
         }
@@ -334,12 +349,12 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
         for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const int d = (lane + c * tpr) * V;
+                const Place<V> at(lane, tpr, c, a.D);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float t = pass ? sb[c][j] : sw[c][j];
                     for (int o = tpr; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
-                    if ((threadIdx.x & 63) < (unsigned)tpr && d < a.D) cw[d + j] = t;
+                    if ((threadIdx.x & 63) < (unsigned)tpr && at.here()) cw[at.d + j] = t;
                 }
             }
             __syncthreads();
@@ -407,42 +422,8 @@ template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow
     }
 }
 
-// Rows that no block holds in registers (behind 8192 values without 16-byte loads, behind 16384 in the backward): read
-// again for each sum, from L2, where a row stays meanwhile.
-template <typename T> __global__ __launch_bounds__(1024) void ln_long_fwd_kernel(LnArgs a) {
-    __shared__ float red[2][1][16];
-    const float invd = 1.f / (float)a.D;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* x = static_cast<const T*>(a.x) + r * a.xs;
-        float s[1] = {0.f};
-#pragma unroll 8
-        for (int d = threadIdx.x; d < a.D; d += 1024) s[0] += (float)x[d];
-        row_sum<true, 1>(s, 1024, red[0]);
-        const float mean = s[0] * invd;
-        s[0] = 0.f;
-#pragma unroll 8
-        for (int d = threadIdx.x; d < a.D; d += 1024) {
-            const float u = (float)x[d] - mean;
-            s[0] = fmaf(u, u, s[0]);
-        }
-        row_sum<true, 1>(s, 1024, red[1]);
-        const float rstd = 1.f / sqrtf(fmaf(s[0], invd, a.eps));
-        T* y = static_cast<T*>(a.y) + r * a.D;
-        const auto finish = [&](auto kind) {
-            using W = decltype(kind);
-#pragma unroll 4
-            for (int d = threadIdx.x; d < a.D; d += 1024) {
-                float w[1], b[1];
-                load_w<1, W>(a.w, a.hw, d, w, 1.f);
-                load_w<1, W>(a.b, a.hb, d, b, 0.f);
-                y[d] = (T)fmaf(((float)x[d] - mean) * rstd, w[0], b[0]);
-            }
-        };
-        if (a.wf32) finish(float());
-        else finish(T());
-        if (a.stat && threadIdx.x == 0) a.stat[r] = make_float2(mean, rstd);
-    }
-}
+// The backward of rows that no block holds in registers (behind 16384 values): read again for each sum, from L2, where a
+// row stays meanwhile.
 template <typename T> __global__ __launch_bounds__(1024) void ln_long_bwd_kernel(LnArgs a) {
     __shared__ float red[2][2][16];
     const float invd = 1.f / (float)a.D;
@@ -521,29 +502,31 @@ struct LnPick {
     bool block;     // a block per row (tpr threads), else rows within waves
 };
 
-// Rows within a wave up to 64 lanes of 8 values (16 with 16-byte loads); behind that a block per row, of as many waves as
-// leave 8 values to a thread while that is up to 512 threads (1024 of single loads), 16 up to 1024, then 32.
-LnPick ln_pick(int D, int V) {
+// Rows within a wave up to 64 lanes of 16 values; behind that a block per row, of as many waves as leave 8 values to a
+// thread while that is up to 1024 threads, 16 up to 1024, then 32.  The forward in 16 bits goes on with 16 values behind 512
+// threads, fewer waves to meet: 16384 rows of 5120 bfloat16 values 64 us, 69 with 8 a thread; its backward has no registers
+// to keep twice the sums and the next row: 163 us with 16, 105 with 8 (float32 alike: 4100 values 318 and 158).
+LnPick ln_pick(int D, int V, bool bwd) {
     if (D <= 64 * V) {
         LnPick p{64, V, false};
         while (p.tpr > 1 && (p.tpr / 2) * V >= D) p.tpr /= 2;
         return p;
     }
-    for (int e = 8; e <= (V > 1 ? 16 : 8); e *= 2)
+    for (int e = 8; e <= 16; e *= 2)
         if (e >= V && D <= 64 * e) return {64, e, false};
     const auto threads = [&](int e) { return ((D + e - 1) / e + 63) / 64 * 64; };
-    if (threads(8) <= (V > 1 ? 512 : 1024)) return {threads(8), 8, true};
+    if (threads(8) <= (V > 4 && !bwd ? 512 : 1024)) return {threads(8), 8, true};
     if (threads(16) <= 1024) return {threads(16), 16, true};
     return {threads(32), 32, true};
 }
 
-int64_t ln_rows_per_block(int D, int V) {
+int64_t ln_rows_per_block(int D, int V, bool bwd) {
     if (D <= LN_NARROW) {
         int tpr = 1;
         while (tpr < D) tpr *= 2;
         return 256 / tpr;
     }
-    const LnPick p = ln_pick(D, V);
+    const LnPick p = ln_pick(D, V, bwd);
     return p.block ? 1 : 256 / p.tpr;
 }
 
@@ -556,13 +539,13 @@ int ln_even(int64_t passes, int64_t most) {
 // The forward keeps 1536 threads of a CU busy.  The backward's partial sums are 8 D bytes per block, written and read
 // once, next to the rows' own 3 tensors: 1024 threads a CU, and no block with fewer than 8 passes.
 int ln_fwd_blocks(int64_t rows, int D, int V) {
-    const int64_t rpb = ln_rows_per_block(D, V), passes = (rows + rpb - 1) / rpb;
-    const int threads = D > LN_NARROW && ln_pick(D, V).block ? ln_pick(D, V).tpr : 256;
+    const int64_t rpb = ln_rows_per_block(D, V, false), passes = (rows + rpb - 1) / rpb;
+    const int threads = D > LN_NARROW && ln_pick(D, V, false).block ? ln_pick(D, V, false).tpr : 256;
     return ln_even(passes, (int64_t)num_cus() * std::max(1, 1536 / threads));
 }
 int ln_bwd_blocks(int64_t rows, int D, int V) {
-    const int64_t rpb = ln_rows_per_block(D, V), passes = (rows + rpb - 1) / rpb;
-    const int threads = D > LN_NARROW && ln_pick(D, V).block ? ln_pick(D, V).tpr : 256;
+    const int64_t rpb = ln_rows_per_block(D, V, true), passes = (rows + rpb - 1) / rpb;
+    const int threads = D > LN_NARROW && ln_pick(D, V, true).block ? ln_pick(D, V, true).tpr : 256;
     const int64_t most = std::min<int64_t>((int64_t)num_cus() * std::max(1, 1024 / threads), (passes + 7) / 8);
     return ln_even(passes, std::max<int64_t>(1, std::min<int64_t>(512, most)));
 }
@@ -580,70 +563,53 @@ template <typename T, int V, int E, bool BLOCK, bool BWD> int ln_go(const LnArgs
     return PCX_OK;
 }
 
-template <typename T, bool BWD> int ln_long(const LnArgs& a, int blocks, hipStream_t s) {
-    if constexpr (BWD) {
-        if (a.cols) {
-            const int64_t slab = (a.rows + blocks - 1) / blocks;
-            ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
-            PCX_LAUNCH_CHECK("ln_long_cols_kernel");
-        }
-        if (!a.dx) return PCX_OK;
-        ln_long_bwd_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a);
-        PCX_LAUNCH_CHECK("ln_long_bwd_kernel");
-    } else {
-        ln_long_fwd_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a);
-        PCX_LAUNCH_CHECK("ln_long_fwd_kernel");
+template <typename T> int ln_long_bwd(const LnArgs& a, int blocks, hipStream_t s) {
+    if (a.cols) {
+        const int64_t slab = (a.rows + blocks - 1) / blocks;
+        ln_long_cols_kernel<T><<<dim3((unsigned)ceil_div(a.D, 256), (unsigned)blocks), 256, 0, s>>>(a, slab);
+        PCX_LAUNCH_CHECK("ln_long_cols_kernel");
     }
+    if (!a.dx) return PCX_OK;
+    ln_long_bwd_kernel<T><<<(unsigned)std::min<int64_t>(a.rows, 1 << 20), 1024, 0, s>>>(a);
+    PCX_LAUNCH_CHECK("ln_long_bwd_kernel");
     return PCX_OK;
 }
 
-template <typename T, int V, bool BWD> int ln_dispatch(LnArgs a, int blocks, hipStream_t s) {
-    const LnPick p = ln_pick(a.D, V);
+template <typename T, bool BWD> int ln_run(LnArgs a, int blocks, hipStream_t s) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (a.D <= LN_NARROW) {
+        a.tpr = 1;
+        while (a.tpr < a.D) a.tpr *= 2;
+        ln_narrow_kernel<T, BWD><<<blocks, 256, 0, s>>>(a);
+        PCX_LAUNCH_CHECK("ln_narrow_kernel");
+        return PCX_OK;
+    }
+    const LnPick p = ln_pick(a.D, V, BWD);
     a.tpr = p.tpr;
     if (!p.block) {
         if (p.ept == V) return ln_go<T, V, V, false, BWD>(a, blocks, s);
         if constexpr (V < 8)
             if (p.ept == 8) return ln_go<T, V, 8, false, BWD>(a, blocks, s);
-        if constexpr (V > 1) return ln_go<T, V, 16, false, BWD>(a, blocks, s);
+        return ln_go<T, V, 16, false, BWD>(a, blocks, s);
     }
     if (p.ept == 8) return ln_go<T, V, 8, true, BWD>(a, blocks, s);
-    if constexpr (V > 1) {
-        if (p.ept == 16) return ln_go<T, V, 16, true, BWD>(a, blocks, s);
-        if constexpr (!BWD) return ln_go<T, V, 32, true, false>(a, blocks, s);
-    }
-    return ln_long<T, BWD>(a, blocks, s);
+    if (p.ept == 16) return ln_go<T, V, 16, true, BWD>(a, blocks, s);
+    if constexpr (BWD) return ln_long_bwd<T>(a, blocks, s);
+    else return ln_go<T, V, 32, true, false>(a, blocks, s);
 }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-// 16-byte loads and stores of a row need rows, weights and strides on 16-byte boundaries
-template <typename T> int ln_run(LnArgs a, bool bwd, int blocks1, int blocksv, hipStream_t s) {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (a.D <= LN_NARROW) {
-        a.tpr = 1;
-        while (a.tpr < a.D) a.tpr *= 2;
-        if (bwd) ln_narrow_kernel<T, true><<<blocks1, 256, 0, s>>>(a);
-        else ln_narrow_kernel<T, false><<<blocks1, 256, 0, s>>>(a);
-        PCX_LAUNCH_CHECK("ln_narrow_kernel");
-        return PCX_OK;
-    }
-    if (blocksv) return bwd ? ln_dispatch<T, V, true>(a, blocksv, s) : ln_dispatch<T, V, false>(a, blocksv, s);
-    return bwd ? ln_dispatch<T, 1, true>(a, blocks1, s) : ln_dispatch<T, 1, false>(a, blocks1, s);
+template <bool BWD> int ln_any(const LnArgs& a, int dtype, int blocks, hipStream_t s) {
+    if (dtype == PCX_F32) return ln_run<float, BWD>(a, blocks, s);
+    if (dtype == PCX_BF16) return ln_run<bf16, BWD>(a, blocks, s);
+    return ln_run<f16, BWD>(a, blocks, s);
 }
 
 int ln_dtype_size(int dtype) { return dtype == PCX_F32 ? 4 : dtype == PCX_BF16 || dtype == PCX_F16 ? 2 : 0; }
-
-bool ln_vectors(const LnArgs& a, int es) {
-    const int V = 16 / es;
-    return a.D > LN_NARROW && a.D % V == 0 && a.xs % V == 0 && a.dys % V == 0 && aligned16(a.x) && aligned16(a.y) &&
-           aligned16(a.dy) && aligned16(a.dx) && aligned16(a.w) && aligned16(a.b);
-}
 
 }  // namespace
 
 size_t layernorm_bwd_ws(int64_t rows, int D, int es) {
     if (rows <= 0 || D <= 0) return 0;
-    const int n = std::max(ln_bwd_blocks(rows, D, 1), ln_bwd_blocks(rows, D, 16 / es));
+    const int n = ln_bwd_blocks(rows, D, 16 / es);
     return n > 1 || D > LN_ALONE ? (size_t)n * 2 * D * sizeof(float) : 0;
 }
 
@@ -669,12 +635,7 @@ LnArgs ln_args(const LayerNormArgs& q) {
 
 int launch_layernorm_fwd(const LayerNormArgs& q, hipStream_t s) {
     const LnArgs a = ln_args(q);
-    const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
-    const int blocks = ln_fwd_blocks(a.rows, a.D, V);
-    const int bv = V > 1 ? blocks : 0;
-    if (q.dtype == PCX_F32) return ln_run<float>(a, false, blocks, bv, s);
-    if (q.dtype == PCX_BF16) return ln_run<bf16>(a, false, blocks, bv, s);
-    return ln_run<f16>(a, false, blocks, bv, s);
+    return ln_any<false>(a, q.dtype, ln_fwd_blocks(a.rows, a.D, 16 / ln_dtype_size(q.dtype)), s);
 }
 
 int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s) {
@@ -683,13 +644,9 @@ int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s) {
     a.dw = q.dw;
     a.db = q.db;
     a.cf32 = q.wdtype == PCX_F32;
-    const int es = ln_dtype_size(q.dtype), V = ln_vectors(a, es) ? 16 / es : 1;
-    const int blocks = ln_bwd_blocks(a.rows, a.D, V);
+    const int blocks = ln_bwd_blocks(a.rows, a.D, 16 / ln_dtype_size(q.dtype));
     if (blocks > 1 || a.D > LN_ALONE) a.part = static_cast<float*>(q.ws);
-    const int bv = V > 1 ? blocks : 0;
-    int rc = q.dtype == PCX_F32 ? ln_run<float>(a, true, blocks, bv, s)
-             : q.dtype == PCX_BF16 ? ln_run<bf16>(a, true, blocks, bv, s)
-                                   : ln_run<f16>(a, true, blocks, bv, s);
+    const int rc = ln_any<true>(a, q.dtype, blocks, s);
     if (rc || !a.cols || !a.part) return rc;
     const int cb = ceil_div(2 * (int64_t)a.D, 32);
     if (q.wdtype == PCX_F32)
