@@ -9,8 +9,9 @@
 // registers between its two reductions (the variance is summed about the mean, not from squares: no cancellation for
 // rows far from zero), and the backward sums dw / db over the rows of its block in registers, so x and dy are read
 // once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
-// Measured: 8192 x 5120 in float16 forward 33.8 us, 5.0 TB/s (29.9 by the kernel's own clock, where a copy's 5.86 TB/s
-// would take 28.6); 16384 x 4096 in bfloat16 with its gradients 139 us, 4.8 TB/s (forward 49.6, backward 85.5 and 6.3).
+// Measured: 8192 x 5120 in float16 forward 33.3 us, 5.0 TB/s (29.9 by the kernel's own clock, where a copy's 5.86 TB/s
+// would take 28.6); 16384 x 4096 in bfloat16 with its gradients 139 us, 4.8 TB/s (forward 49, backward 84 and 6).  Rows of
+// 4097 values, none of them aligned: bfloat16 forward 51 us, float32 100, with gradients 181 and 252.
 // Few rows are latency: 24 x 128 with its gradients 8 us in two kernels, under 60 us of the host's way through autograd.
 //
 // A row belongs to 1 ... 64 lanes of a wave or to a block of just the waves it needs: sub-wave rows need no barrier, and
@@ -537,7 +538,8 @@ int ln_even(int64_t passes, int64_t most) {
 }
 
 // The forward keeps 1536 threads of a CU busy.  The backward's partial sums are 8 D bytes per block, written and read
-// once, next to the rows' own 3 tensors: 1024 threads a CU, and no block with fewer than 8 passes.
+// once, next to the rows' own 3 tensors: 1024 threads a CU, and no block with fewer than 4 passes (kernels of 1003 x 1537
+// in bfloat16 with its gradients 23.8 us with 8, 20.9 with 4, 24.6 with 2; 4096 x 128 in float32 17.7, 14.8, 15.1).
 int ln_fwd_blocks(int64_t rows, int D, int V) {
     const int64_t rpb = ln_rows_per_block(D, V, false), passes = (rows + rpb - 1) / rpb;
     const int threads = D > LN_NARROW && ln_pick(D, V, false).block ? ln_pick(D, V, false).tpr : 256;
@@ -546,7 +548,7 @@ int ln_fwd_blocks(int64_t rows, int D, int V) {
 int ln_bwd_blocks(int64_t rows, int D, int V) {
     const int64_t rpb = ln_rows_per_block(D, V, true), passes = (rows + rpb - 1) / rpb;
     const int threads = D > LN_NARROW && ln_pick(D, V, true).block ? ln_pick(D, V, true).tpr : 256;
-    const int64_t most = std::min<int64_t>((int64_t)num_cus() * std::max(1, 1024 / threads), (passes + 7) / 8);
+    const int64_t most = std::min<int64_t>((int64_t)num_cus() * std::max(1, 1024 / threads), (passes + 3) / 4);
     return ln_even(passes, std::max<int64_t>(1, std::min<int64_t>(512, most)));
 }
 
