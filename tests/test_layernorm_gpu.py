@@ -351,3 +351,28 @@ def test_writes_stay_inside_their_tensors(D, t):
     assert torch.equal(wide.detach(), before)
     for a, r, tol, what in zip(got, *reference(x, w, b, dy, 1e-5), ("y", "dx", "dw", "db")):
         close(a, r, tol, what)
+
+
+@pytest.mark.parametrize("D", [33, 39, 65, 250, 513, 1030, 4097, 9001])
+@pytest.mark.parametrize("t,wt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32")])
+def test_slices_off_every_boundary(D, t, wt):
+    """Rows, gradients and weights that start at each element of a 16-byte group."""
+    from phoneme_contrast_amd.layers import layer_norm
+    x, w, b, dy = inputs(5, D, TYPES[t], TYPES[wt], 17)
+    ref, tol = reference(x, w, b, dy, 1e-5)
+    n = 16 // x.element_size()
+    first = None
+    for off in range(n):
+        wide = torch.zeros(5, 2 * D + 2 * n + 1, dtype=TYPES[t], device="cuda")
+        wide[:, off:off + D], wide[:, D + n:2 * D + n] = x.cuda(), dy.cuda()
+        flat = torch.zeros(2, D + n, dtype=TYPES[wt], device="cuda")
+        flat[0, off:off + D], flat[1, n - off:n - off + D] = w.cuda(), b.cuda()
+        vx = wide[:, off:off + D].requires_grad_(True)
+        vw, vb = flat[0, off:off + D].requires_grad_(True), flat[1, n - off:n - off + D].requires_grad_(True)
+        y = layer_norm(vx, D, vw, vb)
+        got = [y.detach(), *torch.autograd.grad(y, [vx, vw, vb], wide[:, D + n:2 * D + n])]
+        for a, r, lim, what in zip(got, ref, tol, ("y", "dx", "dw", "db")):
+            close(a, r, lim, what)
+        first = first or got
+        for a, c in zip(first, got):
+            assert torch.equal(a, c)  # where a row lies does not change it
