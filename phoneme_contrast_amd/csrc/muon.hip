@@ -25,8 +25,8 @@
 // swizzled in LDS 4059 us at a later step, 3948 as it is now.)
 // A and B are symmetric: only tiles on and below the diagonal are computed, and written twice.
 //
-// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.67 to 3.88 ms (one card and
-// another), 0.53 to 0.56 PFLOP/s of the three products' definition and 1.06 to 1.12 executed (three terms, half of the
+// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.67 to 4.06 ms (one card and
+// another), 0.51 to 0.56 PFLOP/s of the three products' definition and 1.02 to 1.12 executed (three terms, half of the
 // tiles of A and B), where a float16 product of the library reaches 1.08 at that size.  Of a few hundred tiles: LDS, which
 // feeds the MFMAs of 64 x 64 tiles at half their rate, the traffic from L2, and a launch's fixed parts (addresses, first
 // stages, the epilogue's passes).  Small ones: those fixed parts, 5 to 8 us a launch of which 2 to 3 compute.
@@ -264,7 +264,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const void* job) {
     const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
     const int tn = e.np / 64, per = (e.mp / 64) * tn;
-    const int rel = blockIdx.x - un.first[ei], bat = rel / per, tl = rel % per;
+    // (adjacent tiles to one XCD, as in the products: the lines they share are whole in one L2; 16.7 -> 14.3 us of
+    // 6 x 1000 x 333 bfloat16 values)
+    const int rel = xcd_order(blockIdx.x - un.first[ei], per * e.batch), bat = rel / per, tl = rel % per;
     const int i0 = (tl / tn) * 64, j0 = (tl % tn) * 64;  // of X (m x n)
     const Planes P = planes_of(q, e, bat);
     const bool tall = e.rows > e.cols;
