@@ -376,3 +376,19 @@ def test_slices_off_every_boundary(D, t, wt):
         first = first or got
         for a, c in zip(first, got):
             assert torch.equal(a, c)  # where a row lies does not change it
+
+
+@pytest.mark.parametrize("rows,D", [(600000, 4096), (70000, 32768)])
+def test_offsets_that_pass_32_bits(rows, D):
+    from phoneme_contrast_amd.layers import layer_norm
+    x = torch.empty(rows, D, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = torch.linspace(0.5, 1.5, D).bfloat16()
+    b = torch.linspace(-1, 1, D).bfloat16()
+    x.requires_grad_(True)
+    y = layer_norm(x, D, w.cuda(), b.cuda())
+    dy = torch.flip(y.detach(), (0,))
+    (dx,) = torch.autograd.grad(y, [x], dy)
+    pick = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1])
+    ref, tol = reference(x[pick.cuda()].detach().cpu(), w, b, dy[pick.cuda()].cpu(), 1e-5)
+    close(y[pick.cuda()], ref[0], tol[0], "y")
+    close(dx[pick.cuda()], ref[1], tol[1], "dx")

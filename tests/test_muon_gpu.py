@@ -438,3 +438,61 @@ def test_states_of_the_two_optimizers_are_told_apart():
     plain = torch.optim.Adam([torch.nn.Parameter(p.detach().clone()) for p in a.parameters()])
     oa.load_state_dict(plain.state_dict())
     plain.load_state_dict(oa.state_dict())
+
+
+def test_offsets_that_pass_32_bits():
+    """The longest side there is (planes of 2^32 numbers), both ways round, and batches far apart in memory."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(512, 1 << 20, device="cuda", generator=gen).bfloat16()
+    ref = x.double()
+    ref /= torch.linalg.vector_norm(ref) + 1e-7
+    gram = ref @ ref.T.contiguous()
+    # `bound` needs the singular values alone; every step's polynomial in X X^T acts on the left
+    small = torch.diag(torch.linalg.eigvalsh(gram.cpu()).clamp(min=0).sqrt())
+    g = (4 + 2 * math.sqrt(1 << 20)) / (4 + 2 * math.sqrt(512))
+    left = torch.eye(512, dtype=torch.float64, device="cuda")
+    for _ in range(5):
+        a = left @ gram @ left.T.contiguous()
+        left = COEF[0] * left + (COEF[1] * a + COEF[2] * (a @ a)) @ left
+    ref = left @ ref
+    limit = g * bound(small, eps=0.0) + (2.0 ** -8 + 2.0 ** -20) * torch.linalg.vector_norm(ref).item()
+    for t in (x, x.T):
+        out = orthogonalize(t)
+        out = out if t is x else out.T
+        off = sum(torch.linalg.vector_norm(out[i:i + 64].double() - ref[i:i + 64]).item() ** 2 for i in range(0, 512, 64)) ** 0.5
+        assert off <= limit, (off, limit)
+        assert torch.isfinite(out[-1, -1]) and (out[-1, -4096:].double() - ref[-1, -4096:]).abs().max() <= 2.0 ** -7 * ref.abs().max()
+    del x, ref, out
+    far = torch.empty(2 * ((1 << 31) + 7) + 40000, dtype=torch.float16, device="cuda")
+    view = far.as_strided((3, 90, 110), ((1 << 31) + 7, 1, 301))
+    values = torch.stack([gradient(90, 110, s) for s in range(3)]).half()
+    view.copy_(values)
+    for o, v in zip(orthogonalize(view), values):
+        close(o, v.double())
+
+
+def test_two_streams_at_once():
+    from phoneme_contrast_amd.layers import layer_norm
+    from phoneme_contrast_amd.optim import muon_step, orthogonalize
+    xs = [gradient(300, 2000, 1).cuda(), gradient(700, 130, 2).cuda()]
+    want = [orthogonalize(x) for x in xs]
+    norms = [layer_norm(x, x.shape[-1]) for x in xs]
+    start = [[gradient(*s, 3).cuda() for s in ((64, 288), (128, 1152), (40, 9))] for _ in range(3)]
+    p, g, m = ([t.clone() for t in ts] for ts in start)
+    muon_step(p, g, m, lr=0.1)
+    sides = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, (s, x) in enumerate(zip(sides, xs)):
+            with torch.cuda.stream(s):
+                lists = [[t.clone() for t in ts] for ts in start]
+                muon_step(*lists, lr=0.1)
+                got[i].append((orthogonalize(x), layer_norm(x, x.shape[-1]), lists))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, y, lists in got[i]:
+            assert torch.equal(o, want[i]) and torch.equal(y, norms[i])
+            for a, b in zip(lists[0] + lists[2], p + m):
+                assert torch.equal(a, b)
