@@ -1017,13 +1017,15 @@ template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kern
         for (int w = 0; w < NSB_WAVES; ++w) s += red[w];
         const double norm = sqrt(s), inv = 1. / (norm + (double)q.eps);
         if (threadIdx.x == 0) {
-            red[NSB_WAVES] = q.sx * inv;
-            red[NSB_WAVES + 1] = (double)ns_scale(norm * inv, q.growth);
+            const int k = ns_scale(norm * inv, q.growth);
+            red[NSB_WAVES] = ldexp(q.sx * inv, k);
+            red[NSB_WAVES + 1] = (double)k;
         }
     }
     __syncthreads();
     const int lift = (int)red[NSB_WAVES + 1];
-    const float scale = (float)red[NSB_WAVES], more = ldexpf(1.f, lift), unit = ldexpf(1.f / q.sx, -lift);
+    const double scale = red[NSB_WAVES];  // (up to 2^248 where norm and eps are float32's smallest: no float32 holds it)
+    const float unit = ldexpf(1.f / q.sx, -lift);
     // The wave's tiles of X, in pairs along n: of pair i rows 32 tr[i] of m, columns 32 tc[i] of n and the next 32 (a pair
     // at an odd end has no second tile: it computes one that is not stored).  And its pair of tiles of A.
     const int pr = tall ? 1 : pitch, pc = tall ? pitch : 1, row_pairs = (nb + 1) / 2, a_pairs = (mb + 1) / 2;
@@ -1040,7 +1042,7 @@ template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kern
             const float* at = raw + r0 * pr + c * pc;
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-                x[i][j][k] = r0 + acc_row(k, 0) < m && c < n ? at[acc_row(k, 0) * pr] * scale * more : 0.f;
+                x[i][j][k] = r0 + acc_row(k, 0) < m && c < n ? (float)(at[acc_row(k, 0) * pr] * scale) : 0.f;
         }
     }
     const int ar = wave / a_pairs, ac = 2 * (wave % a_pairs);

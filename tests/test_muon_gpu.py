@@ -496,3 +496,29 @@ def test_two_streams_at_once():
             assert torch.equal(o, want[i]) and torch.equal(y, norms[i])
             for a, b in zip(lists[0] + lists[2], p + m):
                 assert torch.equal(a, b)
+
+
+TINY = torch.finfo(torch.float32).tiny
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (2, 3), (8, 9), (64, 64), (128, 128), (200, 333)])  # one block; products
+@pytest.mark.parametrize("eps", [TINY, 2.0 ** -149])
+def test_tiny_eps(rows, cols, eps):
+    """The scale 1 / (|x|_F + eps) leaves float32's range: a zero matrix stays zero on every route, a tiny one is scaled."""
+    from phoneme_contrast_amd.optim import muon_step, orthogonalize
+    x = gradient(rows, cols, 3)
+    x *= 1e-36 / x.norm()
+    batch = torch.stack([torch.zeros_like(x), x, gradient(rows, cols, 4)])
+    out = orthogonalize(batch.cuda(), eps=eps)
+    assert not out[0].any()
+    close(out[1], batch[1].double(), eps=eps)
+    close(out[2], batch[2].double(), eps=eps)
+    # a layer without a gradient is decayed alone
+    if rows == 1:
+        return
+    p = [gradient(rows, cols, 5).cuda() for _ in range(2)]
+    g, m = [torch.zeros_like(p[0]), x.cuda()], [torch.zeros_like(p[0]) for _ in range(2)]
+    want = (p[0].double() * (1 - 0.1 * 0.5)).cpu()
+    muon_step(p, g, m, lr=0.1, weight_decay=0.5, eps=eps)
+    assert ((p[0].cpu().double() - want).abs() <= 2.0 ** -22 * want.abs()).all()
+    assert torch.isfinite(p[1]).all() and not m[0].any()
