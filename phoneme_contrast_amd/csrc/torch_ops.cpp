@@ -178,6 +178,8 @@ Tensor layer_norm(const Tensor& x, at::IntArrayRef shape, const std::optional<Te
                       "layer_norm: weight and bias must have one type");
     TORCH_CHECK_VALUE(eps > 0. && eps < 1e30, "layer_norm: eps must be positive, got ", eps);
     TORCH_CHECK(x.is_cuda(), "layer_norm: tensors must live on a ROCm GPU (got device '", x.device(), "')");
+    for (const Tensor* t : {&x, &w, &b})  // (a tensor outside of a forward-mode level has none)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: no forward-mode derivative");
     std::optional<Tensor> wc, bc;
     if (w.defined()) wc = w.contiguous();
     if (b.defined()) bc = b.contiguous();

@@ -18,7 +18,8 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
 
     x: float32, bfloat16 or float16 on a ROCm GPU, any leading axes and any strides (evenly spaced rows of adjacent
     values are read in place); weight, bias: `normalized_shape`, both of x's type or both float32.  The result has x's
-    type, the gradients their tensors' types.  Up to 32768 values per row.  The gradient is not differentiable again."""
+    type, the gradients their tensors' types.  Up to 32768 values per row.  The gradient is not differentiable again;
+    forward-mode derivatives and torch.func.grad raise."""
     _lib.require_gpu(x, weight, bias, what="layer_norm")
     shape = (normalized_shape,) if isinstance(normalized_shape, numbers.Integral) else normalized_shape
     return _lib.torch_ops().layer_norm(x, shape, weight, bias, eps)

@@ -392,3 +392,34 @@ def test_offsets_that_pass_32_bits(rows, D):
     ref, tol = reference(x[pick.cuda()].detach().cpu(), w, b, dy[pick.cuda()].cpu(), 1e-5)
     close(y[pick.cuda()], ref[0], tol[0], "y")
     close(dx[pick.cuda()], ref[1], tol[1], "dx")
+
+
+def test_transforms():
+    """Nothing is dropped in silence: forward mode, torch.func.grad and tensors without memory raise."""
+    import torch.autograd.forward_ad as fwd
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from phoneme_contrast_amd.layers import layer_norm
+    x, w, b, dy = (t.cuda() for t in inputs(6, 40, torch.float32, torch.float32, 18))
+    with fwd.dual_level():
+        for i in range(3):
+            for leaf in (False, True):
+                args = [t.clone() for t in (x, w, b)]
+                args[i] = fwd.make_dual(args[i].requires_grad_(leaf), torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    layer_norm(args[0], 40, args[1], args[2])
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            layer_norm(fwd.make_dual(x, dy), 40, w, b)
+        layer_norm(x, 40, w, b)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: layer_norm(t, 40, w, b), (x,), (dy,))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layer_norm(t, 40, w, b).sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: layer_norm(t, 40, w.clone().requires_grad_(True), b))(x.view(2, 3, 40))
+    # without gradients torch maps the operator slice by slice
+    rows = torch.func.vmap(lambda t: layer_norm(t, 40, w, b))(x.view(2, 3, 40))
+    assert torch.equal(rows.view(6, 40), layer_norm(x, 40, w, b))
+    weights = torch.func.vmap(lambda u: layer_norm(x, 40, u, b))(torch.stack([w, b]))
+    assert torch.equal(weights[0], layer_norm(x, 40, w, b)) and torch.equal(weights[1], layer_norm(x, 40, b, b))
+    with FakeTensorMode() as mode, pytest.raises((RuntimeError, ValueError)):
+        layer_norm(mode.from_tensor(x), 40)
