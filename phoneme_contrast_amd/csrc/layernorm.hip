@@ -6,9 +6,13 @@
 //   dw = sum_rows dy xhat       db = sum_rows dy
 //
 // Both passes are bound by HBM: 2 tensors move in the forward, 3 in the backward.  A row is read once and stays in
-// registers between its two reductions (the variance is summed about the mean, not from squares: no cancellation for
-// rows far from zero), and the backward sums dw / db over the rows of its block in registers, so x and dy are read
-// once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
+// registers between its reductions, and the backward sums dw / db over the rows of its block in registers, so x and dy
+// are read once for dx, dw and db together.  Every sum is in 32 bits or more and in a fixed order: results repeat bit by bit.
+// Rows far from zero: a mean off by one of its own steps would be the whole of a narrow row's xhat.  So the deviations
+// d = x - m from the first mean m are summed next to their squares, e = sum d / D, var = sum d^2 / D - e^2 and
+// xhat = (d - e) rstd; where e^2 makes up more than a quarter of sum d^2 / D (the subtraction would cancel), m moves to
+// m + e first, which the row does at most twice.  A constant row gives the bias, whatever its value.  The statistics keep
+// m + e rounded to float32: the backward's xhat is off by rstd times half a step of the mean.
 // Measured: 8192 x 5120 in float16 forward 33.3 us, 5.0 TB/s (29.9 by the kernel's own clock, where a copy's 5.86 TB/s
 // would take 28.6); 16384 x 4096 in bfloat16 with its gradients 139 us, 4.8 TB/s (forward 49, backward 84 and 6).  Rows of
 // 4097 values, none of them aligned: bfloat16 forward 51 us, float32 100, with gradients 181 and 252.
@@ -118,28 +122,48 @@ template <typename T> __device__ __forceinline__ void put_column(const LnArgs& a
     else static_cast<T*>(out)[d] = (T)v;
 }
 
-// sums over the lanes of a row: tpr lanes of a wave, or (BLOCK) all waves of the block through `red` with one barrier; the
-// caller alternates between two `red` buffers, so a buffer is rewritten only behind the other's barrier
-template <bool BLOCK, int N> __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float (*red)[16]) {
-    if constexpr (!BLOCK) {
-        for (int o = tpr >> 1; o > 0; o >>= 1) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o, 64);
-        }
+// v of this lane and of the one at 2^LEVEL lanes' distance, in every lane; below LEVEL all lanes hold the same sums, so
+// mirrored lanes serve for distances 4 and 8.  Within the registers: a sum over a wave through LDS (shuffles) waits for it
+// six times, and a row has three of them on its way from its values to its result.
+template <int LEVEL> __device__ __forceinline__ float pair_sum(float v) {
+    if constexpr (LEVEL < 4) {
+        constexpr int ctrl = LEVEL == 0 ? 0xb1 : LEVEL == 1 ? 0x4e : LEVEL == 2 ? 0x141 : 0x140;
+        return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), ctrl, 0xf, 0xf, true));
     } else {
+        const unsigned u = __float_as_uint(v);
+        const auto t = [&] {
+            if constexpr (LEVEL == 4) return __builtin_amdgcn_permlane16_swap(u, u, false, false);
+            else return __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        }();
+        return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+    }
+}
+// sums over groups of n lanes, a power of two (ALL: 2^TOP)
+template <bool ALL, int N, int TOP = 6, int LEVEL = 0> __device__ __forceinline__ void lane_sum(float (&v)[N], int n) {
+    if constexpr (LEVEL < TOP) {
+        if (ALL || n > 1 << LEVEL) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+            for (int i = 0; i < N; ++i) v[i] = pair_sum<LEVEL>(v[i]);
+            lane_sum<ALL, N, TOP, LEVEL + 1>(v, n);
+        }
+    }
+}
+
+// sums over the lanes of a row: tpr lanes of a wave (WHOLE: all of them), or (BLOCK) all waves of the block through `red` with one barrier; the
+// caller alternates between two `red` buffers, so a buffer is rewritten only behind the other's barrier
+template <bool BLOCK, bool WHOLE, int N> __device__ __forceinline__ void row_sum(float (&v)[N], int tpr, float (*red)[16]) {
+    lane_sum<WHOLE, N>(v, tpr);
+    if constexpr (BLOCK) {
         if ((threadIdx.x & 63) == 0) {
 #pragma unroll
             for (int i = 0; i < N; ++i) red[i][threadIdx.x >> 6] = v[i];
         }
         __syncthreads();
+        // (a lane to a wave: a loop over the waves waits for LDS at each)
+        const int w = threadIdx.x & 15;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float s = 0.f;
-            for (int w = 0; w < tpr / 64; ++w) s += red[i][w];
-            v[i] = s;
-        }
+        for (int i = 0; i < N; ++i) v[i] = w < tpr / 64 ? red[i][w] : 0.f;
+        lane_sum<true, N, 4>(v, 16);
     }
 }
 
@@ -149,7 +173,8 @@ template <typename T, int V, int E, bool BLOCK>
 __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
     constexpr bool KEEP = E <= 16, AHEAD = KEEP;  // (what the registers of 1024 threads hold)
-    __shared__ float red[2][1][16];
+    constexpr bool WHOLE = BLOCK || E > V;        // (as ln_pick chooses)
+    __shared__ float red[2][2][16];
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
     const int lane = BLOCK ? (int)threadIdx.x : (int)(threadIdx.x & (unsigned)(tpr - 1));
     const int64_t rpb = BLOCK ? 1 : 256 / tpr, stride = gridDim.x * rpb;
@@ -170,6 +195,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) raw[c] = load_raw<V>(x + Place<V>(lane, tpr, c, a.D).d);
     };
+    int par = 0;
     int64_t r = (int64_t)blockIdx.x * rpb + (BLOCK ? 0 : (int)(threadIdx.x / (unsigned)tpr));
     pack<T, V> next[NC];
     if constexpr (AHEAD) fetch(r, next);
@@ -179,7 +205,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
     }
     for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < a.rows; r0 += stride, r += stride) {
         float v[NC][V];
-        float s[1] = {0.f};
+        float m[1] = {0.f};
         if constexpr (!AHEAD) fetch(r, next);
 #pragma unroll
         for (int c = 0; c < NC; ++c) widen<T, V>(next[c], v[c]);
@@ -189,30 +215,53 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
             const Place<V> at(lane, tpr, c, a.D);
             if (at.whole) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[0] += v[c][j];
+                for (int j = 0; j < V; ++j) m[0] = fmaf(v[c][j], invd, m[0]);  // (a sum of x could overflow)
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[0] += j >= at.skip ? v[c][j] : 0.f;
+                for (int j = 0; j < V; ++j) m[0] = fmaf(j >= at.skip ? v[c][j] : 0.f, invd, m[0]);
             }
         }
-        row_sum<BLOCK, 1>(s, tpr, red[0]);
-        const float mean = s[0] * invd;
-        s[0] = 0.f;
+        row_sum<BLOCK, WHOLE, 1>(m, tpr, red[par]);
+        par ^= 1;
+        float mean = m[0], e, var;
+        // from deviations so far, those from a mean `shift` further -> whether that one is far from theirs
+        const auto deviate = [&](float shift) {
+            float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const Place<V> at(lane, tpr, c, a.D);
+            for (int c = 0; c < NC; ++c) {
+                const Place<V> at(lane, tpr, c, a.D);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] -= mean;
-            if (at.whole) {
+                for (int j = 0; j < V; ++j) v[c][j] -= shift;
+                if (at.whole) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[0] = fmaf(v[c][j], v[c][j], s[0]);
-            } else {
+                    for (int j = 0; j < V; ++j) {
+                        s[0] += v[c][j];
+                        s[1] = fmaf(v[c][j], v[c][j], s[1]);
+                    }
+                } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[0] += j >= at.skip ? v[c][j] * v[c][j] : 0.f;
+                    for (int j = 0; j < V; ++j) {
+                        const float d = j >= at.skip ? v[c][j] : 0.f;
+                        s[0] += d;
+                        s[1] = fmaf(d, d, s[1]);
+                    }
+                }
             }
+            row_sum<BLOCK, WHOLE, 2>(s, tpr, red[par]);
+            par ^= 1;
+            e = s[0] * invd;
+            const float sq = s[1] * invd;
+            var = sq < INFINITY ? fmaxf(sq - e * e, 0.f) : sq;  // (NaN stays NaN)
+            return !(4.f * e * e <= sq && sq < INFINITY);
+        };
+        bool far = deviate(mean);
+#pragma unroll 1
+        for (int turn = 0; turn < 2 && (BLOCK ? far : __any(far)); ++turn) {  // (the same for a row's, and a wave's, lanes)
+            const float to = far ? mean + e : mean, shift = to - mean;
+            mean = to;
+            far = deviate(shift);
         }
-        row_sum<BLOCK, 1>(s, tpr, red[1]);
-        const float rstd = 1.f / sqrtf(fmaf(s[0], invd, a.eps));
+        const float rstd = 1.f / sqrtf(var + a.eps);
         if (r >= a.rows) continue;  // (a whole sub-wave row; the others of its wave go on)
         T* y = static_cast<T*>(a.y) + r * a.D;
 #pragma unroll
@@ -220,13 +269,13 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_fwd_kernel(LnArgs a) {
             const int k = KEEP ? c : 0;
             if constexpr (!KEEP) weights(c, w[0], b[0]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] = fmaf(v[c][j] * rstd, w[k][j], b[k][j]);
+            for (int j = 0; j < V; ++j) v[c][j] = fmaf((v[c][j] - e) * rstd, w[k][j], b[k][j]);
             const Place<V> at(lane, tpr, c, a.D);
             if (at.here()) store_v<V>(y + at.d, v[c]);
             if constexpr (!KEEP)  // (few weights in flight, or the registers spill)
                 if (c % 4 == 3) asm volatile("" ::: "memory");
         }
-        if (a.stat && lane == 0) a.stat[r] = make_float2(mean, rstd);
+        if (a.stat && lane == 0) a.stat[r] = make_float2(mean + e, rstd);
     }
 }
 
@@ -235,6 +284,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
     constexpr int NC = E / V;
     constexpr bool AHEAD = E <= 8 || sizeof(T) == 2;  // (16 float32 values a thread leave no registers for the next row,
     constexpr bool KEEP = E <= 8 || (AHEAD && !BLOCK);  // of 16 bits none for the weights in blocks of 1024 threads)
+    constexpr bool WHOLE = BLOCK || E > V;
     __shared__ float red[2][2][16];
     extern __shared__ __attribute__((aligned(16))) float cols[];  // sub-wave rows: [4 waves][D] of dw, then of db
     const int tpr = BLOCK ? (int)blockDim.x : a.tpr;
@@ -317,7 +367,7 @@ __global__ __launch_bounds__(BLOCK ? 1024 : 256) void ln_bwd_kernel(LnArgs a) {
             }
         }
         if (!a.dx) continue;  // (the same for the whole grid)
-        row_sum<BLOCK, 2>(s, tpr, red[par]);
+        row_sum<BLOCK, WHOLE, 2>(s, tpr, red[par]);
         par ^= 1;
         const float c1 = s[0] * invd, c2 = s[1] * invd;
         if (!on) continue;
@@ -444,7 +494,7 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_long_bwd_kernel
                 s[0] += g;
                 s[1] = fmaf(g, ((float)x[d] - st.x) * st.y, s[1]);
             }
-            row_sum<true, 2>(s, 1024, red[par]);
+            row_sum<true, true, 2>(s, 1024, red[par]);
             const float c1 = s[0] * invd, c2 = s[1] * invd;
             T* dx = static_cast<T*>(a.dx) + r * a.D;
 #pragma unroll 4
@@ -538,8 +588,10 @@ int ln_even(int64_t passes, int64_t most) {
 }
 
 // The forward keeps 1536 threads of a CU busy.  The backward's partial sums are 8 D bytes per block, written and read
-// once, next to the rows' own 3 tensors: 1024 threads a CU, and no block with fewer than 4 passes (kernels of 1003 x 1537
-// in bfloat16 with its gradients 23.8 us with 8, 20.9 with 4, 24.6 with 2; 4096 x 128 in float32 17.7, 14.8, 15.1).
+// once, next to the rows' own 3 tensors: two blocks a CU, one from 513 threads on, and no block with fewer than 4 passes
+// (kernels of 1003 x 1537 in bfloat16 with its gradients 23.8 us with 8, 20.9 with 4, 24.6 with 2; 4096 x 128 in float32
+// 17.7, 14.8, 15.1).  us with 1 / 2 / 3 / 4 blocks a CU, 256 threads each: 65536 x 128 float32 33.3 / 27.8 / 28.0 / 30.0,
+// 65536 x 512 80.6 / 82.6 / 86.0 / 89.6, 131072 x 256 112 / 81 / 83 / 87, 262144 x 128 bfloat16 59 / 46 / 45 / 47.
 int ln_fwd_blocks(int64_t rows, int D, int V) {
     const int64_t rpb = ln_rows_per_block(D, V, false), passes = (rows + rpb - 1) / rpb;
     const int threads = D > LN_NARROW && ln_pick(D, V, false).block ? ln_pick(D, V, false).tpr : 256;
@@ -548,8 +600,7 @@ int ln_fwd_blocks(int64_t rows, int D, int V) {
 int ln_bwd_blocks(int64_t rows, int D, int V) {
     const int64_t rpb = ln_rows_per_block(D, V, true), passes = (rows + rpb - 1) / rpb;
     const int threads = D > LN_NARROW && ln_pick(D, V, true).block ? ln_pick(D, V, true).tpr : 256;
-    const int64_t most = std::min<int64_t>((int64_t)num_cus() * std::max(1, 1024 / threads), (passes + 3) / 4);
-    return ln_even(passes, std::max<int64_t>(1, std::min<int64_t>(512, most)));
+    return ln_even(passes, std::max<int64_t>(1, std::min<int64_t>((int64_t)num_cus() * (threads > 512 ? 1 : 2), (passes + 3) / 4)));
 }
 
 template <typename T, int V, int E, bool BLOCK, bool BWD> int ln_go(const LnArgs& a, int blocks, hipStream_t s) {

@@ -423,3 +423,52 @@ def test_transforms():
     assert torch.equal(weights[0], layer_norm(x, 40, w, b)) and torch.equal(weights[1], layer_norm(x, 40, b, b))
     with FakeTensorMode() as mode, pytest.raises((RuntimeError, ValueError)):
         layer_norm(mode.from_tensor(x), 40)
+
+
+FAR = [(t, v) for t, vs in (("f32", (1.0, 16384.0, 60000.0, -0.1, 1e15, 3e38)), ("f16", (16384.0, 60000.0)),
+                            ("bf16", (16384.0, 0.1))) for v in vs]
+
+
+@pytest.mark.parametrize("t,v", FAR)
+def test_constant_rows_of_any_value(t, v):
+    """A constant row has xhat = 0: y is the bias, dw 0 and dx = rstd (g - c1), whatever the value and the width.  c1 is
+    off by the row sum (at most 32 additions in a thread, 6 in a wave, 16 over waves) and two roundings, rstd by four."""
+    from phoneme_contrast_amd.layers import layer_norm
+    for D in (33, 40, 100, 513, 1025, 1172, 1228, 1537, 2056, 4097, 5000, 8191, 9001, 16383, 20001, 32767):
+        gen = torch.Generator().manual_seed(D)
+        x = torch.full((3, D), v, dtype=TYPES[t]).cuda().requires_grad_(True)
+        w = torch.randn(D, generator=gen).cuda().requires_grad_(True)
+        b = torch.randn(D, generator=gen).cuda().requires_grad_(True)
+        if t == "f32" and D % 2:
+            dy = torch.randn(3, D, generator=gen)
+        else:
+            dy = torch.randn(3, D, generator=gen).to(TYPES[t])
+        y = layer_norm(x, D, w, b)
+        assert torch.equal(y, b.detach().to(TYPES[t]).expand(3, D)), D
+        dx, dw = torch.autograd.grad(y, [x, w], dy.cuda())
+        assert not dw.any(), D
+        g = dy.double() * w.detach().cpu().double()
+        ref = (g - g.mean(1, keepdim=True)) / 1e-5 ** 0.5
+        tol = (8 * U * (g.abs() + g.abs().mean(1, keepdim=True)) + 56 * U * g.abs().mean(1, keepdim=True)) / 1e-5 ** 0.5
+        close(dx, ref, tol, f"dx {D}")
+
+
+@pytest.mark.parametrize("base", [60000.0, -16384.0, 3e7])
+@pytest.mark.parametrize("D", [40, 1025, 1172, 1537, 4100, 20001])
+def test_rows_a_few_steps_wide(base, D):
+    """Values on float32's own grid around a far base: x - m is exact, and y as exact as for rows at zero.  A row sum is off
+    by 54 u (32 additions in a thread, 6 in a wave, 16 over waves at most) and its mean by 55 u; the variance is at least
+    half of sum d^2 / D, so off by 110 u, rstd by 57 u; d - e by one rounding and 55 u of e, which is at most half a step;
+    two more roundings to the result: 60 u |xhat w| + 28 u rstd step |w| + u |y|."""
+    from phoneme_contrast_amd.layers import layer_norm
+    gen = torch.Generator().manual_seed(D)
+    step = 2.0 ** (np.floor(np.log2(abs(base))) - 23)
+    x = (base + step * torch.randint(-3, 4, (4, D), generator=gen).double()).float()
+    x[0], x[0, 0] = base, base + step  # one value off
+    w, b = torch.randn(D, generator=gen), torch.randn(D, generator=gen)
+    xd = x.double()
+    u = xd - xd.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt((u * u).mean(1, keepdim=True) + 1e-5)
+    ref = u * rstd * w.double() + b.double()
+    tol = U * (64 * (u.abs() * rstd + rstd * step) * w.double().abs() + 2 * b.double().abs())
+    close(layer_norm(x.cuda(), D, w.cuda(), b.cuda()), ref, tol, "y")
