@@ -127,7 +127,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (need_w) dw.zero_();
             if (need_b) db.zero_();
         } else {
-            auto [dyr, dyrows, dys] = rows_of(grads[0], D);
+            auto [dyr, dyrows, dys] = rows_of(grads[0].resolve_neg(), D);
             size_t nws = 0;
             if (need_w || need_b) {
                 nws = pcx_layernorm_workspace_bytes(dt, rows, D);
@@ -180,12 +180,14 @@ Tensor layer_norm(const Tensor& x, at::IntArrayRef shape, const std::optional<Te
     TORCH_CHECK(x.is_cuda(), "layer_norm: tensors must live on a ROCm GPU (got device '", x.device(), "')");
     for (const Tensor* t : {&x, &w, &b})  // (a tensor outside of a forward-mode level has none)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: no forward-mode derivative");
+    // (a view whose negation is pending, as the imaginary part of a conjugate, is written out: the kernels read memory)
+    const Tensor xr = x.resolve_neg();
     std::optional<Tensor> wc, bc;
-    if (w.defined()) wc = w.contiguous();
-    if (b.defined()) bc = b.contiguous();
+    if (w.defined()) wc = w.resolve_neg().contiguous();
+    if (b.defined()) bc = b.resolve_neg().contiguous();
     if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
-        return LayerNorm::apply(x, wc, bc, D, eps);
-    return forward(x, wc.value_or(Tensor()), bc.value_or(Tensor()), D, eps, nullptr);
+        return LayerNorm::apply(xr, wc, bc, D, eps);
+    return forward(xr, wc.value_or(Tensor()), bc.value_or(Tensor()), D, eps, nullptr);
 }
 
 }  // namespace

@@ -225,6 +225,7 @@ def orthogonalize(x, ns_steps=5, ns_coefficients=NS_COEFFICIENTS, eps=1e-7):
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
         return out
+    x = x.resolve_neg()  # (the kernels read memory)
     rows, cols = x.shape[-2:]
     if x.dim() == 2:
         batch, bstride = 1, 0
@@ -302,8 +303,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
         for name, t in (("parameter", p), ("gradient", g), ("momentum buffer", m)):
             if t.shape != p.shape:
                 raise ValueError(f"muon_step: {name} {i} has shape {tuple(t.shape)}, {tuple(p.shape)} expected")
-            if t.dtype != torch.float32 or not t.is_contiguous():
-                raise ValueError(f"muon_step: {name} {i} must be contiguous float32")
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.is_neg():
+                raise ValueError(f"muon_step: {name} {i} must be contiguous float32 in memory")
             if t.device != dev:
                 raise RuntimeError(f"muon_step: {name} {i} is on {t.device}, parameter 0 on {dev}")
             spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel(), name != "gradient"))

@@ -472,3 +472,25 @@ def test_rows_a_few_steps_wide(base, D):
     ref = u * rstd * w.double() + b.double()
     tol = U * (64 * (u.abs() * rstd + rstd * step) * w.double().abs() + 2 * b.double().abs())
     close(layer_norm(x.cuda(), D, w.cuda(), b.cuda()), ref, tol, "y")
+
+
+@pytest.mark.parametrize("D", [1, 24, 300])
+def test_pending_negation(D):
+    """The imaginary part of a conjugate is a view of the other sign's memory."""
+    from phoneme_contrast_amd.layers import layer_norm
+    gen = torch.Generator().manual_seed(19)
+    z = torch.randn(5, D, dtype=torch.complex64, generator=gen).cuda()
+    w, b, dy = (t.cuda() for t in inputs(5, D, torch.float32, torch.float32, 20)[1:])
+    views = [(z.conj().imag, w, b, dy), (torch._neg_view(z.real.contiguous()), w, b, dy)]
+    views += [(z.real, torch._neg_view(w), torch._neg_view(b), dy), (z.real, w, b, torch._neg_view(dy))]
+    for args in views:
+        assert any(t.is_neg() for t in args)
+        got, want = [], []
+        for out, src in ((got, args), (want, [torch.neg(torch.neg(t)) for t in args])):
+            leaves = [t.detach().requires_grad_(True) for t in src[:3]]
+            y = layer_norm(leaves[0], D, leaves[1], leaves[2])
+            out += [y.detach(), *torch.autograd.grad(y, leaves, src[3])]
+            with torch.no_grad():
+                out.append(layer_norm(src[0], D, src[1], src[2]))
+        for a, c in zip(got, want):
+            assert torch.equal(a.resolve_neg(), c.resolve_neg())

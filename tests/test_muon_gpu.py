@@ -522,3 +522,18 @@ def test_tiny_eps(rows, cols, eps):
     muon_step(p, g, m, lr=0.1, weight_decay=0.5, eps=eps)
     assert ((p[0].cpu().double() - want).abs() <= 2.0 ** -22 * want.abs()).all()
     assert torch.isfinite(p[1]).all() and not m[0].any()
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 7), (130, 260)])
+def test_pending_negation(rows, cols):
+    """The imaginary part of a conjugate is a view of the other sign's memory."""
+    from phoneme_contrast_amd.optim import muon_step, orthogonalize
+    z = torch.randn(2, rows, cols, dtype=torch.complex64, generator=torch.Generator().manual_seed(1)).cuda()
+    x = z.conj().imag
+    assert x.is_neg() and torch.equal(orthogonalize(x), orthogonalize(torch.neg(z.imag)))
+    n = torch._neg_view(z[0].real.contiguous())
+    assert torch.equal(orthogonalize(n), orthogonalize(-z[0].real))
+    t = [torch.randn(rows, cols, device="cuda") for _ in range(3)]
+    for i in range(3):
+        with pytest.raises(ValueError, match="in memory"):
+            muon_step(*[[n if k == i else t[k]] for k in range(3)], lr=0.1)
