@@ -494,3 +494,20 @@ def test_pending_negation(D):
                 out.append(layer_norm(src[0], D, src[1], src[2]))
         for a, c in zip(got, want):
             assert torch.equal(a.resolve_neg(), c.resolve_neg())
+
+
+def test_column_sums_join_in_64_bits():
+    """db of 4096 x 128 float32 rows: 128 blocks sum 32 rows each in float32 (4 in a lane, 2 lanes, 4 waves), the rest is in
+    64 bits.  Of dy ~ N(0, s^2) a block's sum is about 6 s, in [4 s, 8 s): an addition rounds it by 2^-23 4 s / sqrt(12) =
+    1.4e-7 s rms, the smaller ones before it make that 1.6 times as much, 128 blocks 2.5e-6 s; db is 64 s, so 4e-8 of it,
+    and 3.4e-8 (at most) from its own rounding: 5.3e-8, tested with half as much again.  (Joined in float32: 1.2e-7.)"""
+    from phoneme_contrast_amd.layers import layer_norm
+    off = size = 0.0
+    for seed in range(8):
+        x, w, b, dy = inputs(4096, 128, torch.float32, torch.float32, 100 + seed)
+        leaf = b.cuda().requires_grad_(True)
+        (db,) = torch.autograd.grad(layer_norm(x.cuda(), 128, w.cuda(), leaf), [leaf], dy.cuda())
+        ref = dy.double().sum(0)
+        off += (db.cpu().double() - ref).square().sum().item()
+        size += ref.square().sum().item()
+    assert (off / size) ** 0.5 <= 8e-8
