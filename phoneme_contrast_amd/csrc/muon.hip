@@ -10,7 +10,9 @@
 // the float16 rate.  Each operand is therefore held as two float16 numbers, v S = hi + lo with hi = f16(v S) and
 // lo = f16(v S - hi): 22 bits and the sign of lo, a representation error of 2^-24 as float32's own.  A product is
 // hi hi + hi lo + lo hi, exact in each term and summed in float32 (the dropped lo lo is below 2^-24 of the product):
-// three float16 MFMAs for one of float32, 16 / 3 of its rate at float32's accuracy.  S is a power of two that keeps
+// three float16 MFMAs for one of float32, 16 / 3 of its rate; long sums round more than that (errors of 0.5 to 0.8 of float32
+// arithmetic's from 40 rows on), short ones less (1.7 times its error at 1 x 2000), so matrices of at most 32 rows that one
+// block holds are in float32 (tile_step).  S is a power of two that keeps
 // hi below 2^15 for the largest singular value the coefficients can reach (the caller's interval bound), so nothing
 // overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  A matrix whose norm is
 // far below eps starts far below 1: its S is larger by the power of two that all steps together cannot grow back
@@ -959,7 +961,68 @@ __device__ __forceinline__ void put_across(f16* pl, int d, int rows, int r0, int
     }
 }
 
-template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kernel(NsTable t, NsFirst un, NsArgs q, NsCoef coef) {
+// One step of a matrix whose short side is one tile, in float32 throughout: its sums are short, and the 22 bits of two
+// float16 numbers were most of its error (medians of 40 gradients, times float32 arithmetic's own: 3 x 5 1.7 with planes,
+// 0.8 here; 1 x 50 1.5 and 1.0; 32 x 288 1.1 and 0.9).  It is no slower, as its operands need no splitting and its step two
+// barriers: 9 x 32 21.7 and 17.0 us, 32 x 288 39.7 and 34.3, 32 x 1000 92 and 70.
+// Tiles 0, 1, 16, 17 of X, from the wave's first of n on, are in its registers (the last of them past n are not).
+// A lane holds rows acc_row(k, h) of its column, which are values of K to B X as they stand, and, symmetric, A and B are
+// their own operands; only X X^T takes X through LDS, a tile at a time and the wave's own.
+constexpr int NSB_TILE = 32 * 33;
+template <int T> __device__ __forceinline__ void tile_step(float* lds, f32x16 (&x)[T / 2][2], int n, int waves, int l32, int h,
+                                                           float unit2, float a, float b, float c) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float* own = lds + wave * NSB_TILE;
+    float* all = lds + waves * NSB_TILE;
+    f32x16 g{};
+    if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            if (2 * NSB_WAVES * (i / 2) + i % 2 >= n) continue;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) own[l32 * 33 + acc_row(k, h)] = x[i / 2][i % 2][k];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const float v = own[(2 * k + h) * 33 + l32];
+                g = mfma32(v, v, g);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) own[acc_row(k, h) * 33 + l32] = g[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * 32; i += 64 * NSB_WAVES) {
+        const int at = (i >> 5) * 33 + (i & 31);
+        float s = 0.f;
+        for (int w = 0; w < waves; ++w) s += lds[w * NSB_TILE + at];
+        all[at] = s * unit2;
+    }
+    __syncthreads();
+    if (n <= 0) return;
+    float v[16];
+    f32x16 p{};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = all[l32 * 33 + acc_row(k, h)];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) p = mfma32(v[k], v[k], p);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = fmaf(c, p[k], b * v[k]);
+#pragma unroll
+    for (int i = 0; i < T; ++i) {
+        if (2 * NSB_WAVES * (i / 2) + i % 2 >= n) continue;
+        f32x16 y{};
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y = mfma32(v[k], x[i / 2][i % 2][k], y);
+        x[i / 2][i % 2] = x[i / 2][i % 2] * a + y;
+    }
+}
+
+// kinds of matrices in a launch: short sides of one tile, of more, or some of each (with the code of both, a wave of 4 tiles
+// has too few registers: 64 x 512 78 -> 88 us)
+enum NsKind { NSB_ONE = 1, NSB_MORE = 2, NSB_BOTH = 3 };
+template <int T, int KIND> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kernel(NsTable t, NsFirst un, NsArgs q, NsCoef coef) {
     extern __shared__ __attribute__((aligned(16))) char sm[];
     __shared__ double red[NSB_WAVES + 2];
     const int ei = find_entry(un.first, un.count, blockIdx.x);
@@ -1053,6 +1116,11 @@ template <int T> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_block_kern
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));  // (addresses are formed anew: kept over the steps, they take the registers of X)
         const int l32 = lane & 31, h = lane >> 5;
+        if (KIND == NSB_ONE || (KIND == NSB_BOTH && mb == 1)) {
+            tile_step<T>(reinterpret_cast<float*>(sm), x, tr[0] == 0 ? nb - tc[0] : 0, min(NSB_WAVES, row_pairs), l32, h,
+                         unit * unit, a, b, c);
+            continue;
+        }
         if (step) __syncthreads();  // (X^T and B of the last step are read)
 #pragma unroll
         for (int i = 0; i < T; ++i) {  // X planes: rows of m, K along n
@@ -1266,20 +1334,23 @@ int ns_block_pairs(const NsMat& e) {
 int ns_block_bytes(const NsMat& e) {
     if (std::min(e.rows, e.cols) > 128 || std::max(e.rows, e.cols) > 1024 || ns_block_pairs(e) > 2 * NSB_WAVES) return 0;
     const int64_t mp = round_up(std::min(e.rows, e.cols), 32), np = round_up(std::max(e.rows, e.cols), 32);
-    const int64_t bytes = 4 * (mp * np + (int64_t)mp * mp);
+    int64_t bytes = 4 * (mp * np + (int64_t)mp * mp);
+    if (mp == 32) bytes = std::max<int64_t>(bytes, 4 * NSB_TILE * (std::min(NSB_WAVES, ns_block_pairs(e)) + 1));
     return bytes <= NSB_LDS ? (int)bytes : 0;
 }
 
-// the launch's matrices in blocks of their own: bytes of LDS and pairs of the largest; false if one does not fit
-bool ns_in_blocks(const NsTable& t, int* bytes, int* pairs) {
+// the launch's matrices in blocks of their own: bytes of LDS and pairs of the largest, and their kinds (0: one does not fit)
+int ns_in_blocks(const NsTable& t, int* bytes, int* pairs) {
+    int kind = 0;
     *bytes = *pairs = 0;
     for (int i = 0; i < t.count; ++i) {
         const int b = ns_block_bytes(t.e[i]);
-        if (!b) return false;
+        if (!b) return 0;
         *bytes = std::max(*bytes, b);
         *pairs = std::max(*pairs, ns_block_pairs(t.e[i]));
+        kind |= std::min(t.e[i].rows, t.e[i].cols) <= 32 ? NSB_ONE : NSB_MORE;
     }
-    return true;
+    return kind;
 }
 
 // One launch table's workspace: the job, partial sums and unit of every matrix, counters and partial products of split tiles,
@@ -1351,24 +1422,29 @@ int ns_scales(NsArgs& q, const float* coef, int steps) {
     return PCX_OK;
 }
 
-template <int T> int ns_block_as(const NsTable& t, const NsFirst& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
+template <int T, int KIND> int ns_block_as(const NsTable& t, const NsFirst& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
     if (sm > 64 * 1024)
-        (void)hipFuncSetAttribute((const void*)ns_block_kernel<T>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
-    ns_block_kernel<T><<<n, 64 * NSB_WAVES, sm, s>>>(t, un, q, c);
+        (void)hipFuncSetAttribute((const void*)ns_block_kernel<T, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, sm);
+    ns_block_kernel<T, KIND><<<n, 64 * NSB_WAVES, sm, s>>>(t, un, q, c);
     PCX_LAUNCH_CHECK("ns_block_kernel");
     return PCX_OK;
+}
+template <int T> int ns_block_of(int kind, const NsTable& t, const NsFirst& un, const NsArgs& q, const NsCoef& c, unsigned n, int sm, hipStream_t s) {
+    if (kind == NSB_ONE) return ns_block_as<T, NSB_ONE>(t, un, q, c, n, sm, s);
+    if (kind == NSB_MORE) return ns_block_as<T, NSB_MORE>(t, un, q, c, n, sm, s);
+    return ns_block_as<T, NSB_BOTH>(t, un, q, c, n, sm, s);
 }
 
 int ns_run(const NsTable& t, const NsArgs& q, const float* coef, int steps, hipStream_t s) {
     int most, pairs;
-    if (ns_in_blocks(t, &most, &pairs)) {
+    if (const int kind = ns_in_blocks(t, &most, &pairs)) {
         NsCoef c{};
         c.steps = steps;
         memcpy(c.c, coef, 3 * steps * sizeof(float));
         NsFirst un{};
         const unsigned n = ns_blocks(t, un, [](const NsMat&) { return (int64_t)1; });
-        if (pairs <= NSB_WAVES) return ns_block_as<2>(t, un, q, c, n, most, s);
-        return ns_block_as<4>(t, un, q, c, n, most, s);
+        if (pairs <= NSB_WAVES) return ns_block_of<2>(kind, t, un, q, c, n, most, s);
+        return ns_block_of<4>(kind, t, un, q, c, n, most, s);
     }
     NsJob job{t, q, {}, {}, {}};
     NsPlan plans[4];

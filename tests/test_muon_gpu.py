@@ -537,3 +537,53 @@ def test_pending_negation(rows, cols):
     for i in range(3):
         with pytest.raises(ValueError, match="in memory"):
             muon_step(*[[n if k == i else t[k]] for k in range(3)], lr=0.1)
+
+
+def rms_errors(shapes, run, seeds=40):
+    """Per shape: rms relative errors of `run` (a list of matrices -> theirs orthogonalised) and of the float32 iteration."""
+    own, f32 = [0.0] * len(shapes), [0.0] * len(shapes)
+    for seed in range(seeds):
+        xs = [gradient(r, c, 7 * seed + i) for i, (r, c) in enumerate(shapes)]
+        for i, (x, o) in enumerate(zip(xs, run(xs))):
+            ref = iterate(x.double())
+            own[i] += ((o.cpu().double() - ref).norm() / ref.norm()).item() ** 2
+            f32[i] += ((iterate(x).double() - ref).norm() / ref.norm()).item() ** 2
+    return [((a / seeds) ** 0.5, (b / seeds) ** 0.5) for a, b in zip(own, f32)]
+
+
+SHORT = [(1, 1), (1, 2), (1, 50), (2, 3), (3, 5), (200, 3), (5, 5), (8, 30), (32, 9), (16, 100), (24, 24), (31, 33), (32, 32),
+         (288, 32), (32, 288), (32, 700), (20, 1000)]
+
+
+def by_step(xs):
+    """The same through a step: without momentum, decay or a scale a parameter of 0 becomes minus its gradient's."""
+    from phoneme_contrast_amd.optim import muon_step
+    p = [torch.zeros_like(x, device="cuda") for x in xs]
+    muon_step(p, [x.cuda() for x in xs], [torch.zeros_like(t) for t in p], lr=1.0, momentum=0.0, nesterov=False, adjust=None)
+    return [-t for t in p]
+
+
+def test_short_sides_are_as_exact_as_float32():
+    """Matrices whose short side is one tile are computed in float32 throughout, alone, in batches and in lists that blocks
+    hold: as many roundings as the float32 iteration has, in another order.  Of 40 draws an rms is known to 1 / sqrt(80) =
+    11 %, two to 16 %: half as much again is allowed (operands of 22 bits: 1.9 times at 1 x 50 and 3 x 5)."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    routes = {"alone": lambda xs: [orthogonalize(x.cuda()) for x in xs],
+              "batch": lambda xs: [orthogonalize(torch.stack([x, x]).cuda())[1] for x in xs],
+              "list": lambda xs: by_step(xs[:9]) + by_step(xs[9:]),
+              "mixed list": lambda xs: by_step(xs[:9] + [gradient(64, 64, 1)])[:9] + by_step(xs[9:] + [gradient(96, 300, 1)])[:-1]}
+    for name, run in routes.items():
+        for shape, (own, f32) in zip(SHORT, rms_errors(SHORT, run)):
+            assert own <= 1.5 * f32, (name, shape, own, f32)
+
+
+def test_short_sides_among_the_products():
+    """Behind 1024 values of the long side, or in a list with a matrix that no block holds, operands have 22 bits: twice
+    the float32 iteration's error where sums are short (in the list with the 22 % that two rms of 20 draws may be off)."""
+    from phoneme_contrast_amd.optim import orthogonalize
+    shapes = [(1, 2000), (3, 2000), (20, 1500), (32, 1100)]
+    for shape, (own, f32) in zip(shapes, rms_errors(shapes, lambda xs: [orthogonalize(x.cuda()) for x in xs], 20)):
+        assert own <= 2 * f32, (shape, own, f32)
+    shapes = SHORT[:15]
+    for shape, (own, f32) in zip(shapes, rms_errors(shapes, lambda xs: by_step(xs + [gradient(200, 300, 1)])[:-1], 20)):
+        assert own <= 2.5 * f32, (shape, own, f32)
