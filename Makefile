@@ -60,10 +60,11 @@ $(BUILD)/layernorm.o $(BUILD)/muon.o: CXXFLAGS += -Xclang -target-feature -Xclan
 $(LIB): $(OBJ)
 	$(HIPCC) -shared --offload-arch=$(ARCH) -o $@ $(OBJ)
 
-$(TORCH_LIB): phoneme_contrast_amd/csrc/torch_ops.cpp include/pcx.h $(LIB)
+# (not linked to $(LIB): the process hands it the entry points of the library that it has loaded)
+$(TORCH_LIB): phoneme_contrast_amd/csrc/torch_ops.cpp include/pcx.h
 	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -Iinclude \
 	    -isystem $(TORCH_DIR)/include -isystem $(TORCH_DIR)/include/torch/csrc/api/include -isystem /opt/rocm/include \
-	    $< -o $@ -L$(TORCH_DIR)/lib -ltorch -ltorch_cpu -lc10 -lc10_hip -Lphoneme_contrast_amd -lpcx -Wl,-rpath,'$$ORIGIN'
+	    $< -o $@ -L$(TORCH_DIR)/lib -ltorch -ltorch_cpu -lc10 -lc10_hip
 
 # host-side sanitizer build (no GPU): every source compiled host-only with ASan + UBSan, linked with the
 # plan-builder check tools/plan_check.cpp (tests/test_plan_asan.py runs it)

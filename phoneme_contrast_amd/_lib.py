@@ -162,14 +162,18 @@ def lib():
 
 
 class _TorchOps:
-    """Handles of the torch operators in libpcx_torch.so (csrc/torch_ops.cpp)."""
+    """Handles of the torch operators in libpcx_torch.so (csrc/torch_ops.cpp), which call the entry points of `lib`."""
 
-    def __init__(self):
+    ENTRIES = ("pcx_last_error", "pcx_layernorm_workspace_bytes", "pcx_layernorm_forward", "pcx_layernorm_backward")
+
+    def __init__(self, lib):
         if not os.path.exists(TORCH_OPS_PATH):
             raise RuntimeError(
                 f"phoneme_contrast_amd: native library {TORCH_OPS_PATH} is missing; build it with "
                 "`make` (or __graft_entry__.build()) — there is no CPU fallback")
         torch.ops.load_library(TORCH_OPS_PATH)
+        at = [ctypes.cast(getattr(lib, name), c_void_p) for name in self.ENTRIES]
+        ctypes.CDLL(TORCH_OPS_PATH).pcx_torch_bind((c_void_p * len(at))(*at))
         self.layer_norm = torch.ops.pcx.layer_norm.default
 
 
@@ -180,9 +184,10 @@ def torch_ops():
     """Load libpcx_torch.so once; raise if it is missing (no silent fallback)."""
     global _torch_ops
     if _torch_ops is None:
+        native = lib()
         with _lock:
             if _torch_ops is None:
-                _torch_ops = _TorchOps()
+                _torch_ops = _TorchOps(native)
     return _torch_ops
 
 

@@ -17,6 +17,15 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The C entry points of the library that the process has loaded (linked here, libpcx.so could be a second copy and
+// another build than the one that serves all other calls).
+struct Entries {
+    decltype(&pcx_last_error) last_error;
+    decltype(&pcx_layernorm_workspace_bytes) workspace_bytes;
+    decltype(&pcx_layernorm_forward) layernorm_forward;
+    decltype(&pcx_layernorm_backward) layernorm_backward;
+} pcx;
+
 int dtype_of(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return PCX_F32;
@@ -29,7 +38,7 @@ int dtype_of(const Tensor& t) {
 void check_status(int rc, const char* what) {
     if (rc == PCX_OK) return;
     char msg[512];
-    pcx_last_error(msg, sizeof msg);
+    pcx.last_error(msg, sizeof msg);
     if (rc == PCX_EINVAL || rc == PCX_ESHAPE) TORCH_CHECK_VALUE(false, msg);
     TORCH_CHECK(false, what, " failed (", rc, "): ", msg);
 }
@@ -66,7 +75,7 @@ Tensor forward(const Tensor& x, const Tensor& w, const Tensor& b, int64_t D, dou
     if (stats) *stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
     const int dt = dtype_of(x), wdt = w.defined() ? dtype_of(w) : b.defined() ? dtype_of(b) : dt;
     const c10::DeviceGuard guard(x.device());
-    check_status(pcx_layernorm_forward(dt, wdt, rows, D, xr.const_data_ptr(), xs, address(w), address(b), (float)eps,
+    check_status(pcx.layernorm_forward(dt, wdt, rows, D, xr.const_data_ptr(), xs, address(w), address(b), (float)eps,
                                        y.mutable_data_ptr(), stats ? stats->mutable_data_ptr<float>() : nullptr,
                                        stream_of(x)),
                  "pcx_layernorm_forward");
@@ -130,10 +139,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             auto [dyr, dyrows, dys] = rows_of(grads[0].resolve_neg(), D);
             size_t nws = 0;
             if (need_w || need_b) {
-                nws = pcx_layernorm_workspace_bytes(dt, rows, D);
+                nws = pcx.workspace_bytes(dt, rows, D);
                 if (nws) ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
             }
-            check_status(pcx_layernorm_backward(dt, wdt, rows, D, xr.const_data_ptr(), xs, address(w), (float)eps,
+            check_status(pcx.layernorm_backward(dt, wdt, rows, D, xr.const_data_ptr(), xs, address(w), (float)eps,
                                                 stats.const_data_ptr<float>(), dyr.const_data_ptr(), dys,
                                                 need_x ? dx.mutable_data_ptr() : nullptr,
                                                 need_w ? dw.mutable_data_ptr() : nullptr,
@@ -158,6 +167,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(const Tensor& x, at::IntArrayRef shape, const std::optional<Tensor>& weight,
                   const std::optional<Tensor>& bias, double eps) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    TORCH_CHECK(pcx.layernorm_forward, "layer_norm: phoneme_contrast_amd._lib.torch_ops() has not loaded libpcx.so");
     TORCH_CHECK_VALUE(dtype_of(x) >= 0, "layer_norm: float32, bfloat16 or float16 expected, got ", x.scalar_type());
     const int64_t n = (int64_t)shape.size();
     TORCH_CHECK_VALUE(n >= 1 && x.dim() >= n && x.sizes().slice(x.dim() - n) == shape, "layer_norm: input of shape ", x.sizes(),
@@ -191,6 +201,14 @@ Tensor layer_norm(const Tensor& x, at::IntArrayRef shape, const std::optional<Te
 }
 
 }  // namespace
+
+// addresses of the entry points, in the order of Entries
+extern "C" __attribute__((visibility("default"))) void pcx_torch_bind(void* const* at) {
+    pcx.last_error = reinterpret_cast<decltype(pcx.last_error)>(at[0]);
+    pcx.workspace_bytes = reinterpret_cast<decltype(pcx.workspace_bytes)>(at[1]);
+    pcx.layernorm_forward = reinterpret_cast<decltype(pcx.layernorm_forward)>(at[2]);
+    pcx.layernorm_backward = reinterpret_cast<decltype(pcx.layernorm_backward)>(at[3]);
+}
 
 TORCH_LIBRARY(pcx, m) {
     m.def("layer_norm(Tensor x, int[] shape, Tensor? weight, Tensor? bias, float eps) -> Tensor");

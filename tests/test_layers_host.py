@@ -31,3 +31,34 @@ def test_c_entry_points_refuse_before_any_launch():
     assert bwd(dx=None, dw=None) == _lib.PCX_OK
     assert lib.pcx_layernorm_workspace_bytes(0, 4096, 128) > 0
     assert lib.pcx_layernorm_workspace_bytes(0, 4096, 1 << 20) == 0 and lib.pcx_layernorm_workspace_bytes(9, 4, 8) == 0
+
+
+def test_the_torch_operator_calls_the_library_that_is_loaded(tmp_path):
+    """PCX_LIB_PATH names another build: no second copy of the library comes with the torch operators."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    from phoneme_contrast_amd import _lib
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    here = os.path.join(os.path.dirname(_lib.__file__), "libpcx.so")
+    other = str(tmp_path / "other.so")
+    shutil.copy(here, other)
+    code = ("from phoneme_contrast_amd import _lib; _lib.torch_ops(); "
+            "print(sorted({l.split()[-1] for l in open('/proc/self/maps') if '.so' in l and 'pcx' in l or 'other.so' in l}))")
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, env={**os.environ, "PCX_LIB_PATH": other},
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stderr
+    mapped = out.stdout
+    assert other in mapped and "libpcx_torch.so" in mapped and "libpcx.so" not in mapped, mapped
+
+
+def test_the_torch_operator_alone_says_what_it_lacks():
+    import subprocess
+    import sys
+    from phoneme_contrast_amd import _lib
+    code = (f"import torch; torch.ops.load_library({_lib.TORCH_OPS_PATH!r})\n"
+            "try: torch.ops.pcx.layer_norm(torch.ones(2, 8), (8,), None, None, 1e-5)\n"
+            "except RuntimeError as e: print(e)")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "has not loaded libpcx.so" in out.stdout, out.stdout + out.stderr
