@@ -12,13 +12,18 @@ OBJ = $(patsubst phoneme_contrast_amd/csrc/%.hip,$(BUILD)/%.o,$(SRC))
 HDR = $(wildcard phoneme_contrast_amd/csrc/*.h) include/pcx.h
 LIB ?= phoneme_contrast_amd/libpcx.so
 
-# the torch operators (csrc/torch_ops.cpp) on top of the C ABI, against the installed torch's headers
+# the torch operators (csrc/torch_ops.cpp) on top of the C ABI, against the installed torch's headers; without a torch
+# the C library and the tools are all there is to build
+PYTHON ?= python3
 TORCH_LIB = phoneme_contrast_amd/libpcx_torch.so
-TORCH_DIR := $(shell python3 -c "import importlib.util as u; print(u.find_spec('torch').submodule_search_locations[0])")
+TORCH := $(shell $(PYTHON) -c "import importlib.metadata as m, importlib.util as u; \
+    print(m.version('torch'), u.find_spec('torch').submodule_search_locations[0])" 2>/dev/null)
+TORCH_DIR = $(word 2,$(TORCH))
+TORCH_STAMP = $(BUILD)/torch-$(firstword $(TORCH))
 
 TOOLS = tools/wino_bench tools/ww_bench tools/stem_bench tools/wb_bench tools/ws_bench
 
-all: $(LIB) $(TORCH_LIB) $(TOOLS)
+all: $(LIB) $(TOOLS) $(if $(TORCH),$(TORCH_LIB))
 
 # engine cross-check / micro-benchmark (tests/test_wino_engine_gpu.py runs it)
 tools/wino_bench: tools/wino_bench.cpp $(LIB) $(HDR)
@@ -61,10 +66,16 @@ $(LIB): $(OBJ)
 	$(HIPCC) -shared --offload-arch=$(ARCH) -o $@ $(OBJ)
 
 # (not linked to $(LIB): the process hands it the entry points of the library that it has loaded)
-$(TORCH_LIB): phoneme_contrast_amd/csrc/torch_ops.cpp include/pcx.h
+$(TORCH_LIB): phoneme_contrast_amd/csrc/torch_ops.cpp include/pcx.h $(TORCH_STAMP)
 	$(CXX) -O2 -std=c++17 -fPIC -shared -Wall -D__HIP_PLATFORM_AMD__ -DUSE_ROCM -Iinclude \
 	    -isystem $(TORCH_DIR)/include -isystem $(TORCH_DIR)/include/torch/csrc/api/include -isystem /opt/rocm/include \
 	    $< -o $@ -L$(TORCH_DIR)/lib -ltorch -ltorch_cpu -lc10 -lc10_hip
+
+# (named by torch's version: another one builds anew)
+$(TORCH_STAMP):
+	@mkdir -p $(BUILD)
+	@rm -f $(BUILD)/torch-*
+	@touch $@
 
 # host-side sanitizer build (no GPU): every source compiled host-only with ASan + UBSan, linked with the
 # plan-builder check tools/plan_check.cpp (tests/test_plan_asan.py runs it)

@@ -62,3 +62,27 @@ def test_the_torch_operator_alone_says_what_it_lacks():
             "except RuntimeError as e: print(e)")
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "has not loaded libpcx.so" in out.stdout, out.stdout + out.stderr
+
+
+def test_make_without_torch_and_with_another_one(tmp_path):
+    """The C library needs no torch; libpcx_torch.so is built anew when torch's version is another."""
+    import glob
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    if not shutil.which("make"):
+        pytest.skip("no make")
+
+    def plan(*args):
+        out = subprocess.run(["make", "-n", *args], cwd=root, capture_output=True, text=True, timeout=120)
+        assert out.returncode == 0, out.stderr
+        return out.stdout
+    none = plan("-B", "PYTHON=false", f"BUILD={tmp_path}/obj")
+    assert "adam.hip" in none and "libpcx.so" in none and "torch_ops.cpp" not in none
+    assert "torch_ops.cpp" in plan("-B", f"BUILD={tmp_path}/obj")
+    lib = "phoneme_contrast_amd/libpcx_torch.so"
+    if not (os.path.exists(os.path.join(root, lib)) and glob.glob(os.path.join(root, "build", "torch-*"))):
+        pytest.skip("built elsewhere")
+    assert "torch_ops.cpp" not in plan(lib)
+    assert "torch_ops.cpp" in plan("TORCH=1.0 /somewhere", lib)
