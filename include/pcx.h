@@ -172,8 +172,6 @@ typedef struct pcx_net_config {
     int hidden_dims[4];   /* deep only */
     int use_residual;     /* deep only */
     int conv_bf16;        /* deep only: conv operands rounded to bf16, float32 accumulation (0: fp32) */
-    int proj_norm;        /* norm behind the projection: 0 BatchNorm1d, 1 layer norm (each embedding by itself: no
-                             running statistics in bn_stats, and a training batch of one is allowed) */
 } pcx_net_config;
 
 /* The cnn_deep convolution engine as a standalone op (src/models/phoneme_cnn.py:146-304 convs):
@@ -186,7 +184,10 @@ int pcx_conv2d(int mode, int precision, int B, int cin, int cout, int IH, int IW
                int pad, const float* x, const float* w, const float* dy, float* out, int accumulate, void* ws,
                size_t ws_bytes, hipStream_t stream);
 
+/* pcx_net_create_norm: with the norm behind the projection, 0 BatchNorm1d (as pcx_net_create) or 1 layer norm (each
+ * embedding by itself: no running statistics in bn_stats, and a training batch of one is allowed). */
 void* pcx_net_create(const pcx_net_config* cfg, int64_t B, int64_t F, int64_t T);
+void* pcx_net_create_norm(const pcx_net_config* cfg, int proj_norm, int64_t B, int64_t F, int64_t T);
 void pcx_net_destroy(void* plan);
 size_t pcx_net_workspace_bytes(const void* plan);
 int pcx_net_info(const void* plan, int* nparams, int* nbn, int* ndrop, int* drop_channels);

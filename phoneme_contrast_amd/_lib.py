@@ -44,7 +44,7 @@ class NetConfig(ctypes.Structure):
     _fields_ = [("kind", ctypes.c_int), ("in_channels", ctypes.c_int),
                 ("embedding_dim", ctypes.c_int), ("use_attention", ctypes.c_int),
                 ("hidden_dims", ctypes.c_int * 4), ("use_residual", ctypes.c_int),
-                ("conv_bf16", ctypes.c_int), ("proj_norm", ctypes.c_int)]
+                ("conv_bf16", ctypes.c_int)]
 
 
 class MuonMatrix(ctypes.Structure):
@@ -93,6 +93,7 @@ SIGNATURES = {
     "pcx_adam_segments": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, ctypes.POINTER(Segment), c_int, c_i64, c_float,
                                   c_float, c_float, c_float, c_float, c_float, c_void_p]),
     "pcx_net_create": (c_void_p, [ctypes.POINTER(NetConfig), c_i64, c_i64, c_i64]),
+    "pcx_net_create_norm": (c_void_p, [ctypes.POINTER(NetConfig), c_int, c_i64, c_i64, c_i64]),
     "pcx_net_destroy": (None, [c_void_p]),
     "pcx_net_workspace_bytes": (c_size, [c_void_p]),
     "pcx_net_info": (c_int, [c_void_p, _pi, _pi, _pi, _pi]),

@@ -258,7 +258,7 @@ int build_deep(Plan& p) {
     p.dh = p.carve("dh", (size_t)B * D * 4);
     p.dpooled = p.carve("dpooled", (size_t)B * K * 4);
     p.proj_part = p.carve("proj_part", proj_part_floats(B, D, K) * 4);
-    if (p.cfg.proj_norm) {
+    if (p.proj_norm) {
         p.z = p.carve("z", (size_t)B * D * 4);
         p.lnstat = p.carve("lnstat", (size_t)B * 8);
         p.lnws = p.carve("lnws", layernorm_bwd_ws(B, D, 4));
@@ -272,7 +272,7 @@ int build_deep(Plan& p) {
     if (p.cfg.use_attention) p.stages.push_back(d.ia);
     for (int i = 3; i >= 0; --i) p.stages.push_back(d.blk[i].pidx);
     p.stages.push_back(0);
-    p.nbn = p.cfg.proj_norm ? bnidx : bnidx + 1;
+    p.nbn = p.proj_norm ? bnidx : bnidx + 1;
     p.ndrop = 4;
     for (int i = 0; i < 4; ++i) p.drop_ch[i] = d.h[i];
     p.deep = dp;
@@ -639,7 +639,7 @@ int deep_forward(const Plan& p, const float* const* P, float* const* bnstat, int
         j.bias = P[ip + 1];
         j.gamma = P[ip + 2];
         j.beta = P[ip + 3];
-        if (!p.cfg.proj_norm) {
+        if (!p.proj_norm) {
             j.rmean = bnp(d.bn_proj, 0);
             j.rvar = bnp(d.bn_proj, 1);
             j.nbt = nb(d.bn_proj);

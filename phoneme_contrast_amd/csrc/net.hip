@@ -138,7 +138,7 @@ int build_small(Plan& p) {
     p.dh = p.carve("dh", (size_t)B * D * 4);
     p.dpooled = p.carve("dpooled", (size_t)B * K * 4);
     p.proj_part = p.carve("proj_part", proj_part_floats(B, D, K) * 4);
-    if (p.cfg.proj_norm) {
+    if (p.proj_norm) {
         p.z = p.carve("z", (size_t)B * D * 4);
         p.lnstat = p.carve("lnstat", (size_t)B * 8);
         p.lnws = p.carve("lnws", layernorm_bwd_ws(B, D, 4));
@@ -153,7 +153,7 @@ int build_small(Plan& p) {
     p.stages = {p.cfg.use_attention ? 26 : 24};
     if (p.cfg.use_attention) p.stages.push_back(24);
     for (int l = 6; l >= 1; --l) p.stages.push_back(p_conv_w(l));
-    p.nbn = p.cfg.proj_norm ? 6 : 7;
+    p.nbn = p.proj_norm ? 6 : 7;
     p.ndrop = 3;
     p.drop_ch[0] = 32; p.drop_ch[1] = 64; p.drop_ch[2] = 128;
     return PCX_OK;
@@ -284,7 +284,7 @@ int small_forward(const Plan& p, const float* const* P, float* const* bnstat, in
         j.bias = P[ip + 1];
         j.gamma = P[ip + 2];
         j.beta = P[ip + 3];
-        if (!p.cfg.proj_norm) {
+        if (!p.proj_norm) {
             j.rmean = bnstat[12];
             j.rvar = bnstat[13];
             j.nbt = nbt ? nbt[6] : nullptr;
@@ -541,9 +541,13 @@ int small_backward(const Plan& p, const float* const* P, const float* x, const f
 using pcx::Plan;
 
 extern "C" void* pcx_net_create(const pcx_net_config* cfg, int64_t B, int64_t F, int64_t T) {
+    return pcx_net_create_norm(cfg, 0, B, F, T);
+}
+
+extern "C" void* pcx_net_create_norm(const pcx_net_config* cfg, int proj_norm, int64_t B, int64_t F, int64_t T) {
     using namespace pcx;
     if (!cfg) { set_error("pcx_net_create: NULL config"); return nullptr; }
-    if (cfg->proj_norm != 0 && cfg->proj_norm != 1) { set_error("pcx_net_create: proj_norm %d (0 or 1)", cfg->proj_norm); return nullptr; }
+    if (proj_norm != 0 && proj_norm != 1) { set_error("pcx_net_create: proj_norm %d (0 or 1)", proj_norm); return nullptr; }
     if (cfg->in_channels != 1) { set_error("pcx_net_create: in_channels must be 1 (MFCC input)"); return nullptr; }
     if (B < 1 || F < 1 || T < 1 || B * F * T > ((int64_t)1 << 40)) {
         set_error("pcx_net_create: bad input shape [%lld,1,%lld,%lld]", (long long)B, (long long)F, (long long)T);
@@ -555,6 +559,7 @@ extern "C" void* pcx_net_create(const pcx_net_config* cfg, int64_t B, int64_t F,
     }
     Plan* p = new Plan();
     p->cfg = *cfg;
+    p->proj_norm = proj_norm;
     p->B = (int)B; p->F = (int)F; p->T = (int)T; p->D = cfg->embedding_dim;
     p->total = 256;  // guard: every region has >= 256 readable workspace bytes in front of it (conv_wino X4)
     int rc = PCX_EINVAL;
@@ -606,7 +611,7 @@ extern "C" int pcx_net_forward(const void* plan, const float* const* params, flo
     PCX_CHECK_ARG(plan && params && bn_stats && x && emb && ws, "pcx_net_forward: NULL argument");
     const Plan* p = static_cast<const Plan*>(plan);
     if (ws_bytes < p->total) { set_error("pcx_net_forward: workspace too small"); return PCX_EWORKSPACE; }
-    if (train && p->B < 2 && !p->cfg.proj_norm) {
+    if (train && p->B < 2 && !p->proj_norm) {
         set_error("Expected more than 1 value per channel when training, got input size [1, %d]", p->D);
         return PCX_EINVAL;
     }

@@ -148,6 +148,7 @@ struct DeepPlan;  // deep.hip
 
 struct Plan {
     pcx_net_config cfg;
+    int proj_norm;                   // norm behind the projection: 0 BatchNorm1d, 1 layer norm
     std::shared_ptr<DeepPlan> deep;  // cnn_deep layout (null for cnn_small)
     int B, F, T, D, C6, P6;
     Layer L[7];
@@ -158,7 +159,7 @@ struct Plan {
     size_t dyb;                     // dy of the layer being back-propagated (DMA path)
     size_t wg_part, wg_bytes;       // shared scratch for weight-gradient partials
     size_t proj_part;
-    size_t z, lnstat, lnws;  // cfg.proj_norm: the layer norm's output, row statistics and partial sums
+    size_t z, lnstat, lnws;  // proj_norm: the layer norm's output, row statistics and partial sums
     size_t pooled, att, h, cfp, cfpb, norm, dzp, dh, dpooled, wt, hp_dz, hp_dzx, hp_dwa, hp_dba;
     size_t total;
     std::vector<Region> regions;
@@ -183,9 +184,9 @@ T* at(void* ws, size_t off) {
 }
 
 
-// the layer-norm part of the head's arguments (cfg.proj_norm)
+// the layer-norm part of the head's arguments (proj_norm)
 inline void proj_layer_norm(const Plan& p, ProjArgs& j, void* ws) {
-    if (!p.cfg.proj_norm) return;
+    if (!p.proj_norm) return;
     j.eps = 1e-5f;
     j.z = at<float>(ws, p.z);
     j.lnstat = at<float>(ws, p.lnstat);

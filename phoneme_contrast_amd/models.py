@@ -71,11 +71,11 @@ def _ptr_array(tensors, ctype=ctypes.c_void_p):
 
 
 class _Plan:
-    """Owns one pcx_net plan (host object) for a fixed (config, B, F, T)."""
+    """Owns one pcx_net plan (host object) for a fixed (config, norm behind the projection, B, F, T)."""
 
-    def __init__(self, cfg: "_lib.NetConfig", B: int, F: int, T: int):
+    def __init__(self, cfg: "_lib.NetConfig", proj_norm: int, B: int, F: int, T: int):
         lib = _lib.lib()
-        self.handle = lib.pcx_net_create(ctypes.byref(cfg), B, F, T)
+        self.handle = lib.pcx_net_create_norm(ctypes.byref(cfg), proj_norm, B, F, T)
         if not self.handle:
             raise ValueError(_lib.last_error())
         self.ws_bytes = lib.pcx_net_workspace_bytes(self.handle)
@@ -140,7 +140,7 @@ class _NativeNet(BaseModel):
         key = (B, F, T)
         p = self._plans.get(key)
         if p is None:
-            p = _Plan(self._net_config(), B, F, T)
+            p = _Plan(self._net_config(), 1 if self.projection_norm == "layer" else 0, B, F, T)
             if getattr(self, "_profiling", False):
                 _lib.check(_lib.lib().pcx_net_profile(p.handle, 1), "pcx_net_profile")
                 only = getattr(self, "_profile_only", None)
@@ -342,7 +342,6 @@ class PhonemeNet(_NativeNet):
         cfg.in_channels = self.in_channels
         cfg.embedding_dim = self.embedding_dim
         cfg.use_attention = 1 if self.use_attention else 0
-        cfg.proj_norm = 1 if self.projection_norm == "layer" else 0
         return cfg
 
 
@@ -415,7 +414,6 @@ class PhonemeNetDeep(_NativeNet):
         cfg.in_channels = self.in_channels
         cfg.embedding_dim = self.embedding_dim
         cfg.use_attention = 1 if self.use_attention else 0
-        cfg.proj_norm = 1 if self.projection_norm == "layer" else 0
         for i, d in enumerate(self.hidden_dims[:4]):
             cfg.hidden_dims[i] = d
         cfg.use_residual = 1 if self.use_residual else 0

@@ -86,3 +86,28 @@ def test_make_without_torch_and_with_another_one(tmp_path):
         pytest.skip("built elsewhere")
     assert "torch_ops.cpp" not in plan(lib)
     assert "torch_ops.cpp" in plan("TORCH=1.0 /somewhere", lib)
+
+
+def test_a_config_of_the_older_layout_is_read_to_its_end_alone():
+    """pcx_net_config has no size or version: what lies behind the ten fields a caller may have been built with is not read."""
+    import ctypes
+    from phoneme_contrast_amd import _lib
+    lib = _lib.lib()
+    assert ctypes.sizeof(_lib.NetConfig) == 40
+
+    def plan(behind, norm=None):
+        raw = (ctypes.c_int * 12)(0, 1, 128, 1, 64, 128, 256, 512, 1, 0, behind, behind)
+        cfg = ctypes.cast(raw, ctypes.POINTER(_lib.NetConfig))
+        p = lib.pcx_net_create(cfg, 4, 40, 100) if norm is None else lib.pcx_net_create_norm(cfg, norm, 4, 40, 100)
+        assert p, _lib.last_error()
+        nbn = ctypes.c_int()
+        assert lib.pcx_net_info(p, None, ctypes.byref(nbn), None, None) == _lib.PCX_OK
+        ws = lib.pcx_net_workspace_bytes(p)
+        lib.pcx_net_destroy(p)
+        return nbn.value, ws
+    first = plan(0)
+    assert first[0] == 7 and plan(1) == first and plan(-77) == first and plan(5, norm=0) == first
+    assert plan(0, norm=1)[0] == 6
+    cfg = _lib.NetConfig(0, 1, 128, 1, (64, 128, 256, 512), 1, 0)
+    for norm in (-1, 2):
+        assert not lib.pcx_net_create_norm(ctypes.byref(cfg), norm, 4, 40, 100) and "proj_norm" in _lib.last_error()
