@@ -121,6 +121,7 @@ class _NativeNet(BaseModel):
     dropout masks, autograd glue."""
 
     _kind = None
+    projection_norm = "batch"  # (also of a whole model that was saved before there was a choice)
 
     def __init__(self, config):
         super().__init__(config)

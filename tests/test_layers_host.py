@@ -111,3 +111,12 @@ def test_a_config_of_the_older_layout_is_read_to_its_end_alone():
     cfg = _lib.NetConfig(0, 1, 128, 1, (64, 128, 256, 512), 1, 0)
     for norm in (-1, 2):
         assert not lib.pcx_net_create_norm(ctypes.byref(cfg), norm, 4, 40, 100) and "proj_norm" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kind", ["phoneme_cnn", "phoneme_cnn_deep"])
+def test_a_model_saved_before_the_choice_of_norm(kind):
+    """A whole module unpickled from an older file has no projection_norm of its own."""
+    from phoneme_contrast_amd.models import model_registry
+    m = model_registry.create(kind, {})
+    del m.__dict__["projection_norm"]
+    assert m.projection_norm == "batch" and m._plan(4, 40, 100).nbn == len(m._bn_modules())
