@@ -273,6 +273,7 @@ int build_deep(Plan& p) {
     for (int i = 3; i >= 0; --i) p.stages.push_back(d.blk[i].pidx);
     p.stages.push_back(0);
     p.nbn = p.proj_norm ? bnidx : bnidx + 1;
+    p.least_px = (int64_t)d.blk[3].Ho * d.blk[3].Wo;
     p.ndrop = 4;
     for (int i = 0; i < 4; ++i) p.drop_ch[i] = d.h[i];
     p.deep = dp;

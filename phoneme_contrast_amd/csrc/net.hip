@@ -154,6 +154,7 @@ int build_small(Plan& p) {
     if (p.cfg.use_attention) p.stages.push_back(24);
     for (int l = 6; l >= 1; --l) p.stages.push_back(p_conv_w(l));
     p.nbn = p.proj_norm ? 6 : 7;
+    p.least_px = (int64_t)H5 * W5;
     p.ndrop = 3;
     p.drop_ch[0] = 32; p.drop_ch[1] = 64; p.drop_ch[2] = 128;
     return PCX_OK;
@@ -613,6 +614,11 @@ extern "C" int pcx_net_forward(const void* plan, const float* const* params, flo
     if (ws_bytes < p->total) { set_error("pcx_net_forward: workspace too small"); return PCX_EWORKSPACE; }
     if (train && p->B < 2 && !p->proj_norm) {
         set_error("Expected more than 1 value per channel when training, got input size [1, %d]", p->D);
+        return PCX_EINVAL;
+    }
+    if (train && p->B < 2 && p->least_px < 2) {
+        set_error("Expected more than 1 value per channel when training: one sample of %d x %d leaves the last BatchNorm2d one pixel",
+                  p->F, p->T);
         return PCX_EINVAL;
     }
     if (p->deep) return deep_forward(*p, params, bn_stats, bn_counts, x, dropout, train, emb, ws, stream);

@@ -149,6 +149,7 @@ struct DeepPlan;  // deep.hip
 struct Plan {
     pcx_net_config cfg;
     int proj_norm;                   // norm behind the projection: 0 BatchNorm1d, 1 layer norm
+    int64_t least_px;                // pixels of the smallest plane that a BatchNorm2d sees
     std::shared_ptr<DeepPlan> deep;  // cnn_deep layout (null for cnn_small)
     int B, F, T, D, C6, P6;
     Layer L[7];

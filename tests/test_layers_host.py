@@ -120,3 +120,22 @@ def test_a_model_saved_before_the_choice_of_norm(kind):
     m = model_registry.create(kind, {})
     del m.__dict__["projection_norm"]
     assert m.projection_norm == "batch" and m._plan(4, 40, 100).nbn == len(m._bn_modules())
+
+
+@pytest.mark.parametrize("kind,F,T,fits", [(0, 7, 6, False), (0, 7, 8, True), (0, 40, 4, True), (1, 16, 16, False), (1, 16, 17, True),
+                                           (1, 1, 9, False)])
+def test_one_sample_whose_last_plane_is_one_pixel(kind, F, T, fits):
+    """With the layer norm a training batch of one is allowed, where every BatchNorm2d still sees two values."""
+    import ctypes
+    from phoneme_contrast_amd import _lib
+    lib = _lib.lib()
+    last = (F // 4) * (T // 4) if kind == 0 else ((F + 15) // 16) * ((T + 15) // 16)
+    assert (last > 1) is fits
+    cfg = _lib.NetConfig(kind, 1, 128, 1, (16, 32, 64, 128), 1, 0)
+    p = lib.pcx_net_create_norm(ctypes.byref(cfg), 1, 1, F, T)
+    assert p, _lib.last_error()
+    if not fits:  # (refused before anything is launched)
+        buf = (ctypes.c_void_p * 64)()
+        rc = lib.pcx_net_forward(p, buf, buf, buf, 4096, None, 1, 4096, 4096, lib.pcx_net_workspace_bytes(p), None)
+        assert rc == _lib.PCX_EINVAL and "more than 1 value" in _lib.last_error()
+    lib.pcx_net_destroy(p)
