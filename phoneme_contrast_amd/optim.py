@@ -171,7 +171,8 @@ class FusedAdam(torch.optim.Optimizer):
         return super().state_dict()
 
     def load_state_dict(self, state_dict):
-        if any(("ns_steps" in g) != isinstance(self, FusedMuon) for g in state_dict["param_groups"]):
+        own = isinstance(self, FusedMuon)  # (torch.optim.Muon's groups have ns_steps too)
+        if any(("ns_eps" in g) != own or ("ns_steps" in g) != own for g in state_dict["param_groups"]):
             raise ValueError(f"{type(self).__name__}: this is the state of another optimizer")
         super().load_state_dict(state_dict)
         self._flat = [None] * len(self.param_groups)

@@ -95,3 +95,20 @@ def test_workspaces_off_their_boundary_are_refused():
         assert lib.pcx_orthogonalize(0, 1, 8, 8, BUF, 64, 8, 1, BUF, 1, c, 1e-7, ws, 1 << 30, None) == _lib.PCX_EWORKSPACE
         assert lib.pcx_muon_step(arr, 1, 0.1, 0.9, 1, 0.0, 1.0, 1, c, 1e-7, ws, 1 << 30, None) == _lib.PCX_EWORKSPACE
         assert "boundary" in _lib.last_error()
+
+
+def test_the_state_of_another_muon_is_refused():
+    """torch.optim.Muon's groups have ns_steps, but neither the fields nor the state of FusedMuon's."""
+    from phoneme_contrast_amd.optim import FusedAdam, FusedMuon
+    if not hasattr(torch.optim, "Muon"):
+        pytest.skip("this torch has none")
+
+    def weight():
+        return [torch.nn.Parameter(torch.ones(4, 5))]
+    other = torch.optim.Muon(weight()).state_dict()
+    for opt in (FusedMuon(weight()), FusedAdam(weight())):
+        before = dict(opt.param_groups[0])
+        with pytest.raises(ValueError, match="another optimizer"):
+            opt.load_state_dict(other)
+        assert opt.param_groups[0] == before
+        opt.load_state_dict(opt.state_dict())
