@@ -323,6 +323,7 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
         any_end = max(any_end, end)
         written_end = max(written_end, end) if is_written else written_end
     _muon_launch(mats, len(params), params[0], lr, momentum, nesterov, weight_decay, grad_scale, ns_steps, coef, eps)
+    torch.autograd.graph.increment_version(params + buffers)  # (autograd cannot see the kernels' writes)
 
 
 def _muon_launch(mats, n, at, lr, momentum, nesterov, weight_decay, grad_scale, ns_steps, coef, eps, nws=None):
@@ -439,6 +440,7 @@ class FusedMuon(FusedAdam):
                                                      float(b1), float(b2), float(group["eps"]),
                                                      float(group["weight_decay"]), float(grad_scale),
                                                      _lib.raw_stream(st["flat"])), "pcx_adam_segments")
+            torch.autograd.graph.increment_version(ps)  # (as in muon_step)
         return loss
 
     # ------------------------------------------------------------------ state: momentum_buffer, or Adam's moments

@@ -587,3 +587,28 @@ def test_short_sides_among_the_products():
     shapes = SHORT[:15]
     for shape, (own, f32) in zip(shapes, rms_errors(shapes, lambda xs: by_step(xs + [gradient(200, 300, 1)])[:-1], 20)):
         assert own <= 2.5 * f32, (shape, own, f32)
+
+
+def test_a_graph_that_holds_the_old_weights_is_noticed():
+    """A weight that changes between a forward pass and its backward pass is an error, as with torch's own optimizers."""
+    from phoneme_contrast_amd.optim import FusedMuon, muon_step
+    x = torch.randn(6, 9, device="cuda", requires_grad=True)
+    p, g, m = (torch.randn(8, 9, device="cuda") for _ in range(3))
+    y, z = (x @ p.T).sum(), (x[:, 0] * m[:6, 0]).sum()
+    muon_step([p], [g], [m], lr=0.1)
+    for out in (y, z):
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(out, [x])
+    torch.autograd.grad((x @ p.T).sum(), [x])
+    with torch.inference_mode():  # (such tensors have no version)
+        muon_step([p.clone()], [g], [m.clone()], lr=0.1)
+    model = small_model()
+    opt = FusedMuon(model.parameters())
+    set_grads(model, 0)
+    opt.step()  # (the first step moves the weights into the flat buffer)
+    set_grads(model, 1)
+    ys = [(x[0, 0] * q).sum() for q in model.parameters()]
+    opt.step()
+    for y in ys:
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(y, [x])
