@@ -180,3 +180,33 @@ def test_gradient_buckets_and_global_flat_steps():
     assert torch.linalg.vector_norm(flat).item() <= 1e-3 * 1.001 and norm.item() > 0
     opt.step(flat_grads=[flat])
     assert all(torch.isfinite(p).all() for p in m.parameters())
+
+
+@pytest.mark.parametrize("att", [True, False])
+def test_a_training_embedding_depends_on_no_other_sample(att):
+    """In training the trunk's BatchNorm2d mixes samples; with weights of 0 they hand on their biases, whatever the batch, and
+    the dropout masks tell the samples apart.  The head's embedding of a sample then has the same bits alone and in any
+    batch with the layer norm, and does not with BatchNorm1d.  (The deep network's head is the same code; its last block
+    has no mask behind its last norm.)"""
+    def embed(model, masks, pick, x):
+        for m in model.modules():
+            if isinstance(m, torch.nn.BatchNorm2d):
+                m.weight.data.zero_()
+                m.bias.data.copy_(torch.linspace(0.5, 1.5, m.bias.numel()))
+        model.set_dropout_masks([k[pick] for k in masks])
+        with torch.no_grad():
+            return model(x[pick].cuda())
+    x = torch.randn(9, 1, 40, 100)
+    masks = [(torch.rand(9, c) >= 0.3).float() / 0.7 for c in (32, 64, 128)]
+    layer = build("phoneme_cnn", 128, att, 7).cuda().train()
+    from phoneme_contrast_amd.models import model_registry
+    batch = model_registry.create("phoneme_cnn", {**layer.config, "projection_norm": "batch"})
+    batch.load_state_dict(layer.state_dict(), strict=False)
+    batch = batch.cuda().train()
+    whole, mixed = embed(layer, masks, torch.arange(9), x), embed(batch, masks, torch.arange(9), x)
+    assert (whole[0] - whole[1]).abs().max() > 1e-3  # (the samples do differ)
+    for pick in ([3], [0], [8, 3], [5, 1, 2, 3], [3, 3, 3, 0, 7, 6]):
+        pick = torch.tensor(pick)
+        assert torch.equal(embed(layer, masks, pick, x), whole[pick.cuda()])
+        if len(pick) > 1:
+            assert (embed(batch, masks, pick, x) - mixed[pick.cuda()]).abs().max() > 1e-3
