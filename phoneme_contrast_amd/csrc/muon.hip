@@ -266,8 +266,9 @@ __global__ __launch_bounds__(256) void ns_split_kernel(const void* job) {
     const int ei = find_entry(un.first, un.count, blockIdx.x);
     const NsMat& e = t.e[ei];
     const int tn = e.np / 64, per = (e.mp / 64) * tn;
-    // (adjacent tiles to one XCD, as in the products: the lines they share are whole in one L2; 16.7 -> 14.3 us of
-    // 6 x 1000 x 333 bfloat16 values)
+    // (adjacent tiles to one XCD, as in the products: rows off line boundaries share lines, whole in one L2.  us of this pass
+    // in turn / so, three runs each: 6 x 1000 x 333 bfloat16 16.6 / 14.1, 333 x 1000 11.0 / 10.9; where rows are whole
+    // lines it costs: 512 x 4608 float32 10.0 / 11.2, 4096 x 4096 bfloat16 35.3 / 36.4)
     const int rel = xcd_order(blockIdx.x - un.first[ei], per * e.batch), bat = rel / per, tl = rel % per;
     const int i0 = (tl / tn) * 64, j0 = (tl % tn) * 64;  // of X (m x n)
     const Planes P = planes_of(q, e, bat);
@@ -965,7 +966,7 @@ __device__ __forceinline__ void put_across(f16* pl, int d, int rows, int r0, int
 // float16 numbers were most of its error (medians of 40 gradients, times float32 arithmetic's own: 3 x 5 1.7 with planes,
 // 0.8 here; 1 x 50 1.5 and 1.0; 32 x 288 1.1 and 0.9).  It is no slower, as its operands need no splitting and its step two
 // barriers: 9 x 32 21.7 and 17.0 us, 32 x 288 39.7 and 34.3, 32 x 1000 92 and 70.
-// Tiles 0, 1, 16, 17 of X, from the wave's first of n on, are in its registers (the last of them past n are not).
+// `n`: tiles of X from the wave's first on; it has numbers 0, 1, 16 and 17 of them, as far as they exist.
 // A lane holds rows acc_row(k, h) of its column, which are values of K to B X as they stand, and, symmetric, A and B are
 // their own operands; only X X^T takes X through LDS, a tile at a time and the wave's own.
 constexpr int NSB_TILE = 32 * 33;
