@@ -51,7 +51,8 @@ struct LnArgs {
     int64_t dys;
     void* dx;                    // NULL: not wanted
     bool cols;                   // dw, db wanted
-    float* part;                 // [blocks][2][D] partial dw, db; NULL: one block, which writes them itself
+    void* part;                  // [blocks][2][D] partial dw, db, in 64 bits for narrow rows, else in 32; NULL: one block,
+                                 // which writes them itself
     void* dw;
     void* db;
 };
@@ -111,11 +112,12 @@ template <int V> struct Place {
 };
 
 // a block's sum of column d (pass 0: dw, 1: db)
-template <typename T> __device__ __forceinline__ void put_column(const LnArgs& a, int pass, int d, float v) {
+template <typename T, typename P> __device__ __forceinline__ void put_column(const LnArgs& a, int pass, int d, P sum) {
     if (a.part) {
-        a.part[((int64_t)blockIdx.x * 2 + pass) * a.D + d] = v;
+        static_cast<P*>(a.part)[((int64_t)blockIdx.x * 2 + pass) * a.D + d] = sum;
         return;
     }
+    const float v = (float)sum;
     void* out = pass ? a.db : a.dw;
     if (!out) return;
     if (a.cf32) static_cast<float*>(out)[d] = v;
@@ -466,8 +468,8 @@ template <typename T, bool BWD> __global__ __launch_bounds__(256) void ln_narrow
             if ((threadIdx.x & 63) < (unsigned)tpr && in) cols[threadIdx.x >> 6][d] = t;
             __syncthreads();
             if (threadIdx.x < (unsigned)a.D)
-                put_column<T>(a, pass, threadIdx.x, (float)((cols[0][threadIdx.x] + cols[1][threadIdx.x]) +
-                                                            (cols[2][threadIdx.x] + cols[3][threadIdx.x])));
+                put_column<T>(a, pass, threadIdx.x, (cols[0][threadIdx.x] + cols[1][threadIdx.x]) +
+                                                        (cols[2][threadIdx.x] + cols[3][threadIdx.x]));
             __syncthreads();
         }
     }
@@ -522,15 +524,15 @@ template <typename T> __global__ __launch_bounds__(256) void ln_long_cols_kernel
         sb += g;
         sw = fmaf(g, ((float)static_cast<const T*>(a.x)[r * a.xs + d] - st.x) * st.y, sw);
     }
-    float* pw = a.part + (int64_t)blockIdx.y * 2 * a.D;
+    float* pw = static_cast<float*>(a.part) + (int64_t)blockIdx.y * 2 * a.D;
     pw[d] = sw;
     pw[a.D + d] = sb;
 }
 
-// dw, db from the blocks' partials: 32 columns x 32 slices of blocks per thread block, summed in slice order, in 64 bits (in 32 they
-// were the larger part of the error: dw and db of 4096 x 128 1.2 times a cascaded sum's, up to 1.5)
-template <typename T> __global__ __launch_bounds__(1024) void ln_cols_kernel(const float* __restrict__ part, int nblk, int D,
-                                                                            T* __restrict__ dw, T* __restrict__ db) {
+// dw, db from the blocks' partials: 32 columns x 32 slices of blocks per thread block, summed in slice order, in 64 bits (in
+// 32 they were the larger part of the error: dw and db of 4096 x 128 1.2 times a cascaded sum's, up to 1.5)
+template <typename T, typename P> __global__ __launch_bounds__(1024) void ln_cols_kernel(const P* __restrict__ part, int nblk, int D,
+                                                                                         T* __restrict__ dw, T* __restrict__ db) {
     __shared__ double red[32][33];
     const int c = threadIdx.x & 31, sl = threadIdx.x >> 5;
     const int64_t col = (int64_t)blockIdx.x * 32 + c;  // of 2 D
@@ -664,7 +666,7 @@ int ln_dtype_size(int dtype) { return dtype == PCX_F32 ? 4 : dtype == PCX_BF16 |
 size_t layernorm_bwd_ws(int64_t rows, int D, int es) {
     if (rows <= 0 || D <= 0) return 0;
     const int n = ln_bwd_blocks(rows, D, 16 / es);
-    return n > 1 || D > LN_ALONE ? (size_t)n * 2 * D * sizeof(float) : 0;
+    return n > 1 || D > LN_ALONE ? (size_t)n * 2 * D * (D <= LN_NARROW ? sizeof(double) : sizeof(float)) : 0;
 }
 
 LnArgs ln_args(const LayerNormArgs& q) {
@@ -699,16 +701,19 @@ int launch_layernorm_bwd(const LayerNormArgs& q, hipStream_t s) {
     a.db = q.db;
     a.cf32 = q.wdtype == PCX_F32;
     const int blocks = ln_bwd_blocks(a.rows, a.D, 16 / ln_dtype_size(q.dtype));
-    if (blocks > 1 || a.D > LN_ALONE) a.part = static_cast<float*>(q.ws);
+    if (blocks > 1 || a.D > LN_ALONE) a.part = q.ws;
     const int rc = ln_any<true>(a, q.dtype, blocks, s);
     if (rc || !a.cols || !a.part) return rc;
     const int cb = ceil_div(2 * (int64_t)a.D, 32);
-    if (q.wdtype == PCX_F32)
-        ln_cols_kernel<float><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<float*>(q.dw), static_cast<float*>(q.db));
-    else if (q.wdtype == PCX_BF16)
-        ln_cols_kernel<bf16><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<bf16*>(q.dw), static_cast<bf16*>(q.db));
-    else
-        ln_cols_kernel<f16><<<cb, 1024, 0, s>>>(a.part, blocks, a.D, static_cast<f16*>(q.dw), static_cast<f16*>(q.db));
+    const auto join = [&](auto kind) {
+        using T = decltype(kind);
+        T *dw = static_cast<T*>(q.dw), *db = static_cast<T*>(q.db);
+        if (a.D <= LN_NARROW) ln_cols_kernel<T, double><<<cb, 1024, 0, s>>>(static_cast<const double*>(a.part), blocks, a.D, dw, db);
+        else ln_cols_kernel<T, float><<<cb, 1024, 0, s>>>(static_cast<const float*>(a.part), blocks, a.D, dw, db);
+    };
+    if (q.wdtype == PCX_F32) join(float());
+    else if (q.wdtype == PCX_BF16) join(bf16());
+    else join(f16());
     PCX_LAUNCH_CHECK("ln_cols_kernel");
     return PCX_OK;
 }

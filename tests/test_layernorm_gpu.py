@@ -511,3 +511,18 @@ def test_column_sums_join_in_64_bits():
         off += (db.cpu().double() - ref).square().sum().item()
         size += ref.square().sum().item()
     assert (off / size) ** 0.5 <= 8e-8
+
+
+@pytest.mark.parametrize("D", [1, 2, 7, 32])
+def test_narrow_rows_sum_their_columns_in_64_bits(D):
+    """dw and db of rows of up to 32 values are rounded once, also where the sums of many blocks cancel: every block's dy is
+    followed by almost its negative.  40000 additions in 64 bits are off by 2^-37 of the sum of the terms' sizes at most."""
+    from phoneme_contrast_amd.layers import layer_norm
+    x, w, b, dy = inputs(20000, D, torch.float32, torch.float32, 30)
+    x, dy = torch.cat([x, x]), torch.cat([dy, -dy * (1 + 2.0 ** -14)])
+    leaves = [t.cuda().requires_grad_(True) for t in (w, b)]
+    got = torch.autograd.grad(layer_norm(x.cuda(), D, *leaves), leaves, dy.cuda())
+    ref, _ = reference(x, w, b, dy, 1e-5)
+    xh = (ref[0] - b.double()) / w.double()
+    for g, r, size in zip(got, ref[2:], ((dy.double() * xh).abs().sum(0), dy.double().abs().sum(0))):
+        close(g, r, 2.0 ** -37 * size + 2.0 ** -45 * dy.double().abs().sum(0), "columns")
