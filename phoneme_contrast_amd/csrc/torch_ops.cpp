@@ -66,6 +66,9 @@ std::tuple<Tensor, int64_t, int64_t> rows_of(const Tensor& t, int64_t D) {
     return {t, rows, rows > 1 ? step : D};
 }
 
+// a view whose negation is pending, as the imaginary part of a conjugate, written out: the kernels read memory
+Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
@@ -136,7 +139,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
             if (need_w) dw.zero_();
             if (need_b) db.zero_();
         } else {
-            auto [dyr, dyrows, dys] = rows_of(grads[0].resolve_neg(), D);
+            auto [dyr, dyrows, dys] = rows_of(in_memory(grads[0]), D);
             size_t nws = 0;
             if (need_w || need_b) {
                 nws = pcx.workspace_bytes(dt, rows, D);
@@ -190,11 +193,10 @@ Tensor layer_norm(const Tensor& x, at::IntArrayRef shape, const std::optional<Te
     TORCH_CHECK(x.is_cuda(), "layer_norm: tensors must live on a ROCm GPU (got device '", x.device(), "')");
     for (const Tensor* t : {&x, &w, &b})  // (a tensor outside of a forward-mode level has none)
         TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), "layer_norm: no forward-mode derivative");
-    // (a view whose negation is pending, as the imaginary part of a conjugate, is written out: the kernels read memory)
-    const Tensor xr = x.resolve_neg();
+    const Tensor xr = in_memory(x);
     std::optional<Tensor> wc, bc;
-    if (w.defined()) wc = w.resolve_neg().contiguous();
-    if (b.defined()) bc = b.resolve_neg().contiguous();
+    if (w.defined()) wc = in_memory(w).contiguous();
+    if (b.defined()) bc = in_memory(b).contiguous();
     if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad())))
         return LayerNorm::apply(xr, wc, bc, D, eps);
     return forward(xr, wc.value_or(Tensor()), bc.value_or(Tensor()), D, eps, nullptr);

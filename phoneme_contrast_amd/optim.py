@@ -298,20 +298,21 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
     _update_scale(adjust, 1, 1)
     if not params:
         return
+    _lib.require_gpu(params[0], what="muon_step")
     dev = params[0].device
     mats = (_lib.MuonMatrix * len(params))()
     spans = []
     for i, (p, g, m) in enumerate(zip(params, grads, buffers)):
-        _lib.require_gpu(p, g, m, what="muon_step")
         if p.dim() < 2 or p.numel() == 0:
             raise ValueError(f"muon_step: parameter {i} of shape {tuple(p.shape)} is no matrix")
         for name, t in (("parameter", p), ("gradient", g), ("momentum buffer", m)):
+            if t.device != dev:
+                _lib.require_gpu(t, what="muon_step")
+                raise RuntimeError(f"muon_step: {name} {i} is on {t.device}, parameter 0 on {dev}")
             if t.shape != p.shape:
                 raise ValueError(f"muon_step: {name} {i} has shape {tuple(t.shape)}, {tuple(p.shape)} expected")
             if t.dtype != torch.float32 or not t.is_contiguous() or t.is_neg():
                 raise ValueError(f"muon_step: {name} {i} must be contiguous float32 in memory")
-            if t.device != dev:
-                raise RuntimeError(f"muon_step: {name} {i} is on {t.device}, parameter 0 on {dev}")
             spans.append((t.data_ptr(), t.data_ptr() + 4 * t.numel(), name != "gradient"))
         rows, cols = _matrix_shape(p)
         e = mats[i]
