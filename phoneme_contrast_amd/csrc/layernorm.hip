@@ -13,10 +13,12 @@
 // xhat = (d - e) rstd; where e^2 makes up more than a quarter of sum d^2 / D (the subtraction would cancel), m moves to
 // m + e first, which the row does at most twice.  A constant row gives the bias, whatever its value.  The statistics keep
 // m + e rounded to float32: the backward's xhat is off by rstd times half a step of the mean.
-// Measured: 8192 x 5120 in float16 forward 33.3 us, 5.0 TB/s (29.9 by the kernel's own clock, where a copy's 5.86 TB/s
-// would take 28.6); 16384 x 4096 in bfloat16 with its gradients 139 us, 4.8 TB/s (forward 49, backward 84 and 6).  Rows of
-// 4097 values, none of them aligned: bfloat16 forward 51 us, float32 100, with gradients 181 and 252.
-// Few rows are latency: 24 x 128 with its gradients 8 us in two kernels, under 60 us of the host's way through autograd.
+// Measured: 8192 x 5120 in float16 forward 34 us a call, 4.9 TB/s (29.7 by the kernel's own clock, where a copy's 5.86 TB/s
+// would take 28.6); 16384 x 4096 in bfloat16 with its gradients 140 us, 4.8 TB/s (forward 50, backward 85 and 6).  Rows of
+// 4097 values, none of them aligned: bfloat16 forward 60 us, float32 92, with gradients 181 and 248.  12000 values: 8192
+// rows of bfloat16 with gradients 226 us.  Behind 16384 values nothing is kept from one pass to the next: 4096 x 32768
+// bfloat16 forward 122 us (92 at a copy's rate), with gradients 562 (229).
+// Few rows are latency: 24 x 128 with its gradients 7 us in two kernels, 35 to 65 us of the host's way through autograd.
 //
 // A row belongs to 1 ... 64 lanes of a wave or to a block of just the waves it needs: sub-wave rows need no barrier, and
 // wider ones one barrier per reduction.  Rows of up to 32 values are computed in 64 bits from x itself: at D = 2 the three
@@ -558,8 +560,8 @@ struct LnPick {
 
 // Rows within a wave up to 64 lanes of 16 values; behind that a block per row, of as many waves as leave 8 values to a
 // thread while that is up to 1024 threads, 16 up to 1024, then 32.  The forward in 16 bits goes on with 16 values behind 512
-// threads, fewer waves to meet: 16384 rows of 5120 bfloat16 values 64 us, 69 with 8 a thread; its backward has no registers
-// to keep twice the sums and the next row: 163 us with 16, 105 with 8 (float32 alike: 4100 values 318 and 158).
+// threads, fewer waves to meet: 16384 rows of 5120 bfloat16 values 63 us, 77 with 8 a thread; its backward has no registers
+// to keep twice the sums and the next row: 114 us with 16, 98 with 8 (float32 alike: 4100 values 161 and 146).
 LnPick ln_pick(int D, int V, bool bwd) {
     if (D <= 64 * V) {
         LnPick p{64, V, false};
@@ -592,8 +594,8 @@ int ln_even(int64_t passes, int64_t most) {
 
 // The forward keeps 1536 threads of a CU busy.  The backward's partial sums are 8 D bytes per block, written and read
 // once, next to the rows' own 3 tensors: two blocks a CU, one from 513 threads on, and no block with fewer than 4 passes
-// (kernels of 1003 x 1537 in bfloat16 with its gradients 23.8 us with 8, 20.9 with 4, 24.6 with 2; 4096 x 128 in float32
-// 17.7, 14.8, 15.1).  us with 1 / 2 / 3 / 4 blocks a CU, 256 threads each: 65536 x 128 float32 33.3 / 27.8 / 28.0 / 30.0,
+// (backward of 1003 x 1537 in bfloat16 with 8, 4 and 2: 12.8, 12.8 and 17.5 us; 4096 x 128 in float32 10.1, 9.0 and 9.3).
+// us with 1 / 2 / 3 / 4 blocks a CU, 256 threads each: 65536 x 128 float32 33.3 / 27.8 / 28.0 / 30.0,
 // 65536 x 512 80.6 / 82.6 / 86.0 / 89.6, 131072 x 256 112 / 81 / 83 / 87, 262144 x 128 bfloat16 59 / 46 / 45 / 47.
 int ln_fwd_blocks(int64_t rows, int D, int V) {
     const int64_t rpb = ln_rows_per_block(D, V, false), passes = (rows + rpb - 1) / rpb;
