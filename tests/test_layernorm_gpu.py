@@ -526,3 +526,31 @@ def test_narrow_rows_sum_their_columns_in_64_bits(D):
     xh = (ref[0] - b.double()) / w.double()
     for g, r, size in zip(got, ref[2:], ((dy.double() * xh).abs().sum(0), dy.double().abs().sum(0))):
         close(g, r, 2.0 ** -37 * size + 2.0 ** -45 * dy.double().abs().sum(0), "columns")
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [20, 33, 40, 100, 128, 250, 513, 1025, 5000, 20001])
+def test_a_row_has_the_same_bits_among_any_others(D, t):
+    """Rows of one wave take different numbers of turns about their means: constant ones, far ones, not finite ones."""
+    from phoneme_contrast_amd.layers import layer_norm
+    gen = torch.Generator().manual_seed(D)
+    rows = torch.randn(24, D, generator=gen)
+    rows[1], rows[5], rows[9] = 60000.0, -0.1, 3e37
+    rows[2] = 16384 + torch.randint(0, 2, (D,), generator=gen)
+    rows[6, 0], rows[7, D // 2] = float("nan"), float("inf")
+    rows[11] *= 1e-30
+    rows[13] = 1e6 + rows[13]
+    x = rows.to(TYPES[t]).cuda()
+    w, b = torch.randn(D, generator=gen).cuda(), torch.randn(D, generator=gen).cuda()
+    dy = torch.randn(24, D, generator=gen).to(TYPES[t]).cuda()
+
+    def go(pick):
+        leaf = x[pick].requires_grad_(True)
+        y = layer_norm(leaf, D, w, b)
+        return y.detach(), torch.autograd.grad(y, leaf, dy[pick])[0]
+    whole = go(torch.arange(24))
+    for pick in (torch.randperm(24, generator=gen), torch.arange(24)[::2], *(torch.tensor([i]) for i in range(24))):
+        for a, c in zip(go(pick), whole):
+            assert torch.equal(torch.nan_to_num(a, 7.0), torch.nan_to_num(c[pick.cuda()], 7.0)), pick
+    ok = [i for i in range(24) if i not in (6, 7)]
+    assert all(torch.isfinite(v[ok]).all() for v in whole) and torch.isnan(whole[0][[6, 7]]).all()
