@@ -10,9 +10,10 @@
 // the float16 rate.  Each operand is therefore held as two float16 numbers, v S = hi + lo with hi = f16(v S) and
 // lo = f16(v S - hi): 22 bits and the sign of lo, a representation error of 2^-24 as float32's own.  A product is
 // hi hi + hi lo + lo hi, exact in each term and summed in float32 (the dropped lo lo is below 2^-24 of the product):
-// three float16 MFMAs for one of float32, 16 / 3 of its rate; long sums round more than that (errors of 0.5 to 0.8 of float32
-// arithmetic's from 40 rows on), short ones less (1.7 times its error at 1 x 2000), so matrices of at most 32 rows that one
-// block holds are in float32 (tile_step).  S is a power of two that keeps
+// three float16 MFMAs for one of float32, 16 / 3 of its rate.  Long sums round more than that (errors of 0.5 to 0.8 of
+// float32 arithmetic's from 40 rows on), short ones less (1.9 times its error at 1 x 50), so matrices of at most 32 rows are
+// in float32: tile_step in one block, ns_long_kernel in many.  (In a list with a matrix that is neither short nor held by a
+// block they go by the planes too: launches of their own would add 7 to its 17.)  S is a power of two that keeps
 // hi below 2^15 for the largest singular value the coefficients can reach (the caller's interval bound), so nothing
 // overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  A matrix whose norm is
 // far below eps starts far below 1: its S is larger by the power of two that all steps together cannot grow back
@@ -99,6 +100,7 @@ struct NsArgs {
     unsigned* done;              // [split tiles] parts that have been written
     float* joint;                // [split tiles][parts][tile] their sums
     int ndone;
+    int slices;                  // long matrices of one tile's rows: blocks of their launches
     int dtype;                   // orthogonalize: type of x and out
     int is_step, nesterov;
     float mu, gs, decay;         // momentum, gradient scale, 1 - lr wd
@@ -125,6 +127,11 @@ struct NsStep {
     float a, b, c;
     int src;                     // which X buffer it reads
 };
+
+// slices of a matrix of `tiles` tiles of 32 columns (ns_long_kernel): of 16 tiles, two to a wave, at most 256 of them
+__host__ __device__ inline int long_slices(int tiles) {
+    return tiles >= 256 * 16 ? 256 : (tiles + 15) / 16;
+}
 
 // planes of one matrix, in float16 numbers from its workspace: X hi, lo, X^T hi, lo (two buffers), A hi, lo, B hi, lo
 struct Planes {
@@ -970,6 +977,35 @@ __device__ __forceinline__ void put_across(f16* pl, int d, int rows, int r0, int
 // A lane holds rows acc_row(k, h) of its column, which are values of K to B X as they stand, and, symmetric, A and B are
 // their own operands; only X X^T takes X through LDS, a tile at a time and the wave's own.
 constexpr int NSB_TILE = 32 * 33;
+// g += x x^T, through the wave's own tile in LDS
+__device__ __forceinline__ void tile_gram(float* own, const f32x16& x, int l32, int h, f32x16& g) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) own[l32 * 33 + acc_row(k, h)] = x[k];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const float v = own[(2 * k + h) * 33 + l32];
+        g = mfma32(v, v, g);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+// B = b A + c A A as an operand, from A in LDS
+__device__ __forceinline__ void tile_poly(const float* A, int l32, int h, float b, float c, float (&v)[16]) {
+    f32x16 p{};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = A[l32 * 33 + acc_row(k, h)];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) p = mfma32(v[k], v[k], p);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = fmaf(c, p[k], b * v[k]);
+}
+// a x + B x
+__device__ __forceinline__ f32x16 tile_apply(const float (&v)[16], const f32x16& x, float a) {
+    f32x16 y{};
+#pragma unroll
+    for (int k = 0; k < 16; ++k) y = mfma32(v[k], x[k], y);
+    return x * a + y;
+}
 template <int T> __device__ __forceinline__ void tile_step(float* lds, f32x16 (&x)[T / 2][2], int n, int waves, int l32, int h,
                                                            float unit2, float a, float b, float c) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -979,16 +1015,7 @@ template <int T> __device__ __forceinline__ void tile_step(float* lds, f32x16 (&
     if (n > 0) {
 #pragma unroll
         for (int i = 0; i < T; ++i) {
-            if (2 * NSB_WAVES * (i / 2) + i % 2 >= n) continue;
-#pragma unroll
-            for (int k = 0; k < 16; ++k) own[l32 * 33 + acc_row(k, h)] = x[i / 2][i % 2][k];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float v = own[(2 * k + h) * 33 + l32];
-                g = mfma32(v, v, g);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (2 * NSB_WAVES * (i / 2) + i % 2 < n) tile_gram(own, x[i / 2][i % 2], l32, h, g);
         }
 #pragma unroll
         for (int k = 0; k < 16; ++k) own[acc_row(k, h) * 33 + l32] = g[k];
@@ -1003,21 +1030,10 @@ template <int T> __device__ __forceinline__ void tile_step(float* lds, f32x16 (&
     __syncthreads();
     if (n <= 0) return;
     float v[16];
-    f32x16 p{};
+    tile_poly(all, l32, h, b, c, v);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = all[l32 * 33 + acc_row(k, h)];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) p = mfma32(v[k], v[k], p);
-#pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = fmaf(c, p[k], b * v[k]);
-#pragma unroll
-    for (int i = 0; i < T; ++i) {
-        if (2 * NSB_WAVES * (i / 2) + i % 2 >= n) continue;
-        f32x16 y{};
-#pragma unroll
-        for (int k = 0; k < 16; ++k) y = mfma32(v[k], x[i / 2][i % 2][k], y);
-        x[i / 2][i % 2] = x[i / 2][i % 2] * a + y;
-    }
+    for (int i = 0; i < T; ++i)
+        if (2 * NSB_WAVES * (i / 2) + i % 2 < n) x[i / 2][i % 2] = tile_apply(v, x[i / 2][i % 2], a);
 }
 
 // kinds of matrices in a launch: short sides of one tile, of more, or some of each (with the code of both, a wave of 4 tiles
@@ -1198,6 +1214,129 @@ template <int T, int KIND> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_
     else finish(f16(), Plain<f16>());
 }
 
+// ---------------------------------------------------------------- long matrices of at most 32 rows
+// The same steps in float32 where the long side has more than a block's registers: X lies in memory, in tiles of 32 columns
+// as the registers hold them, a block works on a slice of its tiles, and a launch per step takes A from the slices' sums
+// of the last one (two sets of them, in turn) and leaves its own: X is read and written once a step, and A, B cost every
+// block 32 MFMAs.  Launches: the norm, X with its first sums, and one a step.  As products of planes 22 bits were most of the
+// error, and 17 launches most of the time: 4 x 3999 1.7e-6 and 100 us, 0.6e-6 and 54 us so; 1 x 2000 0.66e-6 and 89 us, 0.44e-6
+// and 57; 32 x 1100 78 and 51 us, 32 x 8192 116 and 60, 32 x 2^20 5.1 and 0.46 ms (1.74 GB move: 3.8 TB/s).
+enum NsLong { NSL_FIRST, NSL_STEP, NSL_LAST };
+
+template <int PHASE> __global__ __launch_bounds__(64 * NSB_WAVES) void ns_long_kernel(const void* job, NsStep st) {
+    const NsTable& t = job_at(job).t;
+    const NsArgs& q = job_at(job).q;
+    const NsFirst& un = job_at(job).split;
+    __shared__ float lds[(NSB_WAVES + 1) * NSB_TILE];
+    __shared__ double red[NSB_WAVES];
+    const int ei = find_entry(un.first, un.count, blockIdx.x);
+    const NsMat& e = t.e[ei];
+    const bool tall = e.rows > e.cols;
+    const int m = tall ? e.cols : e.rows, n = tall ? e.rows : e.cols, tiles = (n + 31) / 32;
+    const int slices = long_slices(tiles), rel = blockIdx.x - un.first[ei], bat = rel / slices, slice = rel - bat * slices;
+    const int each = (tiles + slices - 1) / slices, t0 = slice * each, t1 = min(t0 + each, tiles);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+    float* X = reinterpret_cast<float*>(q.ws + e.ws) + (int64_t)bat * tiles * 1024 + (threadIdx.x & 63) * 4;
+    float* own = lds + wave * NSB_TILE;
+    float* all = lds + NSB_WAVES * NSB_TILE;
+    const auto sums = [&](int set) { return q.joint + ((int64_t)set * q.slices + blockIdx.x) * 1024; };
+    float v[16];
+    double scale = 0.;
+    float unit = 1.f;
+    if (PHASE == NSL_FIRST) {
+        double s = 0.;
+        for (int i = threadIdx.x; i < e.parts; i += 64 * NSB_WAVES) s += q.part[(int64_t)(e.mat + bat) * NS_PART + i];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if ((threadIdx.x & 63) == 0) red[wave] = s;
+        __syncthreads();
+        s = 0.;
+#pragma unroll
+        for (int w = 0; w < NSB_WAVES; ++w) s += red[w];
+        const double norm = sqrt(s), inv = 1. / (norm + (double)q.eps);
+        const int k = ns_scale(norm * inv, q.growth);
+        scale = ldexp(inv, k);
+        if (slice == 0 && threadIdx.x == 0) q.unit[e.mat + bat] = ldexpf(1.f, -k);
+    } else {
+        unit = q.unit[e.mat + bat];
+        const float* from = sums(st.src) - (int64_t)slice * 1024;
+        for (int i = threadIdx.x; i < 1024; i += 64 * NSB_WAVES) {
+            float s = 0.f;
+#pragma unroll 8
+            for (int w = 0; w < slices; ++w) s += from[w * 1024 + i];
+            all[(i >> 5) * 33 + (i & 31)] = s * unit * unit;
+        }
+        __syncthreads();
+        tile_poly(all, l32, h, st.b, st.c, v);
+    }
+    f32x16 g{};
+    for (int at = t0 + wave; at < t1; at += NSB_WAVES) {
+        const int c = 32 * at + l32;
+        f32x16 x;
+        float* to = X + (int64_t)at * 1024;
+        if (PHASE == NSL_FIRST) {
+            const auto fetch = [&](auto kind) {
+                const auto* src = static_cast<const decltype(kind)*>(e.x) + bat * e.xb;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int r = acc_row(k, h), row = tall ? c : r, col = tall ? r : c;
+                    float u = 0.f;
+                    if (r < m && c < n) {
+                        u = (float)src[row * e.xr + col * e.xc];
+                        if (q.is_step) u = nesterov_u(q, u, e.mom[(int64_t)row * e.cols + col]);
+                    }
+                    x[k] = (float)(u * scale);
+                }
+            };
+            if (q.dtype == PCX_F32) fetch(float());
+            else if (q.dtype == PCX_BF16) fetch(bf16());
+            else fetch(f16());
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) {
+                const float4 w = ld4(to + 64 * k);
+                x[k] = w.x;
+                x[k + 1] = w.y;
+                x[k + 2] = w.z;
+                x[k + 3] = w.w;
+            }
+            x = tile_apply(v, x, st.a);
+        }
+        if (PHASE != NSL_LAST) {
+#pragma unroll
+            for (int k = 0; k < 16; k += 4) st4(to + 64 * k, make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]));
+            tile_gram(own, x, l32, h, g);
+            continue;
+        }
+        const auto finish = [&](auto kind, auto put) {
+            using T = decltype(kind);
+            T* out = static_cast<T*>(e.out) + (int64_t)bat * e.rows * e.cols;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int r = acc_row(k, h);
+                if (r >= m || c >= n) continue;
+                T* o = out + (int64_t)(tall ? c : r) * e.cols + (tall ? r : c);
+                *o = put(put.old(o), x[k] * unit);
+            }
+        };
+        if (q.is_step) finish(float(), Descend{q.decay, e.step});
+        else if (q.dtype == PCX_F32) finish(float(), Plain<float>());
+        else if (q.dtype == PCX_BF16) finish(bf16(), Plain<bf16>());
+        else finish(f16(), Plain<f16>());
+    }
+    if (PHASE == NSL_LAST) return;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) own[acc_row(k, h) * 33 + l32] = g[k];
+    __syncthreads();
+    float* to = sums(PHASE == NSL_FIRST ? 0 : 1 - st.src);
+    for (int i = threadIdx.x; i < 1024; i += 64 * NSB_WAVES) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < NSB_WAVES; ++w) s += lds[w * NSB_TILE + (i >> 5) * 33 + (i & 31)];
+        to[i] = s;
+    }
+}
+
 // ---------------------------------------------------------------- host
 int round_up(int v, int k) { return (v + k - 1) / k * k; }
 
@@ -1354,6 +1493,14 @@ int ns_in_blocks(const NsTable& t, int* bytes, int* pairs) {
     return kind;
 }
 
+// the launch's matrices are all of at most 32 rows or columns (and too long for blocks of their own)
+bool ns_all_short(const NsTable& t) {
+    for (int i = 0; i < t.count; ++i)
+        if (std::min(t.e[i].rows, t.e[i].cols) > 32) return false;
+    return true;
+}
+int long_tiles(const NsMat& e) { return (std::max(e.rows, e.cols) + 31) / 32; }
+
 // One launch table's workspace: the job, partial sums and unit of every matrix, counters and partial products of split tiles,
 // then the planes.  Fills in the places; returns its size.
 int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
@@ -1365,10 +1512,18 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
     t.mats = (int)mats;
     int bytes, pairs;
     if (ns_in_blocks(t, &bytes, &pairs)) return 256;  // (nothing passes through memory)
-    for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
-        const NsPlan p = ns_plan(t, ph);
-        counters = std::max(counters, p.counters);
-        joint = std::max(joint, p.joint);
+    const bool all_short = ns_all_short(t);
+    if (all_short) {
+        int64_t slices = 0;
+        for (int i = 0; i < t.count; ++i) slices += (int64_t)long_slices(long_tiles(t.e[i])) * t.e[i].batch;
+        q.slices = (int)slices;
+        joint = 2 * slices * 1024;
+    } else {
+        for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
+            const NsPlan p = ns_plan(t, ph);
+            counters = std::max(counters, p.counters);
+            joint = std::max(joint, p.joint);
+        }
     }
     int64_t off = 0;
     const auto take = [&](int64_t bytes) {
@@ -1389,7 +1544,7 @@ int64_t ns_place(NsTable& t, NsArgs& q, void* ws) {
     q.joint = reinterpret_cast<float*>(d);
     for (int i = 0; i < t.count; ++i) {
         t.e[i].ws = off;
-        take(t.e[i].batch * plane_bytes(t.e[i].mp, t.e[i].np));
+        take(t.e[i].batch * (all_short ? (int64_t)long_tiles(t.e[i]) * 4096 : plane_bytes(t.e[i].mp, t.e[i].np)));
     }
     return off;
 }
@@ -1448,6 +1603,21 @@ int ns_run(const NsTable& t, const NsArgs& q, const float* coef, int steps, hipS
         return ns_block_of<4>(kind, t, un, q, c, n, most, s);
     }
     NsJob job{t, q, {}, {}, {}};
+    if (ns_all_short(t)) {
+        const unsigned nn = ns_blocks(t, job.norm, [](const NsMat& e) { return (int64_t)e.parts; });
+        const unsigned n = ns_blocks(t, job.split, [](const NsMat& e) { return (int64_t)long_slices(long_tiles(e)); });
+        ns_norm_kernel<<<nn, 256, 0, s>>>(job);
+        PCX_LAUNCH_CHECK("ns_norm_kernel");
+        ns_long_kernel<NSL_FIRST><<<n, 64 * NSB_WAVES, 0, s>>>(q.ws, NsStep{});
+        PCX_LAUNCH_CHECK("ns_long_kernel");
+        for (int k = 0; k < steps; ++k) {
+            const NsStep st{coef[3 * k], coef[3 * k + 1], coef[3 * k + 2], k & 1};
+            if (k + 1 < steps) ns_long_kernel<NSL_STEP><<<n, 64 * NSB_WAVES, 0, s>>>(q.ws, st);
+            else ns_long_kernel<NSL_LAST><<<n, 64 * NSB_WAVES, 0, s>>>(q.ws, st);
+            PCX_LAUNCH_CHECK("ns_long_kernel");
+        }
+        return PCX_OK;
+    }
     NsPlan plans[4];
     for (int ph = NS_GRAM; ph <= NS_LAST; ++ph) {
         plans[ph] = ns_plan(t, ph);

@@ -213,9 +213,8 @@ def orthogonalize(x, ns_steps=5, ns_coefficients=NS_COEFFICIENTS, eps=1e-7):
     to about 1 by `ns_steps` Newton-Schulz steps: X = x / (|x|_F + eps), then X <- a X + (b A + c A A) X, A = X X^T.
 
     `ns_coefficients`: (a, b, c), or one triple per step.  Computed for every type with sums in float32 and rounded once to
-    x's: in float32 throughout where the short side is at most 32 and the long one 1024, else from operands of 22 bits, whose
-    error is below float32 arithmetic's own from short sides of 40 on and up to twice it below that (1 x 2000: 1.7 times);
-    it stays below 5e-6 for a matrix whose norm is under a hundredth of eps, where float32 arithmetic has 1e-7.
+    x's: in float32 throughout where the short side is at most 32, else from operands of 22 bits, whose error is below float32
+    arithmetic's own (but for a matrix whose norm is under a hundredth of eps: below 5e-6, where float32 arithmetic has 1e-7).
     A zero matrix stays zero, one with a value that is not finite becomes NaN.  Not differentiable (the result
     carries no gradient)."""
     _lib.require_gpu(x, what="orthogonalize")
@@ -287,8 +286,9 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
 
     with k = 0.2 sqrt(max(rows, cols)) (adjust "rms": the size of an Adam update, so that its learning rate and decay
     serve), sqrt(max(1, rows / cols)) ("spectral") or 1 (None).  A weight of more than two axes is the matrix of its
-    first axis against the rest.  Accuracy as in `orthogonalize` (short sides up to 32 in float32 throughout if every matrix
-    of the list is small enough for one block, 128 x 128 or 64 x 512).  All tensors float32, contiguous and on one GPU; no parameter or buffer shares memory
+    first axis against the rest.  Accuracy as in `orthogonalize`, except that short sides up to 32 take operands of 22
+    bits too, with up to twice float32 arithmetic's error, where some matrix of the list neither has one nor is small enough
+    for one block (128 x 128 or 64 x 512).  All tensors float32, contiguous and on one GPU; no parameter or buffer shares memory
     with another tensor of the call (a gradient may appear twice)."""
     params, grads, buffers = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(buffers):
