@@ -116,8 +116,8 @@ int pcx_layernorm_backward(int dtype, int wdtype, int64_t rows, int64_t D, const
 /* ------------------------------------------------------------------ orthogonalised updates
  * Newton-Schulz iteration: X = u / (|u|_F + eps), transposed where it has more rows than columns; then, for each of
  * `steps` triples (a, b, c) of coef (host memory), A = X X^T and X <- a X + (b A + c A A) X.  Products of operands
- * held to 22 bits or more (float32 for matrices of at most 32 rows or columns, in a list if all its matrices are such or small
- * enough for one block each), summed in float32; sums of squares in float64.  Coefficients that take some singular value
+ * held to 22 bits or more (float32 for matrices of at most 32 rows or columns; among others in a list only if all are small
+ * enough for one block, 128 x 128, 64 x 512 or 32 x 1024), summed in float32; sums of squares in float64.  Coefficients that take some singular value
  * in [0, 1] beyond 8 are refused.  The short side is at most 16384, the long one 2^20, a matrix 2^31 values.
  * Deterministic.
  *

@@ -12,8 +12,8 @@
 // hi hi + hi lo + lo hi, exact in each term and summed in float32 (the dropped lo lo is below 2^-24 of the product):
 // three float16 MFMAs for one of float32, 16 / 3 of its rate.  Long sums round more than that (errors of 0.5 to 0.8 of
 // float32 arithmetic's from 40 rows on), short ones less (1.9 times its error at 1 x 50), so matrices of at most 32 rows are
-// in float32: tile_step in one block, ns_long_kernel in many.  (In a list with a matrix that is neither short nor held by a
-// block they go by the planes too: launches of their own would add 7 to its 17.)  S is a power of two that keeps
+// in float32: tile_step in one block, ns_long_kernel in many.  (In a list with others they go by the planes
+// too, unless blocks hold the whole list: launches of their own would add 7 to its 17.)  S is a power of two that keeps
 // hi below 2^15 for the largest singular value the coefficients can reach (the caller's interval bound), so nothing
 // overflows, and a value's lo part leaves float16's normal range only 2^-13 below the largest.  A matrix whose norm is
 // far below eps starts far below 1: its S is larger by the power of two that all steps together cannot grow back

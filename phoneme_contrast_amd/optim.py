@@ -287,8 +287,8 @@ def muon_step(params, grads, momentum_buffers, *, lr, momentum=0.95, nesterov=Tr
     with k = 0.2 sqrt(max(rows, cols)) (adjust "rms": the size of an Adam update, so that its learning rate and decay
     serve), sqrt(max(1, rows / cols)) ("spectral") or 1 (None).  A weight of more than two axes is the matrix of its
     first axis against the rest.  Accuracy as in `orthogonalize`, except that short sides up to 32 take operands of 22
-    bits too, with up to twice float32 arithmetic's error, where some matrix of the list neither has one nor is small enough
-    for one block (128 x 128 or 64 x 512).  All tensors float32, contiguous and on one GPU; no parameter or buffer shares memory
+    bits too, with up to twice float32 arithmetic's error, in a list with others (each 16 in order count) unless all are small
+    enough for one block (128 x 128, 64 x 512, 32 x 1024).  All tensors float32, contiguous and on one GPU; no parameter or buffer shares memory
     with another tensor of the call (a gradient may appear twice)."""
     params, grads, buffers = list(params), list(grads), list(momentum_buffers)
     if not len(params) == len(grads) == len(buffers):

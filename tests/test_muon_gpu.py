@@ -578,7 +578,7 @@ def test_short_sides_are_as_exact_as_float32():
 
 
 def test_short_sides_among_the_products():
-    """In a list with a matrix that is neither short nor held by a block, operands have 22 bits: twice the float32
+    """In a list with others that blocks do not hold, operands have 22 bits: twice the float32
     iteration's error where sums are short, with the 22 % that two rms of 20 draws may be off; long ones alone have not."""
     from phoneme_contrast_amd.optim import orthogonalize
     shapes = [(1, 2000), (3, 2000), (20, 1500), (32, 1100)]
