@@ -28,8 +28,8 @@
 // swizzled in LDS 4059 us at a later step, 3948 as it is now.)
 // A and B are symmetric: only tiles on and below the diagonal are computed, and written twice.
 //
-// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.67 to 4.06 ms (one card and
-// another), 0.51 to 0.56 PFLOP/s of the three products' definition and 1.02 to 1.12 executed (three terms, half of the
+// What bounds it.  Large matrices: the MFMA rate.  4096 x 4096 in bfloat16, five steps: 3.64 to 4.06 ms (one card and
+// another), 0.51 to 0.57 PFLOP/s of the three products' definition and 1.02 to 1.12 executed (three terms, half of the
 // tiles of A and B), where a float16 product of the library reaches 1.08 at that size.  Of a few hundred tiles: LDS, which
 // feeds the MFMAs of 64 x 64 tiles at half their rate, the traffic from L2, and a launch's fixed parts (addresses, first
 // stages, the epilogue's passes).  Small ones: those fixed parts, 5 to 8 us a launch of which 2 to 3 compute.
